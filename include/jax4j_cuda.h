@@ -640,6 +640,35 @@ J4C_API int j4c_psum_sgd(const float *const *grads, const float *const *upd, uin
                          int rank, int64_t n, int nsegs, const int64_t *seg_len, const float *const *params,
                          float scale, float lr, float *stage, float *out, j4c_stream stream);
 
+/* ---- AdamW over many tensors (no counterpart in the reference) ----
+ * For every element of tensor i, with g' = g * scale:
+ *   m' = beta1 m + (1 - beta1) g',  v' = beta2 v + (1 - beta2) g'^2,
+ *   w' = w - lr wd[i] w - lr (m' / (1 - beta1^t)) / (sqrt(v' / (1 - beta2^t)) + eps)
+ * in the tensors' dtype, each product and sum rounded on its own; t counts
+ * this step.  numel, w, g, state, w_out, state_out and weight_decay are HOST
+ * arrays, read before the call returns.  steps is a device array of three
+ * doubles: the steps taken, beta1 and beta2 to that power (0, 1, 1 before the
+ * first step); steps_out, another such array (or NULL), gets theirs after this
+ * one.  lr_dev, a device float, replaces lr unless it is NULL.
+ * state_bits 32: state[2 i] and state[2 i + 1] are m and v in the tensors'
+ * dtype.  state_bits 8 (FLOAT32 tensors): state[i] is the packed state of the
+ * tensor, j4c_adamw_q8_words(numel[i]) 32-bit words, all zero before the
+ * first step: per block of 128 elements 128 e4m3 codes of m, 128 unsigned
+ * codes (4 exponent bits, 4 fraction bits) of sqrt(v) and one FLOAT32 step
+ * each, a value being its code times its step; first all codes of m, then of
+ * sqrt(v), then the steps of m, then of sqrt(v).  A moment that is not finite
+ * is held as NaN; the update uses the moments before they are rounded.
+ * Outputs may be the inputs of the same index (an update in place), else must
+ * not overlap them.  Tensors of no elements may have NULL pointers. */
+J4C_API int64_t j4c_adamw_q8_words(int64_t n);
+J4C_API int j4c_adamw_step(int dtype, int state_bits, int ntensors, const int64_t *numel, const void *const *w,
+                           const void *const *g, const void *const *state, void *const *w_out, void *const *state_out,
+                           const double *weight_decay, const double *steps, double *steps_out, const float *lr_dev,
+                           double lr, double scale, double beta1, double beta2, double eps, j4c_stream stream);
+/* The FLOAT32 values m and v of packed states. */
+J4C_API int j4c_adamw_moments(int ntensors, const int64_t *numel, const void *const *state, float *const *m_out,
+                              float *const *v_out, j4c_stream stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -215,6 +215,14 @@ public final class J4C {
         JAVA_INT, ADDRESS, ADDRESS, ADDRESS, JAVA_INT, JAVA_INT, JAVA_LONG, JAVA_INT, ADDRESS, ADDRESS,
         JAVA_FLOAT, JAVA_FLOAT, ADDRESS, ADDRESS, ADDRESS));
 
+    // ---- AdamW over many tensors (adamw.cu) ----
+    static final MethodHandle ADAMW_Q8_WORDS = h("j4c_adamw_q8_words", FunctionDescriptor.of(JAVA_LONG, JAVA_LONG));
+    static final MethodHandle ADAMW_STEP = h("j4c_adamw_step", FunctionDescriptor.of(
+        JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, ADDRESS, ADDRESS, ADDRESS, ADDRESS, ADDRESS, ADDRESS, ADDRESS, ADDRESS,
+        ADDRESS, ADDRESS, JAVA_DOUBLE, JAVA_DOUBLE, JAVA_DOUBLE, JAVA_DOUBLE, JAVA_DOUBLE, ADDRESS));
+    static final MethodHandle ADAMW_MOMENTS = h("j4c_adamw_moments", FunctionDescriptor.of(
+        JAVA_INT, JAVA_INT, ADDRESS, ADDRESS, ADDRESS, ADDRESS, ADDRESS));
+
     /** The library's message for the last failed call on this thread. */
     public static String lastError() {
         try {

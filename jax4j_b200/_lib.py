@@ -125,10 +125,14 @@ SIGNATURES = {
     "j4c_psum_sgd_flag_bytes": [],
     "j4c_psum_sgd": [C.POINTER(P), C.POINTER(P), C.POINTER(P), I32, I32, I64, I32, C.POINTER(I64), C.POINTER(P),
                      C.c_float, C.c_float, P, P, P],
+    "j4c_adamw_q8_words": [I64],
+    "j4c_adamw_step": [I32, I32, I32, P, P, P, P, P, P, P, P, P, P, C.c_double, C.c_double, C.c_double, C.c_double,
+                       C.c_double, P],
+    "j4c_adamw_moments": [I32, P, P, P, P, P],
 }
 _RESTYPES = {"j4c_last_error": C.c_char_p, "j4c_dot_workspace_size": C.c_size_t,
              "j4c_split_pitch": C.c_int64, "j4c_split_floats": C.c_int64,
-             "j4c_psum_sgd_flag_bytes": C.c_size_t}
+             "j4c_psum_sgd_flag_bytes": C.c_size_t, "j4c_adamw_q8_words": C.c_int64}
 
 
 def lib() -> C.CDLL:

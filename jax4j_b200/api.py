@@ -407,6 +407,20 @@ class Lax:
                                           for w, g in zip(pl, summed)])
 
 
+    @staticmethod
+    def psumAdamWTree(params: PyTree, grads: PyTree, state, lr, scale: float = 1.0, **hyper):
+        """The AdamW update of a data-parallel step with its gradient
+        all-reduce: Optim.adamW of psumTree(grads), with scale = 1/D for the
+        mean gradient; `hyper` are Optim.adamW's other arguments.  Every shard
+        holds the same summed gradients, so every shard computes the same new
+        parameters and state.  Returns (new parameters, new state)."""
+        from .optim import Optim
+        pl, gl = PyTrees.flatten(params), PyTrees.flatten(grads)
+        if len(pl) != len(gl):
+            raise IllegalArgumentException(f"psumAdamWTree: {len(pl)} parameters but {len(gl)} gradients")
+        return Optim.adamW(params, Lax.psumTree(grads), state, lr, scale=scale, **hyper)
+
+
 # Gradient all-reduce overlapped with the backward pass.  The backward records
 # a CUDA event on each gradient when it is complete; psumTree groups the leaves
 # into buckets (last leaves first, the order the backward completes them) and

@@ -91,26 +91,22 @@ class DType(enum.Enum):
     INT64 = (3, 8, "int64")
     BOOL = (4, 1, "bool")
 
-    @property
-    def ordinal(self) -> int:
-        return self.value[0]
+    def __init__(self, ordinal: int, size: int, text: str):
+        # plain attributes (torch and numpy dtypes set below): an enum
+        # member's hash and value are Python calls, and every array made asks
+        self.ordinal = ordinal
+        self._size = size
+        self._text = text
+        self._floating = text.startswith("float")
 
     def byteSize(self) -> int:
-        return self.value[1]
+        return self._size
 
     def __str__(self):
-        return self.value[2]
-
-    @property
-    def torch(self) -> torch.dtype:
-        return _TORCH[self]
-
-    @property
-    def numpy(self):
-        return _NUMPY[self]
+        return self._text
 
     def is_floating(self) -> bool:
-        return self in (DType.FLOAT32, DType.FLOAT64)
+        return self._floating
 
     @staticmethod
     def promote(d1: "DType", d2: "DType") -> "DType":
@@ -136,6 +132,9 @@ _TORCH = {DType.FLOAT32: torch.float32, DType.FLOAT64: torch.float64, DType.INT3
           DType.INT64: torch.int64, DType.BOOL: torch.uint8}
 _NUMPY = {DType.FLOAT32: np.float32, DType.FLOAT64: np.float64, DType.INT32: np.int32,
           DType.INT64: np.int64, DType.BOOL: np.bool_}
+for _d in DType:
+    _d.torch, _d.numpy = _TORCH[_d], _NUMPY[_d]
+_OF_TORCH = {v: k for k, v in _TORCH.items()} | {torch.bool: DType.BOOL}
 
 
 # ---------------------------------------------------------------------------
@@ -146,8 +145,8 @@ class Shape:
 
     def __init__(self, *dims):
         if len(dims) == 1 and isinstance(dims[0], (list, tuple)):
-            dims = tuple(dims[0])
-        self._d = tuple(int(d) for d in dims)
+            dims = dims[0]
+        self._d = tuple(map(int, dims))
 
     def dimensions(self) -> tuple:
         return self._d
@@ -269,9 +268,9 @@ class Device:
     @classmethod
     def defaultDevice(cls) -> "Device":
         """core/Device.java:82-99: prefers a GPU; here a GPU is required."""
-        with cls._lock:
-            if cls._default is not None:
-                return cls._default
+        d = cls._default  # one reference, set once: read without the lock
+        if d is not None:
+            return d
         d = cls.cuda(cls._default_ordinal)
         with cls._lock:
             cls._default = d
@@ -394,9 +393,10 @@ class ConcreteNDArray(NDArray):
             t = data
             if dtype is None:
                 dtype = _from_torch(t.dtype)
-            if t.dtype != dtype.torch or t.device.type != "cuda" or t.device.index != device.ordinal():
+            if t.dtype is not dtype.torch or not t.is_cuda or t.get_device() != device.ordinal():
                 t = t.to(device=device.torch_device(), dtype=dtype.torch)
-            t = t.reshape(-1)
+            if t.dim() != 1:
+                t = t.reshape(-1)
             if not t.is_contiguous():
                 t = t.contiguous()
         else:
@@ -726,12 +726,10 @@ class ConcreteNDArray(NDArray):
 
 
 def _from_torch(dt: torch.dtype) -> DType:
-    for k, v in _TORCH.items():
-        if v == dt:
-            return k
-    if dt == torch.bool:
-        return DType.BOOL
-    raise IllegalArgumentException(f"unsupported tensor dtype {dt}")
+    k = _OF_TORCH.get(dt)
+    if k is None:
+        raise IllegalArgumentException(f"unsupported tensor dtype {dt}")
+    return k
 
 
 def _dtype_of_numpy(arr: np.ndarray) -> DType:
