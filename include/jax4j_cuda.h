@@ -669,6 +669,35 @@ J4C_API int j4c_adamw_step(int dtype, int state_bits, int ntensors, const int64_
 J4C_API int j4c_adamw_moments(int ntensors, const int64_t *numel, const void *const *state, float *const *m_out,
                               float *const *v_out, j4c_stream stream);
 
+/* ---- layers with an activation (no counterpart in the reference) ----
+ * relu keeps Java's Math.max(0, x); silu(u) = u sigmoid(u); gelu is the tanh
+ * form, u/2 (1 + tanh(sqrt(2/pi) (u + 0.044715 u^3))). */
+#define J4C_ACT_NONE 0
+#define J4C_ACT_RELU 1
+#define J4C_ACT_TANH 2
+#define J4C_ACT_SIGMOID 3
+#define J4C_ACT_SILU 4
+#define J4C_ACT_GELU 5
+
+/* Group norm over x [B, S, C], channels last (B samples of S positions), in
+ * `groups` groups of neighbouring channels, FLOAT32 or FLOAT64:
+ *   y = act(gamma[c] (x - mean) rstd + beta[c]),  rstd = 1 / sqrt(var + eps)
+ * with mean and (biased) variance over the S * C / groups values of a sample's
+ * group.  gamma and beta ([C]) may each be NULL (1 and 0).  mean and rstd
+ * ([B, groups], both or neither NULL) are kept for the gradient.  y may be x.
+ * ws: j4c_group_norm_workspace(..., 0) bytes, 16-byte aligned (NULL when 0),
+ * free again when the call's work is done. */
+J4C_API size_t j4c_group_norm_workspace(int dtype, int64_t B, int64_t S, int64_t C, int64_t groups, int backward);
+J4C_API int j4c_group_norm(int dtype, int64_t B, int64_t S, int64_t C, int64_t groups, const void *x,
+                           const void *gamma, const void *beta, double eps, int act, void *y, void *mean, void *rstd,
+                           void *ws, size_t ws_bytes, j4c_stream stream);
+/* Its gradient: dx [B, S, C] (may be dy or x), dgamma and dbeta [C] (each may
+ * be NULL: not wanted).  ws: j4c_group_norm_workspace(..., 1) bytes. */
+J4C_API int j4c_group_norm_grad(int dtype, int64_t B, int64_t S, int64_t C, int64_t groups, const void *x,
+                                const void *gamma, const void *beta, int act, const void *mean, const void *rstd,
+                                const void *dy, void *dx, void *dgamma, void *dbeta, void *ws, size_t ws_bytes,
+                                j4c_stream stream);
+
 #ifdef __cplusplus
 }
 #endif

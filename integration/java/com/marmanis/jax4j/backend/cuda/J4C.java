@@ -223,6 +223,16 @@ public final class J4C {
     static final MethodHandle ADAMW_MOMENTS = h("j4c_adamw_moments", FunctionDescriptor.of(
         JAVA_INT, JAVA_INT, ADDRESS, ADDRESS, ADDRESS, ADDRESS, ADDRESS));
 
+    // ---- group norm with an activation (group_norm.cu) ----
+    static final MethodHandle GROUP_NORM_WORKSPACE = h("j4c_group_norm_workspace", FunctionDescriptor.of(
+        JAVA_LONG, JAVA_INT, JAVA_LONG, JAVA_LONG, JAVA_LONG, JAVA_LONG, JAVA_INT));
+    static final MethodHandle GROUP_NORM = h("j4c_group_norm", FunctionDescriptor.of(
+        JAVA_INT, JAVA_INT, JAVA_LONG, JAVA_LONG, JAVA_LONG, JAVA_LONG, ADDRESS, ADDRESS, ADDRESS, JAVA_DOUBLE, JAVA_INT,
+        ADDRESS, ADDRESS, ADDRESS, ADDRESS, JAVA_LONG, ADDRESS));
+    static final MethodHandle GROUP_NORM_GRAD = h("j4c_group_norm_grad", FunctionDescriptor.of(
+        JAVA_INT, JAVA_INT, JAVA_LONG, JAVA_LONG, JAVA_LONG, JAVA_LONG, ADDRESS, ADDRESS, ADDRESS, JAVA_INT, ADDRESS,
+        ADDRESS, ADDRESS, ADDRESS, ADDRESS, ADDRESS, ADDRESS, JAVA_LONG, ADDRESS));
+
     /** The library's message for the last failed call on this thread. */
     public static String lastError() {
         try {

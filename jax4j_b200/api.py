@@ -19,6 +19,7 @@ import numpy as np
 import torch
 
 from . import grad as _grad
+from . import layers as _layers
 from . import pmap as _pm
 from ._lib import call, dims as _dims
 from .core import (ConcreteNDArray, Device, DType, IllegalArgumentException, NDArray, PRNGKey,
@@ -43,6 +44,14 @@ class JAX:
         jaxpr = _grad.make_jaxpr(fn, arg)
         primals, tangents = _grad.forward_ad(jaxpr, [arg], [tangent])
         return [primals[0], tangents[0]]
+
+    @staticmethod
+    def vjp(fn: Callable, *args: NDArray):
+        """(fn(*args), pullback): one forward pass, and the function that takes
+        a cotangent of every output to the cotangents of the arguments (a
+        list).  The backward half of value_and_grad (JAX.java:243-245) for any
+        output and any cotangent; the pullback may be called again."""
+        return _grad.vjp(fn, *args)
 
     @staticmethod
     def grad(fn: Callable, argnum: int = None) -> Callable:
@@ -530,6 +539,17 @@ class Nn:
         as in the reference."""
         e = x.exp()
         return e.div(e.sum(-1, True))
+
+    @staticmethod
+    def groupNorm(x: NDArray, groups: int, gamma: Optional[NDArray] = None, beta: Optional[NDArray] = None,
+                  eps: float = 1e-5, activation: str = "none") -> NDArray:
+        """act(gamma * xhat + beta) with xhat = (x - mean) / sqrt(var + eps)
+        over each sample's groups of neighbouring channels; x is [batch, ...,
+        channels], channels last, FLOAT32 or FLOAT64 (groups = 1 over
+        [batch, channels] is layer norm), gamma and beta [channels].  One
+        operation, differentiable in x, gamma and beta.  activation: "none",
+        "relu", "tanh", "sigmoid", "silu" or "gelu" (the tanh form)."""
+        return _layers.group_norm(x, groups, gamma, beta, eps, activation)
 
 
 def _dropout(x: NDArray, key: PRNGKey, rate: float, training: bool) -> NDArray:

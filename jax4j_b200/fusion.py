@@ -46,7 +46,7 @@ OP_CONST = -2
 _VJP_READS = {
     P.MUL: ("in",), P.DIV: ("in",), P.EXP: ("out",), P.LOG: ("in",), P.SIN: ("in",),
     P.COS: ("in",), P.TANH: ("out",), P.RELU: ("out",), P.SIGMOID: ("out",), P.DOT: ("in",),
-    P.MAX: ("in",), P.MIN: ("in",), P.COND: ("in",), P.SCAN: ("in",),
+    P.MAX: ("in",), P.MIN: ("in",), P.COND: ("in",), P.SCAN: ("in",), P.FFI_CALL: ("in", "out"),
 }
 
 

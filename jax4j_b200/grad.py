@@ -235,13 +235,16 @@ def _evaluate(jaxpr: Jaxpr, args: List[NDArray], keep_for_vjp: bool) -> Dict[int
         raise IllegalArgumentException(f"expected {len(jaxpr.inVars)} arguments, got {len(args)}")
     for v, a in zip(jaxpr.inVars, args):
         values[v.id] = a
+    if len(jaxpr.equations) == 1 and jaxpr.equations[0].primitive == Primitive.FFI_CALL:
+        _run_equation(jaxpr.equations[0], values, keep_for_vjp)  # one layer: nothing to plan
+        return values
     if FUSION and all(isinstance(a, ConcreteNDArray) for a in values.values()):
         from . import fusion
         for kind, item in fusion.plan_for(jaxpr, keep_for_vjp).steps:
             if kind == "eq":
                 if keep_for_vjp and item.primitive == Primitive.DOT:
                     _presplit_dot(jaxpr, item, values)
-                _run_equation(item, values)
+                _run_equation(item, values, keep_for_vjp)
             elif kind == "dot_ep":
                 if keep_for_vjp:
                     _presplit_dot(jaxpr, item.dot, values)
@@ -252,12 +255,18 @@ def _evaluate(jaxpr: Jaxpr, args: List[NDArray], keep_for_vjp: bool) -> Dict[int
     for eq in jaxpr.equations:
         if keep_for_vjp and eq.primitive == Primitive.DOT:
             _presplit_dot(jaxpr, eq, values)
-        _run_equation(eq, values)
+        _run_equation(eq, values, keep_for_vjp)
     return values
 
 
-def _run_equation(eq, values: Dict[int, NDArray]) -> None:
+def _run_equation(eq, values: Dict[int, NDArray], keep_for_vjp: bool = False) -> None:
     inputs = [values[v.id] for v in eq.inputs]
+    if eq.primitive == Primitive.FFI_CALL:
+        out = eq.outputs[0].id
+        values[out], saved = eq.metadata.forward(inputs, keep_for_vjp)
+        if saved is not None:
+            values[~out] = saved  # for its VJP, under an id no Var has
+        return
     if eq.primitive == Primitive.SCAN:  # the one two-output primitive
         carry, ys = scan_forward(eq, inputs)
         values[eq.outputs[0].id] = carry
@@ -308,6 +317,8 @@ def forward_ad(jaxpr: Jaxpr, args: List[NDArray], tangents_in: List[NDArray]):
         primals[v.id] = a
         tangents[v.id] = t
     for eq in jaxpr.equations:
+        if eq.primitive == Primitive.FFI_CALL:
+            raise UnsupportedOperationException(f"{eq.metadata.name} is not forward-mode differentiable")
         ins = [primals[v.id] for v in eq.inputs]
         tins = [tangents[v.id] for v in eq.inputs]
         if eq.primitive == Primitive.SCAN:
@@ -586,7 +597,10 @@ def _process_backward_eq(eq, values, grads, need, fused_relu) -> None:
             return
     inputs = [values.get(v.id) for v in eq.inputs]
     out_value = values.get(eq.outputs[0].id)
-    g_ins = compute_vjps(eq.primitive, eq, g_out, inputs, out_value, wanted)
+    if eq.primitive == Primitive.FFI_CALL:
+        g_ins = eq.metadata.vjp(inputs, out_value, values.get(~eq.outputs[0].id), materialize(g_out), wanted)
+    else:
+        g_ins = compute_vjps(eq.primitive, eq, g_out, inputs, out_value, wanted)
     for v, w, g in zip(eq.inputs, wanted, g_ins):
         if w and g is not None:
             _merge(grads, v.id, g)
@@ -651,6 +665,8 @@ def execute_primitive(p: Primitive, eq, inputs: List[NDArray]) -> NDArray:
     if p == Primitive.CHECKPOINT:
         m: CheckpointMeta = eq.metadata
         return forward_interpret(m.subJaxpr, [inputs[0]])[0]
+    if p == Primitive.FFI_CALL:
+        return eq.metadata.forward(inputs, False)[0]
     raise UnsupportedOperationException(str(p))
 
 
@@ -830,6 +846,26 @@ def grad_both(fn: Callable) -> Callable:
     def g(a0, a1):
         return _backward(make_jaxpr(fn, a0, a1), [a0, a1])
     return g
+
+
+def vjp(fn: Callable, *args: NDArray):
+    """JAX.vjp: (fn(*args), pullback)."""
+    if Tracer.current() is not None:
+        raise UnsupportedOperationException("JAX.vjp inside a trace")
+    jaxpr = make_jaxpr(fn, *args)
+    values = fill_forward_values(jaxpr, list(args))
+    outs = [values[v.id] for v in jaxpr.outVars]
+
+    def pullback(*seeds: NDArray) -> List[NDArray]:
+        if len(seeds) != len(outs):
+            raise IllegalArgumentException(f"pullback: {len(outs)} outputs take as many cotangents, got {len(seeds)}")
+        for s, v in zip(seeds, jaxpr.outVars):
+            if s.shape() != v.shape or s.dtype() != _float_or_default(v.dtype):
+                raise IllegalArgumentException(f"pullback: cotangent {s.shape()} {s.dtype()} of an output {v.shape} "
+                                               f"{v.dtype}")
+        return do_backward(jaxpr, values, list(seeds))
+
+    return (tuple(outs) if jaxpr.__dict__.get("_tuple_out") else outs[0]), pullback
 
 
 def _trace_tree(fn: Callable, tree, leaves: List[NDArray]) -> Jaxpr:

@@ -68,6 +68,32 @@ class ScanMeta:
     stepFn: "Jaxpr"
 
 
+class FfiMeta:
+    """An FFI_CALL's function and its VJP (the pair api/FFI.java:17-31
+    registers by name).  Instances hold parameters, never arrays.
+
+    forward(inputs, keep) -> (output, saved): saved is what vjp needs beside
+    the inputs and the output, made only where keep is true.
+    vjp(inputs, output, saved, g, wanted) -> one cotangent per input (None
+    where wanted is false).
+    batch(inputs, batched, batch): the function over a leading axis of the
+    batched inputs (JAX.vmap)."""
+
+    name = "?"
+
+    def forward(self, inputs, keep):
+        raise NotImplementedError
+
+    def vjp(self, inputs, out, saved, g, wanted):
+        raise NotImplementedError
+
+    def batch(self, inputs, batched, batch):
+        raise UnsupportedOperationException(f"vmap has no batching rule for {self.name}")
+
+    def __repr__(self):
+        return self.name + "(" + ", ".join(f"{k}={v}" for k, v in vars(self).items()) + ")"
+
+
 @dataclass
 class Equation:
     inputs: List[Var]

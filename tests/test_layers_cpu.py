@@ -1,0 +1,72 @@
+"""What the fused layers and their C entries refuse before anything reaches a
+GPU, and how they are traced."""
+import ctypes as C
+
+import pytest
+import torch
+
+import jax4j_b200 as J
+from jax4j_b200 import _lib
+from jax4j_b200.layers import ACTIVATIONS
+
+
+def leaf(*shape, dtype=J.DType.FLOAT32):
+    s = J.Shape(*shape)
+    return J.ConcreteNDArray._wrap(torch.zeros(s.size(), dtype=dtype.torch), s, dtype, J.Device(None))
+
+
+def test_activation_codes_match_the_header():
+    import os
+    import re
+    src = open(os.path.join(os.path.dirname(_lib.__file__), "..", "include", "jax4j_cuda.h")).read()
+    codes = {m.group(1).lower(): int(m.group(2)) for m in re.finditer(r"#define J4C_ACT_(\w+) (\d)", src)}
+    assert codes == ACTIVATIONS
+
+
+def test_group_norm_refusals():
+    bad = J.IllegalArgumentException
+    x = leaf(2, 3, 8)
+    for args, text in (((x, 3), "do not divide"), ((x, 0), "do not divide"), ((x, -2), "do not divide"),
+                       ((leaf(8), 2), "batch"), ((leaf(2, 0), 1), "do not divide"),
+                       ((x, 2, leaf(4)), "gamma is"), ((x, 2, None, leaf(1, 8)), "beta is"),
+                       ((leaf(2, 8, dtype=J.DType.INT32), 2), "FLOAT32 or FLOAT64"),
+                       ((x, 2, leaf(8, dtype=J.DType.FLOAT64)), "one floating dtype")):
+        with pytest.raises(bad, match=text):
+            J.Nn.groupNorm(*args)
+    with pytest.raises(bad, match="activation"):
+        J.Nn.groupNorm(x, 2, activation="swish")
+    for eps in (-1e-5, float("nan")):
+        with pytest.raises(bad, match="eps"):
+            J.Nn.groupNorm(x, 2, eps=eps)
+
+
+def test_layers_are_one_equation():
+    jaxpr = J.JAX.make_jaxpr(lambda a: J.Nn.groupNorm(a, 2, leaf(8), activation="silu").tanh(), leaf(2, 3, 8))
+    kinds = [e.primitive for e in jaxpr.equations]
+    assert kinds == [J.Primitive.FFI_CALL, J.Primitive.TANH]
+    assert jaxpr.outVars[0].shape == J.Shape(2, 3, 8)
+    assert "group_norm(groups=2" in repr(jaxpr)
+    with pytest.raises(J.UnsupportedOperationException, match="inside a trace"):
+        J.JAX.make_jaxpr(lambda a: J.JAX.vjp(lambda b: b, a)[0], leaf(3))
+
+
+def test_c_entries_refuse_bad_arguments():
+    L = _lib.lib()
+    fake = C.c_void_p(0x1000)
+
+    def norm(dtype=0, B=2, S=3, c=8, G=2, x=fake, eps=1e-5, act=0, y=fake, mean=None, rstd=None):
+        rc = L.j4c_group_norm(dtype, B, S, c, G, x, None, None, eps, act, y, mean, rstd, None, 0, None)
+        return rc, L.j4c_last_error().decode()
+
+    for kw, text in ((dict(dtype=2), "FLOAT32 or FLOAT64"), (dict(B=-1), "bad extents"), (dict(c=0), "bad extents"),
+                     (dict(G=3), "do not divide"), (dict(G=0), "do not divide"), (dict(eps=-1.0), "eps"),
+                     (dict(eps=float("nan")), "eps"), (dict(act=6), "activation"), (dict(act=-1), "activation"),
+                     (dict(x=None), "NULL"), (dict(y=None), "NULL"), (dict(mean=fake), "go together"),
+                     (dict(S=1 << 31), "not supported"), (dict(S=100000), "workspace")):
+        rc, msg = norm(**kw)
+        assert rc == _lib.E_INVALID and text in msg, (kw, rc, msg)
+    assert norm(B=0)[0] == _lib.OK
+    rc = L.j4c_group_norm_grad(0, 2, 3, 8, 2, fake, None, None, 0, fake, fake, fake, fake, None, None, None, 0, None)
+    assert rc == _lib.E_INVALID and "workspace" in L.j4c_last_error().decode()
+    rc = L.j4c_group_norm_grad(0, 2, 3, 8, 2, fake, None, None, 0, fake, None, fake, fake, None, None, fake, 1 << 20, None)
+    assert rc == _lib.E_INVALID and "NULL" in L.j4c_last_error().decode()
