@@ -29,40 +29,71 @@ __device__ __forceinline__ T gelu_arg_slope(T u) {
     return T(1.5957691216057308) * (T(1) + T(0.134145) * u * u);
 }
 
-template <typename T>
-__device__ __forceinline__ T act_value(int act, T u) {
+// u[i] <- act(u[i]) for N values: one branch on the activation for all of them.
+template <typename T, int N>
+__device__ __forceinline__ void act_values(int act, T (&u)[N]) {
     switch (act) {
-    case J4C_ACT_RELU: return T(0) >= u ? T(0) : u;  // NaN stays
-    case J4C_ACT_TANH: return act_tanh(u);
-    case J4C_ACT_SIGMOID: return act_sigmoid(u);
-    case J4C_ACT_SILU: return u * act_sigmoid(u);
-    case J4C_ACT_GELU: return u * act_sigmoid(gelu_arg(u));
-    default: return u;
+    case J4C_ACT_RELU:
+#pragma unroll
+        for (int i = 0; i < N; i++) u[i] = T(0) >= u[i] ? T(0) : u[i];  // NaN stays
+        break;
+    case J4C_ACT_TANH:
+#pragma unroll
+        for (int i = 0; i < N; i++) u[i] = act_tanh(u[i]);
+        break;
+    case J4C_ACT_SIGMOID:
+#pragma unroll
+        for (int i = 0; i < N; i++) u[i] = act_sigmoid(u[i]);
+        break;
+    case J4C_ACT_SILU:
+#pragma unroll
+        for (int i = 0; i < N; i++) u[i] = u[i] * act_sigmoid(u[i]);
+        break;
+    case J4C_ACT_GELU:
+#pragma unroll
+        for (int i = 0; i < N; i++) u[i] = u[i] * act_sigmoid(gelu_arg(u[i]));
+        break;
+    default: break;
     }
 }
 
-// The derivative at the pre-activation u.
-template <typename T>
-__device__ __forceinline__ T act_slope(int act, T u) {
+// d[i] <- d[i] act'(u[i]), the derivative at the pre-activation u[i].
+template <typename T, int N>
+__device__ __forceinline__ void act_slopes(int act, const T (&u)[N], T (&d)[N]) {
     switch (act) {
-    case J4C_ACT_RELU: return u > T(0) ? T(1) : T(0);
-    case J4C_ACT_TANH: {
-        const T t = act_tanh(u);
-        return T(1) - t * t;
-    }
-    case J4C_ACT_SIGMOID: {
-        const T s = act_sigmoid(u);
-        return s * (T(1) - s);
-    }
-    case J4C_ACT_SILU: {
-        const T s = act_sigmoid(u);
-        return s + u * (s * (T(1) - s));
-    }
-    case J4C_ACT_GELU: {
-        const T s = act_sigmoid(gelu_arg(u)), q = s * (T(1) - s);
-        return q == T(0) ? s : s + u * q * gelu_arg_slope(u);  // q = 0: far out, where a' may overflow
-    }
-    default: return T(1);
+    case J4C_ACT_RELU:
+#pragma unroll
+        for (int i = 0; i < N; i++) d[i] = u[i] > T(0) ? d[i] : T(0);  // Grad.reluGrad (api/Grad.java:593-597)
+        break;
+    case J4C_ACT_TANH:
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const T t = act_tanh(u[i]);
+            d[i] *= T(1) - t * t;
+        }
+        break;
+    case J4C_ACT_SIGMOID:
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const T s = act_sigmoid(u[i]);
+            d[i] *= s * (T(1) - s);
+        }
+        break;
+    case J4C_ACT_SILU:
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const T s = act_sigmoid(u[i]);
+            d[i] *= s + u[i] * (s * (T(1) - s));
+        }
+        break;
+    case J4C_ACT_GELU:
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const T s = act_sigmoid(gelu_arg(u[i])), q = s * (T(1) - s);
+            d[i] *= q == T(0) ? s : s + u[i] * q * gelu_arg_slope(u[i]);  // q = 0: far out, where a' may overflow
+        }
+        break;
+    default: break;
     }
 }
 

@@ -16,14 +16,16 @@
 // dy in, dx out backward (12 B).  Two forms:
 //  * Groups of at most 8192 values (rows of features are S = 1, G = 1: layer
 //    norm) are held in registers, eight values a thread, by 1 to 32 warps:
-//    every value is read once.  Backward a warp set keeps its group and walks
-//    over samples, so dgamma and dbeta gather in registers too.
-//  * Larger groups are cut into tiles of rows.  Forward, one kernel reads a
-//    tile into shared memory and leaves its mean and squared differences per
-//    group; a second one merges the tiles' (Chan, Golub and LeVeque's pairwise
-//    update, in FP64) and applies.  Backward the same with per-channel sums of
-//    du and du xhat.  The second read of a tile comes from L2: the batch is
-//    walked in parts of at most kL2Part bytes.
+//    every value is read once, and while a group is worked on the thread's
+//    values of the next one are on their way to shared memory (cp.async).
+//    Backward a warp set keeps its group and walks over samples, so dgamma and
+//    dbeta gather in registers too.
+//  * Larger groups are cut into tiles of rows.  Forward, one kernel leaves every
+//    tile's mean and squared differences per group -- of a thread's batch of
+//    values from registers, merged by Chan, Golub and LeVeque's pairwise update,
+//    so one read is enough; a second one merges the tiles' in FP64 and applies.
+//    Backward the same with the tiles' sums of h and h xhat.  The second read
+//    of a tile comes from L2: the batch is walked in parts of kL2Part bytes.
 #include <algorithm>
 #include <type_traits>
 
@@ -35,8 +37,7 @@ namespace {
 
 constexpr int kHeld = 8;             // values a thread holds
 constexpr int64_t kMaxHeld = 32 * 32 * kHeld;
-constexpr int kTileThreads = 256;
-constexpr int kTileBytes = 48 * 1024;
+constexpr int kTileThreads = 512;    // at most: a tile's CTA has whole rows of columns
 constexpr int kTileChannels = 2048;  // channels of a tile at most
 constexpr int64_t kL2Part = 40ll << 20;
 
@@ -55,6 +56,20 @@ struct Args {
     T *y;   // y or dx
     T *dpart;  // per-channel sums of du, then of du xhat: see the kernels
 };
+
+// An asynchronous copy of 4, 8 or 16 bytes to shared memory.
+template <typename V>
+__device__ __forceinline__ void copy_async(V *to, const V *from) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from),
+                 "n"(sizeof(V))
+                 : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// All but the last LEFT committed groups have arrived.
+template <int LEFT>
+__device__ __forceinline__ void copies_done() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+}
 
 template <typename T>
 __device__ __forceinline__ T warp_sum(T v) {
@@ -109,39 +124,96 @@ struct Place {
     }
 };
 
+// A thread's slots in shared memory for its values of an item: slot i of
+// thread t at i * blockDim + t.  Nobody else touches them.  Two sets of slots
+// take turns: the copies of the next item start before the current one is
+// read, into the set whose values the item before has used up.  FLOAT64
+// backward has room for one set only, and no item ahead.
+template <typename T, bool BACKWARD>
+constexpr int kAhead = sizeof(T) == 8 && BACKWARD ? 0 : 1;
+template <typename T, int V, int WARPS, int NV>
+__device__ __forceinline__ void fetch(Vec<T, V> *slots, const T *from, const Place<V, WARPS, NV> &at) {
+#pragma unroll
+    for (int i = 0; i < NV; i++)
+        if (at.col[i] >= 0)
+            copy_async(slots + i * blockDim.x + threadIdx.x, reinterpret_cast<const Vec<T, V> *>(from + at.off[i]));
+}
+template <typename T, int V, int WARPS, int NV>
+__device__ __forceinline__ void take(const Vec<T, V> *slots, T (&x)[kHeld], const Place<V, WARPS, NV> &at) {
+#pragma unroll
+    for (int i = 0; i < NV; i++)
+        if (at.col[i] >= 0) {
+            const Vec<T, V> v = slots[i * blockDim.x + threadIdx.x];
+#pragma unroll
+            for (int e = 0; e < V; e++) x[i * V + e] = v.e[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; e++) x[i * V + e] = T(0);
+        }
+}
+template <typename T, int V, int WARPS, int NV>
+__device__ __forceinline__ void put(T *to, const T (&x)[kHeld], const Place<V, WARPS, NV> &at) {
+#pragma unroll
+    for (int i = 0; i < NV; i++)
+        if (at.col[i] >= 0) {
+            Vec<T, V> v;
+#pragma unroll
+            for (int e = 0; e < V; e++) v.e[e] = x[i * V + e];
+            *reinterpret_cast<Vec<T, V> *>(to + at.off[i]) = v;
+        }
+}
+// The group's parameters of the thread's values (from L1 after the first item).
+template <typename T, int V, int WARPS, int NV>
+__device__ __forceinline__ void params(const T *p, int64_t c0, T (&v)[kHeld], const Place<V, WARPS, NV> &at) {
+#pragma unroll
+    for (int i = 0; i < NV; i++)
+        if (at.col[i] >= 0) {
+            const Vec<T, V> w = *reinterpret_cast<const Vec<T, V> *>(p + c0 + at.col[i]);
+#pragma unroll
+            for (int e = 0; e < V; e++) v[i * V + e] = w.e[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; e++) v[i * V + e] = T(0);
+        }
+}
+
 template <typename T, int V, int WARPS>
-__global__ void __launch_bounds__(32 * Held<WARPS>::CTA) held_forward_kernel(const Args<T> a) {
+__global__ void __launch_bounds__(32 * Held<WARPS>::CTA, 1024 / (32 * Held<WARPS>::CTA))
+held_forward_kernel(const Args<T> a) {
     using H = Held<WARPS>;
     constexpr int NV = kHeld / V;
     __shared__ T sums[2][H::CTA];
+    extern __shared__ __align__(16) unsigned char raw[];
+    Vec<T, V> *slots = reinterpret_cast<Vec<T, V> *>(raw);
     const int set = threadIdx.x / H::THREADS, t = threadIdx.x % H::THREADS;
     const Place<V, WARPS, NV> at(t, a.S, a.C, a.D);
-    const int64_t items = a.B * a.G;
+    const int64_t items = a.B * a.G, step = (int64_t)gridDim.x * H::SETS;
     const T n = (T)(a.S * a.D);
-    for (int64_t item = (int64_t)blockIdx.x * H::SETS + set; item < items; item += (int64_t)gridDim.x * H::SETS) {
-        const int64_t b = item / a.G, g = item - b * a.G;
-        const int64_t base = b * a.S * a.C + g * a.D;
-        Vec<T, V> x[NV];
+    const int64_t sample = a.S * a.C, b_step = step / a.G, g_step = step - b_step * a.G;
+    const int turn = NV * blockDim.x;
+    int64_t item = (int64_t)blockIdx.x * H::SETS + set;
+    int64_t b = item / a.G, g = item - b * a.G;
+    if (item < items) fetch(slots, a.x + b * sample + g * a.D, at);
+    copies_commit();
+    for (int now = 0; item < items; item += step, now ^= 1) {
+        const int64_t base = b * sample + g * a.D, c0 = g * a.D;
+        T x[kHeld], p[kHeld];
+        b += b_step, g += g_step;  // the next item's, without a division
+        if (g >= a.G) b++, g -= a.G;
+        if (item + step < items) fetch(slots + (now ^ 1) * turn, a.x + b * sample + g * a.D, at);
+        copies_commit();
+        copies_done<1>();
+        take(slots + now * turn, x, at);
         T sum = T(0);
 #pragma unroll
-        for (int i = 0; i < NV; i++)
-            if (at.col[i] >= 0) x[i] = *reinterpret_cast<const Vec<T, V> *>(a.x + base + at.off[i]);
-#pragma unroll
-        for (int i = 0; i < NV; i++)
-            if (at.col[i] >= 0) {
-#pragma unroll
-                for (int e = 0; e < V; e++) sum += x[i].e[e];
-            }
+        for (int i = 0; i < kHeld; i++) sum += x[i];
         const T mean = set_sum<T, WARPS>(sum, sums[0], set) / n;
         T sq = T(0);
 #pragma unroll
-        for (int i = 0; i < NV; i++)
-            if (at.col[i] >= 0) {
-#pragma unroll
-                for (int e = 0; e < V; e++) {
-                    x[i].e[e] -= mean;
-                    sq += x[i].e[e] * x[i].e[e];
-                }
+        for (int i = 0; i < kHeld; i++)
+            if (at.col[i / V] >= 0) {
+                x[i] -= mean;
+                sq += x[i] * x[i];
             }
         const T rstd = inv_sqrt(set_sum<T, WARPS>(sq, sums[1], set) / n + a.eps);
         if (t == 0 && a.mean) {
@@ -149,18 +221,19 @@ __global__ void __launch_bounds__(32 * Held<WARPS>::CTA) held_forward_kernel(con
             a.rstd[item] = rstd;
         }
 #pragma unroll
-        for (int i = 0; i < NV; i++)
-            if (at.col[i] >= 0) {
-                const int64_t c = g * a.D + at.col[i];
+        for (int i = 0; i < kHeld; i++) x[i] *= rstd;
+        if (a.gamma) {
+            params(a.gamma, c0, p, at);
 #pragma unroll
-                for (int e = 0; e < V; e++) {
-                    T u = x[i].e[e] * rstd;
-                    if (a.gamma) u *= a.gamma[c + e];
-                    if (a.beta) u += a.beta[c + e];
-                    x[i].e[e] = act_value(a.act, u);
-                }
-                *reinterpret_cast<Vec<T, V> *>(a.y + base + at.off[i]) = x[i];
-            }
+            for (int i = 0; i < kHeld; i++) x[i] *= p[i];
+        }
+        if (a.beta) {
+            params(a.beta, c0, p, at);
+#pragma unroll
+            for (int i = 0; i < kHeld; i++) x[i] += p[i];
+        }
+        act_values(a.act, x);
+        put(a.y + base, x, at);
     }
 }
 
@@ -168,88 +241,109 @@ __global__ void __launch_bounds__(32 * Held<WARPS>::CTA) held_forward_kernel(con
 // (nb sets for every group).  a.dpart, unless NULL, gets its sums over samples
 // and positions: [nb, C] of du, then [nb, C] of du xhat.
 template <typename T, int V, int WARPS>
-__global__ void __launch_bounds__(32 * Held<WARPS>::CTA) held_backward_kernel(const Args<T> a, int64_t nb) {
+__global__ void __launch_bounds__(32 * Held<WARPS>::CTA, 1024 / (32 * Held<WARPS>::CTA))
+held_backward_kernel(const Args<T> a, int64_t nb) {
     using H = Held<WARPS>;
     constexpr int NV = kHeld / V;
     __shared__ T sums[2][H::CTA];
     extern __shared__ __align__(16) unsigned char raw[];
+    constexpr int AHEAD = kAhead<T, true>;
+    const int turn = NV * blockDim.x;
+    Vec<T, V> *xs = reinterpret_cast<Vec<T, V> *>(raw), *ds = xs + (1 + AHEAD) * turn;
     const int set = threadIdx.x / H::THREADS, t = threadIdx.x % H::THREADS;
     const Place<V, WARPS, NV> at(t, a.S, a.C, a.D);
     const int64_t k = (int64_t)blockIdx.x * H::SETS + set;
-    if (k >= nb * a.G) return;  // a whole set: barriers are the set's own
-    const int64_t g = k % a.G;
+    const bool on = k < nb * a.G;  // a whole set: the barriers in the loop are the set's own
+    const int64_t g = k % a.G, sample = a.S * a.C;
     const T n = (T)(a.S * a.D);
     T du_sum[kHeld], dux_sum[kHeld];
 #pragma unroll
     for (int i = 0; i < kHeld; i++) du_sum[i] = dux_sum[i] = T(0);
-    for (int64_t b = k / a.G; b < a.B; b += nb) {
-        const int64_t base = b * a.S * a.C + g * a.D;
-        Vec<T, V> x[NV], h[NV];
-#pragma unroll
-        for (int i = 0; i < NV; i++)
-            if (at.col[i] >= 0) {
-                x[i] = *reinterpret_cast<const Vec<T, V> *>(a.x + base + at.off[i]);
-                h[i] = *reinterpret_cast<const Vec<T, V> *>(a.dy + base + at.off[i]);
-            }
+    auto fetch_both = [&](int64_t sb, int to) {
+        if (sb < a.B) {
+            fetch(xs + to * turn, a.x + sb * sample + g * a.D, at);
+            fetch(ds + to * turn, a.dy + sb * sample + g * a.D, at);
+        }
+        copies_commit();
+    };
+    int64_t b = on ? k / a.G : a.B;
+    if (AHEAD) fetch_both(b, 0);
+    for (int now = 0; b < a.B; b += nb, now ^= AHEAD) {
+        fetch_both(b + AHEAD * nb, now ^ AHEAD);
         const T mean = a.mean[b * a.G + g], rstd = a.rstd[b * a.G + g];
+        T x[kHeld], h[kHeld], u[kHeld], p[kHeld];
+        copies_done<AHEAD>();
+        take(xs + now * turn, x, at);
+        take(ds + now * turn, h, at);
+#pragma unroll
+        for (int i = 0; i < kHeld; i++) x[i] = at.col[i / V] >= 0 ? (x[i] - mean) * rstd : T(0);
+        if (a.act != J4C_ACT_NONE) {
+#pragma unroll
+            for (int i = 0; i < kHeld; i++) u[i] = x[i];
+            if (a.gamma) {
+                params(a.gamma, g * a.D, p, at);
+#pragma unroll
+                for (int i = 0; i < kHeld; i++) u[i] *= p[i];
+            }
+            if (a.beta) {
+                params(a.beta, g * a.D, p, at);
+#pragma unroll
+                for (int i = 0; i < kHeld; i++) u[i] += p[i];
+            }
+            act_slopes(a.act, u, h);
+        }
+#pragma unroll
+        for (int i = 0; i < kHeld; i++) {
+            du_sum[i] += h[i];
+            dux_sum[i] += h[i] * x[i];
+        }
+        if (a.gamma) {
+            params(a.gamma, g * a.D, p, at);
+#pragma unroll
+            for (int i = 0; i < kHeld; i++) h[i] *= p[i];
+        }
         T s1 = T(0), s2 = T(0);
 #pragma unroll
-        for (int i = 0; i < NV; i++)
-            if (at.col[i] >= 0) {
-                const int64_t c = g * a.D + at.col[i];
-#pragma unroll
-                for (int e = 0; e < V; e++) {
-                    const T xhat = (x[i].e[e] - mean) * rstd;
-                    const T gm = a.gamma ? a.gamma[c + e] : T(1);
-                    T u = xhat * gm;
-                    if (a.beta) u += a.beta[c + e];
-                    const T du = h[i].e[e] * act_slope(a.act, u);
-                    du_sum[i * V + e] += du;
-                    dux_sum[i * V + e] += du * xhat;
-                    x[i].e[e] = xhat;
-                    h[i].e[e] = du * gm;
-                    s1 += h[i].e[e];
-                    s2 += h[i].e[e] * xhat;
-                }
-            }
+        for (int i = 0; i < kHeld; i++) {
+            s1 += h[i];
+            s2 += h[i] * x[i];
+        }
         s1 = set_sum<T, WARPS>(s1, sums[0], set) / n;
         s2 = set_sum<T, WARPS>(s2, sums[1], set) / n;
 #pragma unroll
-        for (int i = 0; i < NV; i++)
-            if (at.col[i] >= 0) {
-#pragma unroll
-                for (int e = 0; e < V; e++) x[i].e[e] = rstd * (h[i].e[e] - s1 - x[i].e[e] * s2);
-                *reinterpret_cast<Vec<T, V> *>(a.y + base + at.off[i]) = x[i];
-            }
+        for (int i = 0; i < kHeld; i++) x[i] = rstd * (h[i] - s1 - x[i] * s2);
+        put(a.y + b * sample + g * a.D, x, at);
     }
     if (!a.dpart) return;
-    // sums over samples: now over the positions of a channel, through shared memory
-    T *buf = reinterpret_cast<T *>(raw) + (size_t)set * a.S * a.D;
+    // sums over samples: now over the positions of a channel, through shared
+    // memory (the slots' space: every set's copies have been read)
+    copies_done<0>();
+    __syncthreads();
+    T *buf = reinterpret_cast<T *>(raw) + (size_t)set * H::THREADS * kHeld;
     for (int which = 0; which < 2; which++) {
 #pragma unroll
-        for (int i = 0; i < NV; i++)
-            if (at.col[i] >= 0) {
-                const int64_t s = (at.off[i] - at.col[i]) / a.C;
-#pragma unroll
-                for (int e = 0; e < V; e++)
-                    buf[s * a.D + at.col[i] + e] = which ? dux_sum[i * V + e] : du_sum[i * V + e];
+        for (int i = 0; i < kHeld; i++)
+            if (at.col[i / V] >= 0) {
+                const int64_t s = (at.off[i / V] - at.col[i / V]) / a.C;
+                buf[s * a.D + at.col[i / V] + i % V] = which ? dux_sum[i] : du_sum[i];
             }
-        asm volatile("bar.sync %0, %1;" ::"r"(1 + set), "n"(32 * WARPS) : "memory");
-        for (int c = t; c < a.D; c += H::THREADS) {
-            T v = T(0);
-            for (int s = 0; s < a.S; s++) v += buf[s * a.D + c];
-            a.dpart[((int64_t)which * nb + k / a.G) * a.C + g * a.D + c] = v;
-        }
-        asm volatile("bar.sync %0, %1;" ::"r"(1 + set), "n"(32 * WARPS) : "memory");
+        __syncthreads();
+        if (on)
+            for (int c = t; c < a.D; c += H::THREADS) {
+                T v = T(0);
+                for (int s = 0; s < a.S; s++) v += buf[s * a.D + c];
+                a.dpart[((int64_t)which * nb + k / a.G) * a.C + g * a.D + c] = v;
+            }
+        __syncthreads();
     }
 }
 
 // out[j] = sum over r of in[r, j], r < rows, for two [rows, cols] arrays back
-// to back: 32 columns and 8 lanes of rows a CTA; either output may be NULL.
+// to back: 32 columns and 32 lanes of rows a CTA; either output may be NULL.
 template <typename T>
-__global__ void __launch_bounds__(256) sum_rows_kernel(const T *__restrict__ in, int64_t rows, int64_t cols, T *out0,
-                                                       T *out1) {
-    __shared__ T part[8][33];
+__global__ void __launch_bounds__(1024) sum_rows_kernel(const T *__restrict__ in, int64_t rows, int64_t cols, T *out0,
+                                                        T *out1) {
+    __shared__ T part[32][33];
     const int lane = threadIdx.x % 32, rl = threadIdx.x / 32;
     const int64_t c = (int64_t)blockIdx.x * 32 + lane;
     T *out = blockIdx.y ? out1 : out0;
@@ -258,21 +352,20 @@ __global__ void __launch_bounds__(256) sum_rows_kernel(const T *__restrict__ in,
     T v = T(0);
     if (c < cols) {
         int64_t r = rl;
-        for (; r + 24 < rows; r += 32) {
+        for (; r + 96 < rows; r += 128) {
             T w[4];
 #pragma unroll
-            for (int u = 0; u < 4; u++) w[u] = in[(r + 8 * u) * cols + c];
+            for (int u = 0; u < 4; u++) w[u] = in[(r + 32 * u) * cols + c];
             v += (w[0] + w[1]) + (w[2] + w[3]);
         }
-        for (; r < rows; r += 8) v += in[r * cols + c];
+        for (; r < rows; r += 32) v += in[r * cols + c];
     }
     part[rl][lane] = v;
     __syncthreads();
-    if (rl == 0 && c < cols) {
-#pragma unroll
-        for (int i = 1; i < 8; i++) v += part[i][lane];
-        out[c] = v;
-    }
+    // the warp of a column adds the column's 32 lanes
+    v = warp_sum(part[lane][rl]);
+    const int64_t mine = (int64_t)blockIdx.x * 32 + rl;
+    if (lane == 0 && mine < cols) out[mine] = v;
 }
 
 // ---- groups cut into tiles ------------------------------------------------------------
@@ -282,18 +375,18 @@ __global__ void __launch_bounds__(256) sum_rows_kernel(const T *__restrict__ in,
 struct Geo {
     int64_t S, C, G, D;
     int rows, row_tiles, width, col_tiles, per, cuts;
+    int dcols;  // columns of V channels of a group (of a tile, where per = 0)
     __host__ __device__ int parts() const { return row_tiles * cuts; }  // tiles of a (sample, group)
 };
 
 struct Tile {
     int64_t b, c0, g0;
     int r0, rows, width, groups, cut;
-    __device__ __forceinline__ Tile(const Geo &q, int64_t block) {
-        const int ct = (int)(block % q.col_tiles);
-        const int64_t br = block / q.col_tiles;
-        const int rt = (int)(br % q.row_tiles);
-        b = br / q.row_tiles;
-        r0 = rt * q.rows;
+    // grid: row tiles, column tiles, samples
+    __device__ __forceinline__ explicit Tile(const Geo &q) {
+        const int ct = blockIdx.y;
+        b = blockIdx.z;
+        r0 = blockIdx.x * q.rows;
         rows = (int)min((int64_t)q.rows, q.S - r0);
         if (q.per) {
             g0 = (int64_t)ct * q.per;
@@ -318,277 +411,356 @@ struct Lanes {
     bool on;
     __device__ __forceinline__ Lanes(int width, int V) {
         cols = width / V;
-        rows = cols >= kTileThreads ? 1 : kTileThreads / cols;
-        j = cols >= kTileThreads ? threadIdx.x : threadIdx.x % cols;
-        r = cols >= kTileThreads ? 0 : threadIdx.x / cols;
+        rows = cols >= (int)blockDim.x ? 1 : blockDim.x / cols;
+        j = cols >= (int)blockDim.x ? threadIdx.x : threadIdx.x % cols;
+        r = cols >= (int)blockDim.x ? 0 : threadIdx.x / cols;
         on = r < rows;
     }
 };
 
-// Sums red[lane of rows][column] over each group's columns; out[group], by one warp a group.
-template <typename T, typename Store>
-__device__ __forceinline__ void sum_groups(const T *red, const Lanes &l, int groups, Store store) {
-    const int per = l.cols / groups, all = per * l.rows;
-    for (int g = threadIdx.x / 32; g < groups; g += kTileThreads / 32) {
-        T v = T(0);
-        for (int k = threadIdx.x % 32; k < all; k += 32) {
-            const int r = k / per;
-            v += red[r * l.cols + g * per + (k - r * per)];
-        }
-        v = warp_sum(v);
-        if (threadIdx.x % 32 == 0) store(g, v);
+// Every group of the tile by a power of two of lanes, as many as there are
+// threads for (at most a warp): body(group, whether it is one, lane, lanes).
+// All threads get there as often.
+template <typename Body>
+__device__ __forceinline__ void by_group(int groups, Body body) {
+    int lanes = 1;
+    while (lanes < 32 && 2 * lanes * groups <= (int)blockDim.x) lanes *= 2;
+    for (int g0 = 0; g0 < groups; g0 += blockDim.x / lanes) {
+        const int g = g0 + threadIdx.x / lanes;
+        body(g, g < groups, threadIdx.x % lanes, lanes);
+    }
+}
+template <typename T>
+__device__ __forceinline__ T lanes_sum(T v, int lanes) {
+    for (int o = lanes / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// A thread's values of a column, in batches of VALUES whose loads are in flight
+// together: f(the batch's first row, whether it is whole, its rows) -- whole
+// batches, but for the last, without a test for every row.
+template <int V, int VALUES>
+constexpr int kRows = VALUES / V;
+template <int U, typename F>
+__device__ __forceinline__ void by_batch(const Lanes &l, int rows, F f) {
+    int left = (rows - l.r + l.rows - 1) / l.rows, r = l.r;
+    for (; left >= U; left -= U, r += U * l.rows) f(r, std::true_type{}, U);
+    if (left > 0) f(r, std::false_type{}, left);
+}
+template <bool WHOLE, typename T, int V, int N>
+__device__ __forceinline__ void load_rows(T (&x)[N], const T *p, int64_t pitch, int rows) {
+#pragma unroll
+    for (int i = 0; i < N / V; i++, p += pitch) {
+        Vec<T, V> v{};
+        if (WHOLE || i < rows) v = *reinterpret_cast<const Vec<T, V> *>(p);
+#pragma unroll
+        for (int e = 0; e < V; e++) x[i * V + e] = v.e[e];
+    }
+}
+template <bool WHOLE, typename T, int V, int N>
+__device__ __forceinline__ void store_rows(T *p, const T (&x)[N], int64_t pitch, int rows) {
+#pragma unroll
+    for (int i = 0; i < N / V; i++, p += pitch) {
+        Vec<T, V> v;
+#pragma unroll
+        for (int e = 0; e < V; e++) v.e[e] = x[i * V + e];
+        if (WHOLE || i < rows) *reinterpret_cast<Vec<T, V> *>(p) = v;
     }
 }
 
-// stats[(b G + g) parts + part] = (mean, sum of squared differences from it) of a tile's part of a group.
+// (mean, m2) of n values joined by those of n2 more.
+template <typename T>
+__device__ __forceinline__ void join(T &n, T &mean, T &m2, T n2, T mean2, T m22) {
+    const T all = n + n2, d = mean2 - mean, share = n2 / all;
+    mean += d * share;
+    m2 += m22 + d * d * (n * share);
+    n = all;
+}
+
+// stats[((b G + g) parts + part) 2] = mean, sum of squared differences from it, of a tile's part of a group.
 template <typename T, int V>
-__global__ void __launch_bounds__(kTileThreads) tile_stats_kernel(const Args<T> a, const Geo q, T *__restrict__ stats) {
+__global__ void __launch_bounds__(kTileThreads, 2) tile_stats_kernel(const Args<T> a, const Geo q,
+                                                                     T *__restrict__ stats) {
+    constexpr int N = 16, U = kRows<V, N>;
     extern __shared__ __align__(16) unsigned char raw[];
-    T *tile = reinterpret_cast<T *>(raw);
-    T *red = tile + (size_t)q.rows * q.width;
-    T *means = red + max(kTileThreads, q.width / V);
-    const Tile w(q, blockIdx.x);
+    T *red = reinterpret_cast<T *>(raw);  // (mean, m2) of [lanes of rows][columns]
+    const Tile w(q);
     const Lanes l(w.width, V);
     const T *x = a.x + (w.b * q.S + w.r0) * q.C + w.c0;
+    const int64_t pitch = l.rows * q.C;
     if (l.on)
-        for (int j = l.j; j < l.cols; j += kTileThreads) {
-            T sum = T(0);
-#pragma unroll 8
-            for (int r = l.r; r < w.rows; r += l.rows) {
-                const Vec<T, V> v = *reinterpret_cast<const Vec<T, V> *>(x + r * q.C + j * V);
-                *reinterpret_cast<Vec<T, V> *>(tile + (size_t)r * w.width + j * V) = v;
+        for (int j = l.j; j < l.cols; j += blockDim.x) {
+            T n = T(0), mean = T(0), m2 = T(0);
+            by_batch<U>(l, w.rows, [&](int r, auto whole, int rows) {
+                constexpr bool WHOLE = decltype(whole)::value;
+                T v[N];
+                load_rows<WHOLE, T, V>(v, x + r * q.C + j * V, pitch, rows);
+                T sum = T(0), sq = T(0);
 #pragma unroll
-                for (int e = 0; e < V; e++) sum += v.e[e];
-            }
-            red[l.r * l.cols + j] = sum;
+                for (int i = 0; i < N; i++) sum += v[i];
+                const T count = (T)(rows * V), mb = WHOLE ? sum * T(1.0 / N) : sum / count;
+#pragma unroll
+                for (int i = 0; i < N; i++)
+                    if (WHOLE || i / V < rows) sq += (v[i] - mb) * (v[i] - mb);
+                if (r == l.r) n = count, mean = mb, m2 = sq;
+                else join(n, mean, m2, count, mb, sq);
+            });
+            red[2 * (l.r * l.cols + j)] = mean;
+            red[2 * (l.r * l.cols + j) + 1] = m2;
         }
     __syncthreads();
-    const T n = (T)((int64_t)w.rows * (w.width / w.groups));
-    sum_groups(red, l, w.groups, [&](int g, T v) { means[g] = v / n; });
-    __syncthreads();
-    const int per = l.cols / w.groups;
-    if (l.on)
-        for (int j = l.j; j < l.cols; j += kTileThreads) {
-            const T mean = means[j / per];
-            T sum = T(0);
-#pragma unroll 4
-            for (int r = l.r; r < w.rows; r += l.rows) {
-                const Vec<T, V> v = *reinterpret_cast<const Vec<T, V> *>(tile + (size_t)r * w.width + j * V);
-#pragma unroll
-                for (int e = 0; e < V; e++) sum += (v.e[e] - mean) * (v.e[e] - mean);
+    // the threads of a group: lane r of a column has rows r, r + l.rows, ...
+    by_group(w.groups, [&](int g, bool is, int lane, int lanes) {
+        auto each = [&](auto f) {
+            if (!is) return;
+            for (int r = 0; r < l.rows && r < w.rows; r++) {
+                const T n = (T)(V * ((w.rows - r + l.rows - 1) / l.rows));
+                const T *p = red + 2 * (r * l.cols + g * q.dcols);
+                const int cols = min(q.dcols, l.cols - g * q.dcols);
+                for (int k = lane; k < cols; k += lanes) f(n, p + 2 * k);
             }
-            red[l.r * l.cols + j] = sum;
+        };
+        T sum = T(0), m2 = T(0);
+        each([&](T n, const T *p) { sum += n * p[0]; });
+        const T mean = lanes_sum(sum, lanes) / (T)((int64_t)w.rows * (q.per ? (int)q.D : w.width));
+        each([&](T n, const T *p) { m2 += p[1] + n * (p[0] - mean) * (p[0] - mean); });
+        m2 = lanes_sum(m2, lanes);
+        if (is && lane == 0) {
+            T *s = stats + 2 * ((w.b * q.G + w.g0 + g) * q.parts() + (int)blockIdx.x * q.cuts + w.cut);
+            s[0] = mean;
+            s[1] = m2;
         }
-    __syncthreads();
-    const int part = (w.r0 / q.rows) * q.cuts + w.cut;
-    sum_groups(red, l, w.groups, [&](int g, T v) {
-        T *s = stats + 2 * ((w.b * q.G + w.g0 + g) * q.parts() + part);
-        s[0] = means[g];
-        s[1] = v;
     });
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kTileThreads) tile_apply_kernel(const Args<T> a, const Geo q,
-                                                                  const T *__restrict__ stats) {
+__global__ void __launch_bounds__(kTileThreads, 2) tile_apply_kernel(const Args<T> a, const Geo q,
+                                                                     const T *__restrict__ stats) {
+    constexpr int N = 8, U = kRows<V, N>;
     extern __shared__ __align__(16) unsigned char raw[];
-    const Tile w(q, blockIdx.x);
+    const Tile w(q);
     T *means = reinterpret_cast<T *>(raw), *rstds = means + w.groups;
-    // merge the group's parts, one warp a group
-    const int lane = threadIdx.x % 32;
-    for (int g = threadIdx.x / 32; g < w.groups; g += kTileThreads / 32) {
+    const double n = (double)q.S * q.D;
+    by_group(w.groups, [&](int g, bool is, int lane, int lanes) {
         const T *s = stats + 2 * (w.b * q.G + w.g0 + g) * q.parts();
-        const double n = (double)q.S * q.D;
-        auto count = [&](int p) {
-            const int rows = (int)min((int64_t)q.rows, q.S - (int64_t)(p / q.cuts) * q.rows);
-            const int64_t cols = q.per ? q.D : min((int64_t)q.width, q.D - (int64_t)(p % q.cuts) * q.width);
-            return (double)(rows * cols);
-        };
-        double sum = 0.0;
-        for (int p = lane; p < q.parts(); p += 32) sum += count(p) * (double)s[2 * p];
-        const double mean = warp_sum(sum) / n;
-        double m2 = 0.0;
-        for (int p = lane; p < q.parts(); p += 32) {
-            const double d = (double)s[2 * p] - mean;
-            m2 += (double)s[2 * p + 1] + count(p) * d * d;
+        const int parts = q.parts();
+        double sum = 0.0, m2 = 0.0, mean;
+        if (q.cuts == 1) {
+            // every part but the last has `full` values: weights come in once
+            const int64_t cols = q.D, last_rows = q.S - (int64_t)(q.row_tiles - 1) * q.rows;
+            const double full = (double)(q.rows * cols), less = full - (double)(last_rows * cols);
+            const double tail = is ? (double)s[2 * parts - 2] : 0.0;
+            if (is) {
+#pragma unroll 4
+                for (int p = lane; p < parts; p += lanes) sum += (double)s[2 * p];
+            }
+            mean = (lanes_sum(sum, lanes) * full - less * tail) / n;
+            double sq = 0.0;
+            if (is) {
+#pragma unroll 4
+                for (int p = lane; p < parts; p += lanes) {
+                    const double d = (double)s[2 * p] - mean;
+                    sq += d * d;
+                    m2 += (double)s[2 * p + 1];
+                }
+            }
+            m2 = lanes_sum(m2 + full * sq, lanes) - less * (tail - mean) * (tail - mean);
+        } else {
+            auto count = [&](int p) {
+                const int64_t cols = p % q.cuts == q.cuts - 1 ? q.D - (int64_t)(q.cuts - 1) * q.width : q.width;
+                const int64_t rows = p / q.cuts == q.row_tiles - 1 ? q.S - (int64_t)(q.row_tiles - 1) * q.rows : q.rows;
+                return (double)(rows * cols);
+            };
+            if (is)
+                for (int p = lane; p < parts; p += lanes) sum += count(p) * (double)s[2 * p];
+            mean = lanes_sum(sum, lanes) / n;
+            if (is)
+                for (int p = lane; p < parts; p += lanes) {
+                    const double d = (double)s[2 * p] - mean;
+                    m2 += (double)s[2 * p + 1] + count(p) * d * d;
+                }
+            m2 = lanes_sum(m2, lanes);
         }
-        m2 = warp_sum(m2);
-        if (lane == 0) {
+        if (is && lane == 0) {
             means[g] = (T)mean;
-            rstds[g] = inv_sqrt((T)(m2 / n) + a.eps);
+            rstds[g] = inv_sqrt((T)((m2 < 0.0 ? 0.0 : m2) / n) + a.eps);  // NaN stays
             if (w.r0 == 0 && w.cut == 0 && a.mean) {
                 a.mean[w.b * q.G + w.g0 + g] = means[g];
                 a.rstd[w.b * q.G + w.g0 + g] = rstds[g];
             }
         }
-    }
+    });
     __syncthreads();
     const Lanes l(w.width, V);
-    const int per = l.cols / w.groups;
-    const int64_t base = (w.b * q.S + w.r0) * q.C + w.c0;
+    const int64_t base = (w.b * q.S + w.r0) * q.C + w.c0, pitch = l.rows * q.C;
     if (!l.on) return;
-    for (int j = l.j; j < l.cols; j += kTileThreads) {
-        const T mean = means[j / per], rstd = rstds[j / per];
-        Vec<T, V> gm, bt;
+    for (int j = l.j; j < l.cols; j += blockDim.x) {
+        const int g = j / q.dcols;
+        const T mean = means[g];
+        T scale[V], shift[V];
 #pragma unroll
         for (int e = 0; e < V; e++) {
-            gm.e[e] = a.gamma ? a.gamma[w.c0 + j * V + e] : T(1);
-            bt.e[e] = a.beta ? a.beta[w.c0 + j * V + e] : T(0);
+            scale[e] = a.gamma ? rstds[g] * a.gamma[w.c0 + j * V + e] : rstds[g];
+            shift[e] = a.beta ? a.beta[w.c0 + j * V + e] : T(0);
         }
-#pragma unroll 4
-        for (int r = l.r; r < w.rows; r += l.rows) {
-            Vec<T, V> v = *reinterpret_cast<const Vec<T, V> *>(a.x + base + r * q.C + j * V);
+        by_batch<U>(l, w.rows, [&](int r, auto whole, int rows) {
+            constexpr bool WHOLE = decltype(whole)::value;
+            const int64_t at = base + r * q.C + j * V;
+            T u[N];
+            load_rows<WHOLE, T, V>(u, a.x + at, pitch, rows);
 #pragma unroll
-            for (int e = 0; e < V; e++) {
-                T u = (v.e[e] - mean) * rstd * gm.e[e];
-                if (a.beta) u += bt.e[e];
-                v.e[e] = act_value(a.act, u);
-            }
-            *reinterpret_cast<Vec<T, V> *>(a.y + base + r * q.C + j * V) = v;
-        }
+            for (int i = 0; i < N; i++) u[i] = (u[i] - mean) * scale[i % V] + shift[i % V];
+            act_values(a.act, u);
+            store_rows<WHOLE, T, V>(a.y + at, u, pitch, rows);
+        });
     }
 }
 
-// sums[(b row_tiles + rt) C + c] = sum over the tile's rows of du, and behind
-// all of these ([B row_tiles, C]) of du xhat.
+// A column's parameters in the gradient.
 template <typename T, int V>
-__global__ void __launch_bounds__(kTileThreads) tile_sums_kernel(const Args<T> a, const Geo q, int64_t samples,
-                                                                 T *__restrict__ sums) {
+struct Column {
+    T mean, rstd, gm[V], bt[V];
+    __device__ __forceinline__ void set(const Args<T> &a, int64_t bg, int64_t c) {
+        mean = a.mean[bg], rstd = a.rstd[bg];
+#pragma unroll
+        for (int e = 0; e < V; e++) {
+            gm[e] = a.gamma ? a.gamma[c + e] : T(1);
+            bt[e] = a.beta ? a.beta[c + e] : T(0);
+        }
+    }
+    // x <- xhat, d <- du, for a batch of x and dy (rows behind the tile: d is 0)
+    __device__ __forceinline__ void du(int act, T (&x)[8], T (&d)[8]) const {
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = (x[i] - mean) * rstd;
+        if (act != J4C_ACT_NONE) {
+            T u[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) u[i] = x[i] * gm[i % V] + bt[i % V];
+            act_slopes(act, u, d);
+        }
+    }
+};
+
+// hsums[((b G + g) parts + part) 2] = sum of h, of h xhat, over a tile's part of
+// a group; and, unless a.dpart is NULL, its per-channel sums over the tile's
+// rows: dpart[(b row_tiles + rt) C + c] of du, `half` behind it of du xhat.
+template <typename T, int V>
+__global__ void __launch_bounds__(kTileThreads, 2) tile_sums_kernel(const Args<T> a, const Geo q, int64_t half,
+                                                                    T *__restrict__ hsums) {
+    constexpr int N = 8, U = kRows<V, N>;
     extern __shared__ __align__(16) unsigned char raw[];
-    T *red = reinterpret_cast<T *>(raw);  // [2][lanes of rows][width], where there are several lanes of rows
-    const Tile w(q, blockIdx.x);
+    T *red = reinterpret_cast<T *>(raw);  // [2][lanes of rows][width]
+    const Tile w(q);
     const Lanes l(w.width, V);
-    const int per = l.cols / w.groups;
-    const int64_t base = (w.b * q.S + w.r0) * q.C + w.c0;
-    T *out0 = sums + (w.b * q.row_tiles + w.r0 / q.rows) * q.C + w.c0, *out1 = out0 + samples * q.row_tiles * q.C;
+    const int64_t base = (w.b * q.S + w.r0) * q.C + w.c0, pitch = l.rows * q.C;
     if (l.on)
-        for (int j = l.j; j < l.cols; j += kTileThreads) {
-            const int64_t g = w.g0 + j / per;
-            const T mean = a.mean[w.b * q.G + g], rstd = a.rstd[w.b * q.G + g];
-            Vec<T, V> gm, bt, s1, s2;
+        for (int j = l.j; j < l.cols; j += blockDim.x) {
+            Column<T, V> k;
+            k.set(a, w.b * q.G + w.g0 + j / q.dcols, w.c0 + j * V);
+            T s1[V], s2[V];
+#pragma unroll
+            for (int e = 0; e < V; e++) s1[e] = s2[e] = T(0);
+            by_batch<U>(l, w.rows, [&](int r, auto whole, int rows) {
+                constexpr bool WHOLE = decltype(whole)::value;
+                const int64_t at = base + r * q.C + j * V;
+                T x[N], d[N];
+                load_rows<WHOLE, T, V>(x, a.x + at, pitch, rows);
+                load_rows<WHOLE, T, V>(d, a.dy + at, pitch, rows);  // zeros behind the tile
+                k.du(a.act, x, d);
+#pragma unroll
+                for (int i = 0; i < N; i++) {
+                    s1[i % V] += d[i];
+                    s2[i % V] += WHOLE || i / V < rows ? d[i] * x[i] : T(0);
+                }
+            });
 #pragma unroll
             for (int e = 0; e < V; e++) {
-                gm.e[e] = a.gamma ? a.gamma[w.c0 + j * V + e] : T(1);
-                bt.e[e] = a.beta ? a.beta[w.c0 + j * V + e] : T(0);
-                s1.e[e] = s2.e[e] = T(0);
-            }
-#pragma unroll 4
-            for (int r = l.r; r < w.rows; r += l.rows) {
-                const Vec<T, V> x = *reinterpret_cast<const Vec<T, V> *>(a.x + base + r * q.C + j * V);
-                const Vec<T, V> dy = *reinterpret_cast<const Vec<T, V> *>(a.dy + base + r * q.C + j * V);
-#pragma unroll
-                for (int e = 0; e < V; e++) {
-                    const T xhat = (x.e[e] - mean) * rstd;
-                    T u = xhat * gm.e[e];
-                    if (a.beta) u += bt.e[e];
-                    const T du = dy.e[e] * act_slope(a.act, u);
-                    s1.e[e] += du;
-                    s2.e[e] += du * xhat;
-                }
-            }
-#pragma unroll
-            for (int e = 0; e < V; e++) {
-                if (l.rows == 1) {
-                    out0[j * V + e] = s1.e[e];
-                    out1[j * V + e] = s2.e[e];
-                } else {
-                    red[l.r * w.width + j * V + e] = s1.e[e];
-                    red[(l.rows + l.r) * w.width + j * V + e] = s2.e[e];
-                }
+                red[l.r * w.width + j * V + e] = s1[e];
+                red[(l.rows + l.r) * w.width + j * V + e] = s2[e];
             }
         }
-    if (l.rows == 1) return;
     __syncthreads();
-    for (int c = threadIdx.x; c < 2 * w.width; c += kTileThreads) {
+    // over the lanes of rows: red[which][0][c] is the channel's sum
+    const int64_t row = (w.b * q.row_tiles + (int)blockIdx.x) * q.C + w.c0;
+    for (int c = threadIdx.x; c < 2 * w.width; c += blockDim.x) {
         const int which = c >= w.width, cc = c - which * w.width;
         T v = T(0);
         for (int r = 0; r < l.rows; r++) v += red[(which * l.rows + r) * w.width + cc];
-        (which ? out1 : out0)[cc] = v;
-    }
-}
-
-// Per (sample, group), one CTA: the tiles' sums added up per channel (chan[b C + c],
-// and chan_half behind it the ones of du xhat) and, weighted with gamma, over the
-// group: group[2 (b G + g)] = mean(h), mean(h xhat).
-template <typename T>
-__global__ void __launch_bounds__(256) merge_sums_kernel(const Args<T> a, const Geo q, int64_t samples,
-                                                         const T *__restrict__ sums, T *__restrict__ chan,
-                                                         int64_t chan_half, T *__restrict__ group) {
-    __shared__ T part[2][8];
-    const int64_t b = blockIdx.x / q.G, g = blockIdx.x - b * q.G;
-    const int64_t half = samples * q.row_tiles * q.C;
-    T s1 = T(0), s2 = T(0);
-    for (int64_t d = threadIdx.x; d < q.D; d += 256) {
-        const int64_t c = g * q.D + d;
-        const T *p = sums + b * q.row_tiles * q.C + c;
-        T v1 = T(0), v2 = T(0);
-#pragma unroll 4
-        for (int r = 0; r < q.row_tiles; r++) {
-            v1 += p[r * q.C];
-            v2 += p[half + r * q.C];
-        }
-        chan[b * q.C + c] = v1;
-        chan[chan_half + b * q.C + c] = v2;
-        const T gm = a.gamma ? a.gamma[c] : T(1);
-        s1 += gm * v1;
-        s2 += gm * v2;
-    }
-    s1 = warp_sum(s1);
-    s2 = warp_sum(s2);
-    if (threadIdx.x % 32 == 0) {
-        part[0][threadIdx.x / 32] = s1;
-        part[1][threadIdx.x / 32] = s2;
+        red[which * l.rows * w.width + cc] = v;
+        if (a.dpart) a.dpart[which * half + row + cc] = v;
     }
     __syncthreads();
-    if (threadIdx.x < 2) {
-        T v = T(0);
-        for (int i = 0; i < 8; i++) v += part[threadIdx.x][i];
-        group[2 * (b * q.G + g) + threadIdx.x] = v / (T)(q.S * q.D);
-    }
+    const int part = (int)blockIdx.x * q.cuts + w.cut, span = q.per ? (int)q.D : w.width;
+    by_group(w.groups, [&](int g, bool is, int lane, int lanes) {
+        T s1 = T(0), s2 = T(0);
+        if (is)
+            for (int k = lane; k < span; k += lanes) {
+                const int c = g * span + k;
+                const T gm = a.gamma ? a.gamma[w.c0 + c] : T(1);
+                s1 += gm * red[c];
+                s2 += gm * red[l.rows * w.width + c];
+            }
+        s1 = lanes_sum(s1, lanes);
+        s2 = lanes_sum(s2, lanes);
+        if (is && lane == 0) {
+            T *s = hsums + 2 * ((w.b * q.G + w.g0 + g) * q.parts() + part);
+            s[0] = s1;
+            s[1] = s2;
+        }
+    });
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kTileThreads) tile_grad_kernel(const Args<T> a, const Geo q,
-                                                                 const T *__restrict__ group) {
-    const Tile w(q, blockIdx.x);
-    const Lanes l(w.width, V);
-    const int per = l.cols / w.groups;
-    const int64_t base = (w.b * q.S + w.r0) * q.C + w.c0;
-    if (!l.on) return;
-    for (int j = l.j; j < l.cols; j += kTileThreads) {
-        const int64_t bg = w.b * q.G + w.g0 + j / per;
-        const T mean = a.mean[bg], rstd = a.rstd[bg], h1 = group[2 * bg], h2 = group[2 * bg + 1];
-        Vec<T, V> gm, bt;
-#pragma unroll
-        for (int e = 0; e < V; e++) {
-            gm.e[e] = a.gamma ? a.gamma[w.c0 + j * V + e] : T(1);
-            bt.e[e] = a.beta ? a.beta[w.c0 + j * V + e] : T(0);
-        }
+__global__ void __launch_bounds__(kTileThreads, 2) tile_grad_kernel(const Args<T> a, const Geo q,
+                                                                    const T *__restrict__ hsums) {
+    constexpr int N = 8, U = kRows<V, N>;
+    extern __shared__ __align__(16) unsigned char raw[];
+    const Tile w(q);
+    T *mean_h = reinterpret_cast<T *>(raw), *mean_hx = mean_h + w.groups;
+    by_group(w.groups, [&](int g, bool is, int lane, int lanes) {
+        const T *s = hsums + 2 * (w.b * q.G + w.g0 + g) * q.parts();
+        T s1 = T(0), s2 = T(0);
+        if (is)
 #pragma unroll 4
-        for (int r = l.r; r < w.rows; r += l.rows) {
-            Vec<T, V> x = *reinterpret_cast<const Vec<T, V> *>(a.x + base + r * q.C + j * V);
-            const Vec<T, V> dy = *reinterpret_cast<const Vec<T, V> *>(a.dy + base + r * q.C + j * V);
-#pragma unroll
-            for (int e = 0; e < V; e++) {
-                const T xhat = (x.e[e] - mean) * rstd;
-                T u = xhat * gm.e[e];
-                if (a.beta) u += bt.e[e];
-                const T h = dy.e[e] * act_slope(a.act, u) * gm.e[e];
-                x.e[e] = rstd * (h - h1 - xhat * h2);
+            for (int p = lane; p < q.parts(); p += lanes) {
+                s1 += s[2 * p];
+                s2 += s[2 * p + 1];
             }
-            *reinterpret_cast<Vec<T, V> *>(a.y + base + r * q.C + j * V) = x;
+        s1 = lanes_sum(s1, lanes);
+        s2 = lanes_sum(s2, lanes);
+        if (is && lane == 0) {
+            mean_h[g] = s1 / (T)(q.S * q.D);
+            mean_hx[g] = s2 / (T)(q.S * q.D);
         }
+    });
+    __syncthreads();
+    const Lanes l(w.width, V);
+    const int64_t base = (w.b * q.S + w.r0) * q.C + w.c0, pitch = l.rows * q.C;
+    if (!l.on) return;
+    for (int j = l.j; j < l.cols; j += blockDim.x) {
+        const int g = j / q.dcols;
+        Column<T, V> k;
+        k.set(a, w.b * q.G + w.g0 + g, w.c0 + j * V);
+        const T h1 = mean_h[g], h2 = mean_hx[g];
+        by_batch<U>(l, w.rows, [&](int r, auto whole, int rows) {
+            constexpr bool WHOLE = decltype(whole)::value;
+            const int64_t at = base + r * q.C + j * V;
+            T x[N], d[N];
+            load_rows<WHOLE, T, V>(x, a.x + at, pitch, rows);
+            load_rows<WHOLE, T, V>(d, a.dy + at, pitch, rows);
+            k.du(a.act, x, d);
+#pragma unroll
+            for (int i = 0; i < N; i++) x[i] = k.rstd * (d[i] * k.gm[i % V] - h1 - x[i] * h2);
+            store_rows<WHOLE, T, V>(a.y + at, x, pitch, rows);
+        });
     }
 }
 
 // ---- host ----------------------------------------------------------------------------
 inline bool held(int64_t S, int64_t D) { return D <= kMaxHeld && S <= kMaxHeld && S * D <= kMaxHeld; }
 
-// Rows of a tile: as many as shared memory takes, fewer when the batch would
-// leave SMs without a tile; at most `most` (the backward sums need no shared
-// memory, and a tile's sums cost 2 / rows of a pass).
 template <typename T>
-Geo make_geo(int64_t B, int64_t S, int64_t C, int64_t G, bool backward) {
+Geo make_geo(int64_t B, int64_t S, int64_t C, int64_t G) {
     Geo q;
     q.S = S, q.C = C, q.G = G, q.D = C / G;
     if (q.D <= kTileChannels) {
@@ -602,13 +774,13 @@ Geo make_geo(int64_t B, int64_t S, int64_t C, int64_t G, bool backward) {
         q.cuts = (int)ceil_div(q.D, q.width);
         q.col_tiles = (int)(G * q.cuts);
     }
-    const int64_t fit = std::max<int64_t>(1, kTileBytes / ((int64_t)q.width * sizeof(T)));
-    int64_t rows = fit;
-    if (backward) rows = std::max<int64_t>(fit, ceil_div(B * S * q.col_tiles, (int64_t)sm_count() * 16));
-    // two tiles for every SM, where there are rows enough
-    const int64_t tiles_wanted = ceil_div((int64_t)sm_count() * 2, B * q.col_tiles);
-    rows = std::min(rows, std::max<int64_t>(4, ceil_div(S, tiles_wanted)));
-    rows = std::min(rows, S);
+    // Tiles of about 192 KB, as many as fill whole waves of two CTAs an SM: a tile
+    // costs its threads some 500 instructions beside its values.  At least four rows.
+    const int64_t slots = (int64_t)sm_count() * 2;
+    const int64_t target = std::max<int64_t>(4, 192 * 1024 / ((int64_t)q.width * sizeof(T)));
+    const int64_t waves = std::max<int64_t>(1, (B * S * q.col_tiles + target * slots / 2) / (target * slots));
+    const int64_t per_sample = std::max<int64_t>(1, waves * slots / (B * q.col_tiles));  // tiles of rows
+    const int64_t rows = std::min(S, std::max<int64_t>(4, ceil_div(S, per_sample)));
     q.rows = (int)rows;
     q.row_tiles = (int)ceil_div(S, rows);
     return q;
@@ -637,32 +809,36 @@ size_t workspace(int64_t B, int64_t S, int64_t C, int64_t G, bool backward) {
     const int64_t es = sizeof(T);
     if (held(S, C / G)) return backward ? (size_t)(2 * es * C * held_sets(B, G, held_warps(S * (C / G)))) : 0;
     const int64_t part = samples_of_part(B, (backward ? 2 : 1) * S * C * es);
-    const Geo q = make_geo<T>(part, S, C, G, backward);
-    if (!backward) return (size_t)(2 * es * part * G * q.parts());
-    return (size_t)(es * (2 * part * q.row_tiles * C + 2 * B * C + 2 * part * G));
+    const Geo q = make_geo<T>(part, S, C, G);
+    // the parts' statistics, and backward the tiles' sums of every channel
+    return (size_t)(2 * es * (part * G * q.parts() + (backward ? B * q.row_tiles * C : 0)));
 }
 
 template <typename T, int V, int WARPS>
 int launch_held(const Args<T> &a, bool backward, T *dgamma, T *dbeta, cudaStream_t s) {
     using H = Held<WARPS>;
     const int threads = 32 * H::CTA;
+    const size_t smem = (size_t)threads * kHeld * sizeof(T) *
+                        (backward ? 2 * (1 + kAhead<T, true>) : 1 + kAhead<T, false>);
+    auto allow = [&](auto kernel) {
+        return smem > 48 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)
+                                : cudaSuccess;
+    };
     if (!backward) {
         const int64_t ctas = ceil_div(a.B * a.G, H::SETS);
-        const unsigned grid = (unsigned)std::min<int64_t>(ctas, (int64_t)sm_count() * (2048 / threads));
-        held_forward_kernel<T, V, WARPS><<<grid, threads, 0, s>>>(a);
+        const unsigned grid = (unsigned)std::min<int64_t>(ctas, (int64_t)sm_count() * (1024 / threads));
+        J4C_CUDA(allow(held_forward_kernel<T, V, WARPS>));
+        held_forward_kernel<T, V, WARPS><<<grid, threads, smem, s>>>(a);
         J4C_LAUNCH_CHECK("held_forward_kernel");
         return J4C_OK;
     }
     const int64_t nb = held_sets(a.B, a.G, WARPS);
     if (ceil_div(nb * a.G, H::SETS) >= (1ll << 31)) return set_error(J4C_E_UNSUPPORTED, "j4c_group_norm: too many groups");
-    const size_t smem = a.dpart ? (size_t)H::SETS * a.S * a.D * sizeof(T) : 0;
-    if (smem > 48 * 1024)
-        J4C_CUDA(cudaFuncSetAttribute(held_backward_kernel<T, V, WARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      (int)smem));
+    J4C_CUDA(allow(held_backward_kernel<T, V, WARPS>));
     held_backward_kernel<T, V, WARPS><<<(unsigned)ceil_div(nb * a.G, H::SETS), threads, smem, s>>>(a, nb);
     J4C_LAUNCH_CHECK("held_backward_kernel");
     if (a.dpart) {
-        sum_rows_kernel<T><<<dim3((unsigned)ceil_div(a.C, 32), 2), 256, 0, s>>>(a.dpart, nb, a.C, dbeta, dgamma);
+        sum_rows_kernel<T><<<dim3((unsigned)ceil_div(a.C, 32), 2), 1024, 0, s>>>(a.dpart, nb, a.C, dbeta, dgamma);
         J4C_LAUNCH_CHECK("sum_rows_kernel");
     }
     return J4C_OK;
@@ -684,44 +860,39 @@ template <typename T, int V>
 int run_tiles(const Args<T> &whole, bool backward, T *dgamma, T *dbeta, void *ws, cudaStream_t s) {
     const int64_t B = whole.B, S = whole.S, C = whole.C, G = whole.G;
     const int64_t part = samples_of_part(B, (backward ? 2 : 1) * S * C * (int64_t)sizeof(T));
-    const Geo q = make_geo<T>(part, S, C, G, backward);
-    const int64_t tiles_of_sample = (int64_t)q.row_tiles * q.col_tiles;
-    if (part * tiles_of_sample >= (1ll << 31) || part * G >= (1ll << 31))
-        return set_error(J4C_E_UNSUPPORTED, "j4c_group_norm: too many tiles");
-    T *w = static_cast<T *>(ws);
+    Geo q = make_geo<T>(part, S, C, G);
+    q.dcols = (q.per ? (int)q.D : q.width) / V;
+    if (q.col_tiles > 65535 || part > 65535)
+        return set_error(J4C_E_UNSUPPORTED, "j4c_group_norm: %lld channels are too many", (long long)C);
+    T *stats = static_cast<T *>(ws), *sums = stats + 2 * part * G * q.parts();
+    const int cols = q.width / V;
+    const int threads = cols >= kTileThreads ? kTileThreads : (int)ceil_div(kTileThreads / cols * cols, 32) * 32;
+    const size_t per_group = 2 * (size_t)std::max(q.per, 1) * sizeof(T);
+    const size_t stats_smem = 2 * (size_t)std::max(kTileThreads, cols) * sizeof(T);
+    const size_t sums_smem = 2 * (size_t)std::max(kTileThreads * V, q.width) * sizeof(T);
     for (int64_t b0 = 0; b0 < B; b0 += part) {
         const int64_t nb = std::min(part, B - b0);
         Args<T> a = whole;
         a.B = nb;
         a.x += b0 * S * C, a.y += b0 * S * C;
         if (a.mean) a.mean += b0 * G, a.rstd += b0 * G;
-        const unsigned grid = (unsigned)(nb * tiles_of_sample);
+        const dim3 grid((unsigned)q.row_tiles, (unsigned)q.col_tiles, (unsigned)nb);
         if (!backward) {
-            const size_t smem = ((size_t)q.rows * q.width + std::max(kTileThreads, q.width / V) + std::max(q.per, 1)) *
-                                sizeof(T);
-            if (smem > 48 * 1024)  // the tile and the columns' sums: at most 72 KB
-                J4C_CUDA(cudaFuncSetAttribute(tile_stats_kernel<T, V>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                              96 * 1024));
-            tile_stats_kernel<T, V><<<grid, kTileThreads, smem, s>>>(a, q, w);
+            tile_stats_kernel<T, V><<<grid, threads, stats_smem, s>>>(a, q, stats);
             J4C_LAUNCH_CHECK("tile_stats_kernel");
-            tile_apply_kernel<T, V><<<grid, kTileThreads, 2 * std::max(q.per, 1) * sizeof(T), s>>>(a, q, w);
+            tile_apply_kernel<T, V><<<grid, threads, per_group, s>>>(a, q, stats);
             J4C_LAUNCH_CHECK("tile_apply_kernel");
             continue;
         }
         a.dy += b0 * S * C;
-        T *sums = w, *chan = w + 2 * part * q.row_tiles * C, *group = chan + 2 * B * C;
-        const size_t smem = 2 * (size_t)std::max(kTileThreads * V, q.width) * sizeof(T);
-        tile_sums_kernel<T, V><<<grid, kTileThreads, smem, s>>>(a, q, nb, sums);
+        if (a.dpart) a.dpart = sums + b0 * q.row_tiles * C;
+        tile_sums_kernel<T, V><<<grid, threads, sums_smem, s>>>(a, q, B * q.row_tiles * C, stats);
         J4C_LAUNCH_CHECK("tile_sums_kernel");
-        // chan is [2, B, C] over the whole batch: this part's rows of each half
-        merge_sums_kernel<T><<<(unsigned)(nb * G), 256, 0, s>>>(a, q, nb, sums, chan + b0 * C, B * C, group);
-        J4C_LAUNCH_CHECK("merge_sums_kernel");
-        tile_grad_kernel<T, V><<<grid, kTileThreads, 0, s>>>(a, q, group);
+        tile_grad_kernel<T, V><<<grid, threads, per_group, s>>>(a, q, stats);
         J4C_LAUNCH_CHECK("tile_grad_kernel");
     }
-    if (backward && (dgamma || dbeta)) {
-        sum_rows_kernel<T><<<dim3((unsigned)ceil_div(C, 32), 2), 256, 0, s>>>(w + 2 * part * q.row_tiles * C, B, C, dbeta,
-                                                                              dgamma);
+    if (backward && whole.dpart) {
+        sum_rows_kernel<T><<<dim3((unsigned)ceil_div(C, 32), 2), 1024, 0, s>>>(sums, B * q.row_tiles, C, dbeta, dgamma);
         J4C_LAUNCH_CHECK("sum_rows_kernel");
     }
     return J4C_OK;
@@ -733,7 +904,7 @@ int group_norm(const Args<T> &a, bool backward, T *dgamma, T *dbeta, void *ws, c
     constexpr int W = 16 / sizeof(T);
     auto fits = [&](int v) {
         auto ok = [&](const void *p) { return reinterpret_cast<uintptr_t>(p) % (v * sizeof(T)) == 0; };
-        return a.D % v == 0 && ok(a.x) && ok(a.y) && ok(a.dy);
+        return a.D % v == 0 && ok(a.x) && ok(a.y) && ok(a.dy) && ok(a.gamma) && ok(a.beta);
     };
     const int v = fits(W) ? W : W > 2 && fits(2) ? 2 : 1;
     const bool small = held(a.S, a.D);
