@@ -129,6 +129,11 @@ SIGNATURES = {
     "j4c_adamw_step": [I32, I32, I32, P, P, P, P, P, P, P, P, P, P, C.c_double, C.c_double, C.c_double, C.c_double,
                        C.c_double, P],
     "j4c_adamw_moments": [I32, P, P, P, P, P],
+    "j4c_dot_split_act": [P, P, P, P, I64, I64, I64, P, I32, P, P, P, P, P],
+    "j4c_dot_act": [P, P, I64, I64, I64, I32, I32, P, I32, P, P, P, P],
+    "j4c_dense_finish": [I32, P, I64, I64, P, I32, P, P, P],
+    "j4c_dense_grad_workspace": [I32, I64, I64],
+    "j4c_dense_grad": [I32, I64, I64, P, P, I32, I32, P, P, P, P, C.c_size_t, P],
     "j4c_group_norm_workspace": [I32, I64, I64, I64, I64, I32],
     "j4c_group_norm": [I32, I64, I64, I64, I64, P, P, P, C.c_double, I32, P, P, P, P, C.c_size_t, P],
     "j4c_group_norm_grad": [I32, I64, I64, I64, I64, P, P, P, I32, P, P, P, P, P, P, P, C.c_size_t, P],
@@ -136,7 +141,7 @@ SIGNATURES = {
 _RESTYPES = {"j4c_last_error": C.c_char_p, "j4c_dot_workspace_size": C.c_size_t,
              "j4c_split_pitch": C.c_int64, "j4c_split_floats": C.c_int64,
              "j4c_psum_sgd_flag_bytes": C.c_size_t, "j4c_adamw_q8_words": C.c_int64,
-             "j4c_group_norm_workspace": C.c_size_t}
+             "j4c_group_norm_workspace": C.c_size_t, "j4c_dense_grad_workspace": C.c_size_t}
 
 
 def lib() -> C.CDLL:

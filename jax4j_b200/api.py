@@ -541,6 +541,15 @@ class Nn:
         return e.div(e.sum(-1, True))
 
     @staticmethod
+    def dense(x: NDArray, w: NDArray, bias: Optional[NDArray] = None, activation: str = "none",
+              residual: Optional[NDArray] = None) -> NDArray:
+        """act(x . w + bias) + residual as one operation: x [..., K], w [K, N],
+        bias [N], residual like the output [..., N]; FLOAT32 or FLOAT64,
+        differentiable in all four.  Bias, activation and residual are applied
+        in the product's store; activations as for groupNorm."""
+        return _layers.dense(x, w, bias, activation, residual)
+
+    @staticmethod
     def groupNorm(x: NDArray, groups: int, gamma: Optional[NDArray] = None, beta: Optional[NDArray] = None,
                   eps: float = 1e-5, activation: str = "none") -> NDArray:
         """act(gamma * xhat + beta) with xhat = (x - mean) / sqrt(var + eps)

@@ -332,6 +332,10 @@ class PRNGKey:
 # ---------------------------------------------------------------------------
 # Streams: one per (thread, GPU) via torch's thread-local current stream.
 # ---------------------------------------------------------------------------
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda ordinal: torch.cuda.current_stream(ordinal).cuda_stream)
+
+
 def stream_of(ordinal: int) -> int:
     """Handle of the device's current torch stream, with that device made the
     calling thread's current device first: the library launches on the current
@@ -339,7 +343,7 @@ def stream_of(ordinal: int) -> int:
     another GPU's array must not run with a different device current."""
     if torch.cuda.current_device() != ordinal:
         torch.cuda.set_device(ordinal)
-    return torch.cuda.current_stream(ordinal).cuda_stream
+    return _raw_stream(ordinal)  # torch.cuda.current_stream(ordinal).cuda_stream, without the Stream object
 
 
 # ---------------------------------------------------------------------------

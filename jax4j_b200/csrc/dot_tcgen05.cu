@@ -62,6 +62,7 @@
 #include <mutex>
 #include <vector>
 
+#include "act.cuh"
 #include "common.cuh"
 
 namespace j4c {
@@ -466,6 +467,10 @@ __device__ __forceinline__ Unit unit_of(int u, int full_tiles, int splits, int n
 // bit c & 31 of word c / 32 of a row of bits_words words, set where the
 // mask is > 0), and the relu output's bits (act > 0) may be written the same
 // way (act_bits): 1/32 of the bytes.  Bits need C stored untransposed.
+// With ACT (a template parameter of the kernel; operands both K-major, C
+// untransposed, one batch entry) instead:
+//   v = acc + bias[col],  C[row][col] = v,  act[row][col] = act_kind(v) + residual[row][col]
+// (C and residual may be NULL) and the line words of act.
 struct Epilogue {
     const float *bias;
     const float *mask;
@@ -476,6 +481,8 @@ struct Epilogue {
     const uint32_t *mask_bits;
     uint32_t *act_bits;
     int bits_words;
+    int act_kind;
+    const float *residual;
 };
 
 // The bits of |v| for finite v, else 0.
@@ -494,7 +501,7 @@ __device__ __forceinline__ float ep_relu(float v) { return (0.0f >= v) ? 0.0f : 
 // are its lines (read K-major, not transposed) is src[(z * L + l) * K + k];
 // otherwise (MN-major, or a transposed split) src[(z * K + k) * L + l], with
 // z the batch entry of a batched operand and L = M for A, N for B.
-template <int BN>
+template <int BN, bool ACT>
 __device__ void exact_tiles(const float *__restrict__ A, bool a_col, const float *__restrict__ B, bool b_col,
                             float *__restrict__ C, int M, int N, int K, int store_t, const Epilogue &ep,
                             int batch, int a_batched, int b_batched) {
@@ -525,6 +532,22 @@ __device__ void exact_tiles(const float *__restrict__ A, bool a_col, const float
             }
             const size_t idx = boff + (store_t ? (size_t)j * M + i : (size_t)i * N + j);
             float v = ep.bias ? __fadd_rn(s, __ldg(ep.bias + (store_t ? i : j))) : s;
+            if constexpr (ACT) {
+                if (C) C[idx] = v;
+                float o[1] = {v};
+                act_values(ep.act_kind, o);
+                if (ep.residual) o[0] = __fadd_rn(o[0], __ldg(ep.residual + idx));
+                ep.act[idx] = o[0];
+                if (ep.out_lines) {
+                    const uint32_t m = finite_bits(o[0]);
+                    if (m) {
+                        atomicMax(ep.out_lines + i, m);
+                        atomicMax(ep.out_lines + ep.out_rows + j, m);
+                    }
+                    if ((__float_as_uint(o[0]) & 0x7F800000u) == 0x7F800000u) atomicOr(ep.out_flag, 1u);
+                }
+                continue;
+            }
             if (ep.mask_bits)
                 v = (__ldg(ep.mask_bits + (size_t)i * ep.bits_words + (j >> 5)) >> (j & 31)) & 1u ? v : 0.0f;
             else if (ep.mask)
@@ -568,7 +591,7 @@ __device__ __forceinline__ void load_operand(uint32_t dst, const CUtensorMap *ma
 
 // F16: the 3xFP16 split (else 3xTF32).  ahdr / bhdr: the headers of the
 // operands' hi arrays, whose line words give the scales.
-template <int BN, int STAGES, int BK, bool A_MN, bool B_MN, bool F16, bool PAIR>
+template <int BN, int STAGES, int BK, bool A_MN, bool B_MN, bool F16, bool PAIR, bool ACT>
 __global__ void __launch_bounds__(kThreads, 1)
 gemm_3xtf32_kernel(const __grid_constant__ CUtensorMap tAh, const __grid_constant__ CUtensorMap tAl,
                    const __grid_constant__ CUtensorMap tBh, const __grid_constant__ CUtensorMap tBl,
@@ -594,7 +617,7 @@ gemm_3xtf32_kernel(const __grid_constant__ CUtensorMap tAh, const __grid_constan
             return;
         }
         if (ahdr->nonfinite | bhdr->nonfinite) {
-            exact_tiles<BN>(reinterpret_cast<const float *>(ahdr->src), A_MN || (a_layout & kLayoutT),
+            exact_tiles<BN, ACT>(reinterpret_cast<const float *>(ahdr->src), A_MN || (a_layout & kLayoutT),
                             reinterpret_cast<const float *>(bhdr->src), B_MN || (b_layout & kLayoutT), C, M, N, K,
                             store_t, ep, batch, a_batched, b_batched);
             return;
@@ -896,7 +919,61 @@ gemm_3xtf32_kernel(const __grid_constant__ CUtensorMap tAh, const __grid_constan
             // Store; afterwards acc[j] holds the stored value (the relu output
             // when act is written; 0 outside C), from which the line maxima are
             // taken.
-            if (vec_full) {
+            if constexpr (ACT) {
+                // eight columns at a time: the activation's branch is taken once
+                // for them, and few values live beside the accumulators
+                const size_t base = (size_t)row * (size_t)N + col0;
+#pragma unroll
+                for (int c = 0; c < Q::COLS_PER_WARP / 8; c++) {
+                    float x[8];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) x[e] = acc[8 * c + e];
+                    if (vec_full) {
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            float *const xh = x + 4 * h;
+                            if (ep.bias) {
+                                const float4 b = __ldg(reinterpret_cast<const float4 *>(ep.bias + col0) + 2 * c + h);
+                                xh[0] = __fadd_rn(xh[0], b.x); xh[1] = __fadd_rn(xh[1], b.y);
+                                xh[2] = __fadd_rn(xh[2], b.z); xh[3] = __fadd_rn(xh[3], b.w);
+                            }
+                            if (Cb)
+                                reinterpret_cast<float4 *>(Cb + base)[2 * c + h] = make_float4(xh[0], xh[1], xh[2], xh[3]);
+                        }
+                        act_values(ep.act_kind, x);
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            float *const xh = x + 4 * h;
+                            if (ep.residual) {
+                                const float4 r = __ldg(reinterpret_cast<const float4 *>(ep.residual + base) + 2 * c + h);
+                                xh[0] = __fadd_rn(xh[0], r.x); xh[1] = __fadd_rn(xh[1], r.y);
+                                xh[2] = __fadd_rn(xh[2], r.z); xh[3] = __fadd_rn(xh[3], r.w);
+                            }
+                            reinterpret_cast<float4 *>(ep.act + base)[2 * c + h] = make_float4(xh[0], xh[1], xh[2], xh[3]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            const int j = 8 * c + e;
+                            if (row_ok && col0 + j < N) {
+                                if (ep.bias) x[e] = __fadd_rn(x[e], __ldg(ep.bias + col0 + j));
+                                if (Cb) Cb[base + j] = x[e];
+                            }
+                        }
+                        act_values(ep.act_kind, x);
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            const int j = 8 * c + e;
+                            if (row_ok && col0 + j < N) {
+                                if (ep.residual) x[e] = __fadd_rn(x[e], __ldg(ep.residual + base + j));
+                                ep.act[base + j] = x[e];
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8; e++) acc[8 * c + e] = x[e];
+                }
+            } else if (vec_full) {
                 const size_t base = (size_t)row * (size_t)N + col0;
 #pragma unroll
                 for (int v4 = 0; v4 < Q::COLS_PER_WARP / 4; v4++) {
@@ -1613,12 +1690,12 @@ size_t tail_scratch_bound(int64_t m, int64_t n, int64_t batch) {
     return most;
 }
 
-template <int BN, int STAGES, int BK, bool A_MN, bool B_MN, bool F16, bool PAIR>
+template <int BN, int STAGES, int BK, bool A_MN, bool B_MN, bool F16, bool PAIR, bool ACT = false>
 static int launch_gemm(const float *ah, const float *al, const float *bh, const float *bl, float *c,
                        int64_t M, int64_t N, int64_t K, bool store_t, const Epilogue &ep, int64_t batch,
                        bool a_bat, bool b_bat, void *tail_ws, cudaStream_t s) {
     using Q = Cfg<BN, STAGES, BK, F16, PAIR>;
-    auto kernel = gemm_3xtf32_kernel<BN, STAGES, BK, A_MN, B_MN, F16, PAIR>;
+    auto kernel = gemm_3xtf32_kernel<BN, STAGES, BK, A_MN, B_MN, F16, PAIR, ACT>;
     static std::mutex mu;
     static std::vector<char> configured;
     int dev = 0;
@@ -1651,7 +1728,8 @@ static int launch_gemm(const float *ah, const float *al, const float *bh, const 
     const int64_t units = tp.full_tiles + (tiles - tp.full_tiles) * tp.splits;
     const int grid = (int)std::min<int64_t>(units, slots) * (PAIR ? 2 : 1);
     const int vec = (N % 4 == 0) && aligned16(c) && (!ep.bias || aligned16(ep.bias)) &&
-                    (!ep.mask || aligned16(ep.mask)) && (!ep.act || aligned16(ep.act));
+                    (!ep.mask || aligned16(ep.mask)) && (!ep.act || aligned16(ep.act)) &&
+                    (!ep.residual || aligned16(ep.residual));
     float *part = nullptr;
     int *arrivals = nullptr;
     void *owned = nullptr;
@@ -1911,7 +1989,7 @@ static int gemm_presplit_ws(const float *ah, const float *al, const float *bh, c
     J4C_REQUIRE(!act_bits || act, "dot: relu bits need the relu output");
     J4C_REQUIRE(!(mask_bits || act_bits) || batch == 1, "dot: mask bits of a batched product");
     const tc::Epilogue ep{bias,      mask,     act, out_lines, (int)M, out_lines ? out_lines + M + N : nullptr,
-                          mask_bits, act_bits, (int)ceil_div(N, 32)};
+                          mask_bits, act_bits, (int)ceil_div(N, 32), J4C_ACT_NONE, nullptr};
     const bool ab = a_batched != 0, bb = b_batched != 0;
     // CTA pairs (256-row tiles, cta_group::2) for 3xFP16 products whose
     // stored rows (the kernel's M: N when C is stored transposed) fill them
@@ -1928,6 +2006,30 @@ static int gemm_presplit_ws(const float *ah, const float *al, const float *bh, c
     if (variant == 0)
         return tc::launch_gemm_any<256, 2, 32, false>(ah, al, bh, bl, c, M, N, K, a_mn, b_mn, ep, batch, ab, bb, tail_ws, s);
     return tc::launch_gemm_any<256, 4, 16, false>(ah, al, bh, bl, c, M, N, K, a_mn, b_mn, ep, batch, ab, bb, tail_ws, s);
+}
+
+// y = act(A . B + bias) + residual from A's row-line split and B's transposed
+// split (both K-major); z, unless NULL, the pre-activation.
+int tc_gemm_act(const float *ah, const float *al, const float *bh, const float *bl, int64_t M, int64_t K, int64_t N,
+                const float *bias, int act, const float *residual, float *z, float *y, uint32_t *out_lines,
+                cudaStream_t s) {
+    J4C_REQUIRE(aligned16(ah) && aligned16(al) && aligned16(bh) && aligned16(bl),
+                "dot: split operands must be 16-byte aligned");
+    const tc::Epilogue ep{bias,    nullptr, y, out_lines, (int)M, out_lines ? out_lines + M + N : nullptr,
+                          nullptr, nullptr, 0, act,       residual};
+    static const bool pair = [] {
+        const char *v = getenv("J4C_GEMM_PAIR");
+        return !(v && v[0] == '0');
+    }();
+    // the variants of gemm_presplit_ws
+    if (tc::split_fp16() && pair && M >= 2 * tc::BM)
+        return tc::launch_gemm<256, 6, 16, false, false, true, true, true>(ah, al, bh, bl, z, M, N, K, false, ep, 1, false,
+                                                                           false, nullptr, s);
+    if (tc::split_fp16())
+        return tc::launch_gemm<256, 4, 16, false, false, true, false, true>(ah, al, bh, bl, z, M, N, K, false, ep, 1, false,
+                                                                            false, nullptr, s);
+    return tc::launch_gemm<256, 4, 16, false, false, false, false, true>(ah, al, bh, bl, z, M, N, K, false, ep, 1, false,
+                                                                         false, nullptr, s);
 }
 
 int tc_gemm_presplit(const float *ah, const float *al, const float *bh, const float *bl, float *c, int64_t M,

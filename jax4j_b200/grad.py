@@ -534,9 +534,11 @@ def _do_backward(jaxpr: Jaxpr, values: Dict[int, NDArray], seeds: List[NDArray])
     for v, s in zip(jaxpr.outVars, seeds):
         _merge(grads, v.id, s)
     # The equation after which each input's cotangent is complete (its first
-    # consumer): there a CUDA event is recorded on the gradient, so a
-    # collective over it (Lax.psumTree) can start while the rest of the
+    # consumer): inside a pmap there a CUDA event is recorded on the gradient,
+    # so a collective over it (Lax.psumTree) can start while the rest of the
     # backward pass still runs.
+    from .pmap import PmapContext
+    overlap = PmapContext.current() is not None
     in_ids = {v.id for v in jaxpr.inVars}
     last_use = {}
     for i, e in enumerate(jaxpr.equations):
@@ -552,8 +554,7 @@ def _do_backward(jaxpr: Jaxpr, values: Dict[int, NDArray], seeds: List[NDArray])
             g = grads.get(vid)
             if isinstance(g, Deferred):
                 g = grads[vid] = materialize(g)
-            if isinstance(g, ConcreteNDArray) and g.tensor().is_cuda:
-                import torch
+            if overlap and isinstance(g, ConcreteNDArray) and g.tensor().is_cuda:
                 ev = torch.cuda.Event()
                 ev.record(torch.cuda.current_stream(g.tensor().device))
                 g._ready = ev

@@ -1,4 +1,5 @@
-"""Layers that run as single operations: group norm with an activation.
+"""Layers that run as single operations: a dense layer with its bias, activation
+and residual, and group norm with an activation.
 
 Nothing here has a counterpart in the reference, whose layers are chains of
 NDArray operations (examples/MNISTFromScratch.java:103-125).  Under a trace a
@@ -15,7 +16,7 @@ import torch
 from . import _lib
 from ._lib import call
 from .core import (ConcreteNDArray, DType, IllegalArgumentException, NDArray, Primitive, Shape,
-                   UnsupportedOperationException)
+                   UnsupportedOperationException, _dot_raw, _make_splits, _split_of)
 from .tracing import Equation, FfiMeta, TracedNDArray, Tracer, to_var
 
 # J4C_ACT_* (include/jax4j_cuda.h)
@@ -155,3 +156,161 @@ class _GroupNorm(FfiMeta):
         d = x.shape().dimensions()
         y = self.forward([x.reshape(Shape((d[0] * d[1],) + d[2:]))] + list(inputs[1:]), False)[0]
         return y.reshape(x.shape())
+
+
+# ---------------------------------------------------------------------------
+# dense layer
+# ---------------------------------------------------------------------------
+# FLOAT32 products of at most this many multiply-adds run on the CUDA cores
+# straight from their arrays (j4c_dot_act); the tensor-core product first
+# splits both operands (eight launches with the line maxima), which larger ones
+# win back.
+SMALL_PRODUCT = 1 << 28
+
+
+def _small(M: int, K: int, N: int) -> bool:
+    return M * K * N <= SMALL_PRODUCT
+
+
+def dense(x: NDArray, w: NDArray, bias: Optional[NDArray], activation: Optional[str],
+          residual: Optional[NDArray]) -> NDArray:
+    xd, wd = x.shape().dimensions(), w.shape().dimensions()
+    act = activation_code(activation)
+    if len(xd) < 1 or len(wd) != 2:
+        raise IllegalArgumentException(f"dense takes [..., K] and a weight [K, N], got {x.shape()} and {w.shape()}")
+    if xd[-1] != wd[0]:
+        raise IllegalArgumentException(f"dense: inner dimensions differ ({x.shape()} . {w.shape()})")
+    _floating("dense", x, (w, bias, residual))
+    out = Shape(xd[:-1] + (wd[1],))
+    if bias is not None and bias.shape().dimensions() != (wd[1],):
+        raise IllegalArgumentException(f"dense: bias is {bias.shape()}, the outputs are [{wd[1]}]")
+    if residual is not None and residual.shape() != out:
+        raise IllegalArgumentException(f"dense: residual is {residual.shape()}, the output {out}")
+    inputs = [x, w] + [p for p in (bias, residual) if p is not None]
+    return _apply(_Dense(bias is not None, residual is not None, act), inputs, out)
+
+
+def _product(a: ConcreteNDArray, b: ConcreteNDArray, trans_a: bool, trans_b: bool, dev) -> ConcreteNDArray:
+    """op(a) . op(b), which is zeros (of no extent, perhaps) where an extent is 0."""
+    if a._t.numel() and b._t.numel():
+        return _dot_raw(a, b, trans_a, trans_b, dev)
+    return ConcreteNDArray.full(Shape(a._shape[1 if trans_a else 0], b._shape[0 if trans_b else 1]), 0.0, a._dtype, dev)
+
+
+class _Dense(FfiMeta):
+    name = "dense"
+
+    def __init__(self, has_bias: bool, has_residual: bool, act: int):
+        self.has_bias, self.has_residual, self.act = has_bias, has_residual, act
+
+    def _params(self, inputs):
+        return inputs[2] if self.has_bias else None, inputs[-1] if self.has_residual else None
+
+    @staticmethod
+    def _extents(inputs):
+        K, N = inputs[1]._shape._d
+        M = 1
+        for n in inputs[0]._shape._d[:-1]:
+            M *= n
+        return M, K, N
+
+    # The output tells the slope (and is kept anyway) unless a residual was
+    # added to it or the activation is not monotone.
+    def _from_output(self) -> bool:
+        return not self.has_residual and self.act <= ACTIVATIONS["sigmoid"]
+
+    def forward(self, inputs, keep):
+        x, w = inputs[0], inputs[1]
+        bias, residual = self._params(inputs)
+        dev = _device_of(inputs)
+        M, K, N = self._extents(inputs)
+        dt, t = x._dtype, x._t
+        stream = x._stream()
+        x2 = x if x._shape.rank() == 2 else x.reshape(Shape(M, K))
+        out_shape = Shape(x._shape._d[:-1] + (N,))
+        f32, keep_z = dt == DType.FLOAT32, keep and self.act and not self._from_output()
+        y = torch.empty(M * N, dtype=t.dtype, device=t.device) if f32 or keep_z else None
+        z = torch.empty(M * N, dtype=t.dtype, device=t.device) if f32 and keep_z else None
+        bp = bias._t.data_ptr() if bias is not None else None
+        rp = residual._t.data_ptr() if residual is not None else None
+        zp = z.data_ptr() if z is not None else None
+        lines = None
+        if f32 and (_small(M, K, N) or not (M and N and K)):
+            call("j4c_dot_act", t.data_ptr(), w._t.data_ptr(), M, K, N, 0, 0, bp, self.act, rp, zp, y.data_ptr(), stream)
+        elif f32:
+            if keep:  # with those that the gradient's products take, each operand's in one pass
+                _make_splits(x2, ["r", "t" if K < N else "c"])
+                _make_splits(w, ["t", "r"])
+            (xh, xl), (wh, wl) = _split_of(x2, "r"), _split_of(w, "t")
+            lines = torch.empty(M + N + 1, dtype=torch.int32, device=t.device)
+            call("j4c_dot_split_act", xh.data_ptr(), xl.data_ptr(), wh.data_ptr(), wl.data_ptr(), M, K, N, bp, self.act,
+                 rp, zp, y.data_ptr(), lines.data_ptr(), stream)
+        else:
+            c = _product(x2, w, False, False, dev)._t  # FLOAT64: the product, then the rest in place or beside it
+            if keep_z:
+                z = c
+            else:
+                y = c
+            call("j4c_dense_finish", dt.ordinal, c.data_ptr(), M, N, bp, self.act, rp, y.data_ptr(), stream)
+        out = ConcreteNDArray._wrap(y, out_shape, dt, dev)
+        if lines is not None and len(out_shape) == 2:
+            out._lines = lines
+        return out, ((x2, z) if keep else None)
+
+    def vjp(self, inputs, out, saved, g, wanted):
+        x, w = inputs[0], inputs[1]
+        x2, z = saved
+        M, K, N = self._extents(inputs)
+        dt, t, dev = x._dtype, g._t, g._device
+        stream = g._stream()
+        want_bias = self.has_bias and wanted[2]
+        products = wanted[0] or wanted[1]
+        f32 = dt == DType.FLOAT32
+        small = f32 and (_small(M, K, N) or not (M and N and K))
+        dz, dbias, lines = t, None, None
+        if want_bias or (products and (self.act or (f32 and not small))):
+            L = _lib.lib()
+            if self.act:
+                dz = torch.empty(M * N, dtype=t.dtype, device=t.device)
+            if want_bias:
+                dbias = torch.empty(N, dtype=t.dtype, device=t.device)
+            if f32 and not small and products:
+                lines = torch.empty(M + N + 1, dtype=torch.int32, device=t.device)
+            need = L.j4c_dense_grad_workspace(dt.ordinal, M, N) if want_bias else 0
+            ws = torch.empty(need, dtype=torch.uint8, device=t.device) if need else None
+            u = z if z is not None else out._t
+            call("j4c_dense_grad", dt.ordinal, M, N, t.data_ptr(), u.data_ptr() if self.act else None, self.act,
+                 int(z is None), dz.data_ptr() if self.act else None, dbias.data_ptr() if want_bias else None,
+                 lines.data_ptr() if lines is not None else None, ws.data_ptr() if need else None, need, stream)
+        grads: List[Optional[ConcreteNDArray]] = [None, None]
+        if small:
+            if wanted[0]:
+                dx = torch.empty(M * K, dtype=t.dtype, device=t.device)
+                call("j4c_dot_act", dz.data_ptr(), w._t.data_ptr(), M, N, K, 0, 1, None, 0, None, None, dx.data_ptr(),
+                     stream)
+                grads[0] = ConcreteNDArray._wrap(dx, x._shape, dt, dev)
+            if wanted[1]:
+                dw = torch.empty(K * N, dtype=t.dtype, device=t.device)
+                call("j4c_dot_act", x2._t.data_ptr(), dz.data_ptr(), K, M, N, 1, 0, None, 0, None, None, dw.data_ptr(),
+                     stream)
+                grads[1] = ConcreteNDArray._wrap(dw, w._shape, dt, dev)
+        elif products:
+            d = ConcreteNDArray._wrap(dz, Shape(M, N), dt, dev)
+            if f32:
+                d._lines = lines
+                _make_splits(d, (["r"] if wanted[0] else []) + ([("c" if K < N else "t")] if wanted[1] else []))
+            if wanted[0]:
+                grads[0] = _product(d, w, False, True, dev).reshape(x._shape)
+            if wanted[1]:
+                grads[1] = _product(x2, d, True, False, dev)
+        if self.has_bias:
+            grads.append(ConcreteNDArray._wrap(dbias, inputs[2]._shape, dt, dev) if want_bias else None)
+        if self.has_residual:
+            grads.append(g)
+        return grads
+
+    def batch(self, inputs, batched, batch):
+        # x alone, or x and the residual: examples are rows side by side
+        if not batched[0] or batched[1] or (self.has_bias and batched[2]) or (self.has_residual and not batched[-1]):
+            raise UnsupportedOperationException("vmap of dense batches x, together with the residual")
+        return self.forward(inputs, False)[0]

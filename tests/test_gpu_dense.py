@@ -1,0 +1,305 @@
+"""Nn.dense and its gradients against their formulas in 64 bits: the CUDA-core
+products, the tensor-core products and FLOAT64."""
+import numpy as np
+import pytest
+
+from tests.layers_ref import ACTS, U, act
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def J():
+    import jax4j_b200 as j
+    return j
+
+
+def arr(J, x, offset=0):
+    import torch
+    x = np.ascontiguousarray(x)
+    buf = torch.empty(x.size + offset, dtype=torch.from_numpy(x).dtype, device="cuda")
+    buf[offset:] = torch.from_numpy(x.reshape(-1))
+    return J.ConcreteNDArray(buf[offset:], J.Shape(x.shape))
+
+
+def steps(K, tensor):
+    """Error of a K-term product, in half steps of sum |a||b|.  CUDA cores: K
+    roundings of mean zero, 8 standard deviations of their sum.  Tensor cores:
+    48 truncating MMAs of a 256-deep chunk at 3.6e-8 (29 U), the splits' 2^-22
+    (4 U) and K / 256 additions of chunks."""
+    return 33 + K / 256 + 8 if tensor else 8 * np.sqrt(K) + 8
+
+
+def reference(x, w, bias, name, residual, dy, unit, tensor):
+    k = unit / U
+    x, w = x.astype(np.float64), w.astype(np.float64)
+    lead = x.shape[:-1]
+    x = x.reshape(int(np.prod(lead)), x.shape[-1])
+    M, K = x.shape
+    N = w.shape[1]
+    dy = dy.astype(np.float64).reshape(M, N)
+    b = np.zeros(N) if bias is None else bias.astype(np.float64)
+    z = x @ w + b
+    ez = unit * (steps(K, tensor) * (np.abs(x) @ np.abs(w)) + np.abs(z))
+    y, slope, curve, ey, es = act(z, name)
+    ey = 1.2 * ez + k * ey + unit * np.abs(y)
+    out = y if residual is None else y + residual.astype(np.float64).reshape(M, N)
+    res = {"y": (out, ey + unit * np.abs(out))}
+    if residual is None and name in ("tanh", "sigmoid"):
+        # the slope comes from the stored output: 1 - y^2, y (1 - y)
+        es = (2 * np.abs(y) if name == "tanh" else 1.0) * ey / k + 2 * U
+    dz = dy * slope
+    edz = np.abs(dy) * (curve * ez + k * es) + unit * np.abs(dz)
+    res["dx"] = (dz @ w.T, edz @ np.abs(w).T + unit * steps(N, tensor) * (np.abs(dz) @ np.abs(w).T))
+    res["dw"] = (x.T @ dz, np.abs(x).T @ edz + unit * steps(M, tensor) * (np.abs(x).T @ np.abs(dz)))
+    # column sums: a warp's rows, eight warps, the groups: under 32 + M / 8 additions
+    res["dbias"] = (dz.sum(0), edz.sum(0) + unit * (32 + M / 8) * np.abs(dz).sum(0))
+    res["dresidual"] = (dy.reshape(lead + (N,)), 0 * dy.reshape(lead + (N,)))
+    res["y"] = tuple(a.reshape(lead + (N,)) for a in res["y"])
+    res["dx"] = tuple(a.reshape(lead + (K,)) for a in res["dx"])
+    return {n: (v, 1.01 * e + 1e-37) for n, (v, e) in res.items()}
+
+
+def run(J, x, w, bias, name, residual, dy, offset=0):
+    parts = {"dx": x, "dw": w, "dbias": bias, "dresidual": residual}
+    names = [n for n, a in parts.items() if a is not None]
+    arrays = [arr(J, parts[n], offset) for n in names]
+
+    def f(*a):
+        a = dict(zip(names, a))
+        return J.Nn.dense(a["dx"], a["dw"], a.get("dbias"), name, a.get("dresidual"))
+
+    y, pull = J.JAX.vjp(f, *arrays)
+    np.testing.assert_array_equal(f(*arrays).numpy(), y.numpy())
+    DY = arr(J, dy, offset)
+    grads = pull(DY)
+    for a, b in zip(grads, pull(DY)):
+        np.testing.assert_array_equal(a.numpy(), b.numpy())
+    return {"y": y.numpy(), **{n: v.numpy() for n, v in zip(names, grads)}}
+
+
+def check(got, ref):
+    for n, v in got.items():
+        value, tol = ref[n]
+        assert v.shape == value.shape, n
+        if not v.size:
+            continue
+        off = np.abs(v.astype(np.float64) - value) - tol
+        assert np.all(off <= 0), (n, float(off.max()), int((off > 0).sum()), v.size)
+
+
+def make(seed, x_shape, N, dt=np.float32, bias=True, residual=True):
+    r = np.random.default_rng(seed)
+    K = x_shape[-1]
+    x = r.standard_normal(x_shape).astype(dt)
+    w = (r.standard_normal((K, N)) / np.sqrt(max(K, 1))).astype(dt)
+    b = (0.3 * r.standard_normal(N)).astype(dt) if bias else None
+    res = r.standard_normal(x_shape[:-1] + (N,)).astype(dt) if residual else None
+    return x, w, b, res, r.standard_normal(x_shape[:-1] + (N,)).astype(dt)
+
+
+SMALL = [((1, 1), 1), ((7,), 5), ((1, 784), 512), ((2, 333), 2400), ((3, 100), 10), ((4, 64), 4736), ((7, 50), 1184),
+         ((16, 257), 130), ((17, 33), 65), ((2, 3, 20), 9), ((64, 64), 64), ((100, 1), 7), ((65, 1025), 66), ((5, 0), 4),
+         ((0, 3), 4), ((3, 4), 0), ((256, 784), 512), ((700, 16), 300)]
+
+
+@pytest.mark.parametrize("shape,N", SMALL, ids=[f"{'x'.join(map(str, s))}x{n}" for s, n in SMALL])
+@pytest.mark.parametrize("f64", [False, True], ids=["f32", "f64"])
+def test_small_products(J, shape, N, f64):
+    name = ACTS[2 + (sum(shape) + N) % 4]
+    x, w, b, res, dy = make(sum(shape) + N, shape, N, np.float64 if f64 else np.float32, bias=N % 2 == 0,
+                            residual=sum(shape) % 2 == 0)
+    check(run(J, x, w, b, name, res, dy), reference(x, w, b, name, res, dy, 2.0 ** -53 if f64 else U, False))
+
+
+LARGE = [((1, 5), 3), ((128, 64), 256), ((130, 64), 260), ((257, 1000), 513), ((300, 513), 1000), ((3, 100, 48), 77),
+         ((1024, 300), 1000), ((600, 2048), 512)]
+
+
+@pytest.mark.parametrize("shape,N", LARGE, ids=[f"{'x'.join(map(str, s))}x{n}" for s, n in LARGE])
+@pytest.mark.parametrize("name", ["none", "tanh", "gelu"])
+@pytest.mark.parametrize("extras", [True, False])
+def test_tensor_core_products(J, monkeypatch, shape, N, name, extras):
+    from jax4j_b200 import layers
+    monkeypatch.setattr(layers, "SMALL_PRODUCT", 0)
+    x, w, b, res, dy = make(sum(shape) + N, shape, N, bias=extras, residual=extras)
+    check(run(J, x, w, b, name, res, dy), reference(x, w, b, name, res, dy, U, True))
+
+
+@pytest.mark.parametrize("name", ACTS)
+@pytest.mark.parametrize("extras", ["both", "bias", "residual", "none"])
+@pytest.mark.parametrize("small", [True, False])
+def test_activations_and_optional_inputs(J, monkeypatch, name, extras, small):
+    from jax4j_b200 import layers
+    monkeypatch.setattr(layers, "SMALL_PRODUCT", layers.SMALL_PRODUCT if small else 0)
+    x, w, b, res, dy = make(3, (70, 40), 96, bias=extras in ("both", "bias"), residual=extras in ("both", "residual"))
+    if name == "relu":  # where either slope is right: dy is 0 there
+        z, ez = reference(x, w, b, "none", None, dy, U, not small)["y"]
+        dy[np.abs(z) <= ez] = 0
+    check(run(J, x, w, b, name, res, dy), reference(x, w, b, name, res, dy, U, not small))
+
+
+@pytest.mark.parametrize("small", [True, False])
+@pytest.mark.parametrize("offset", [1, 2])
+def test_unaligned_arrays(J, monkeypatch, small, offset):
+    from jax4j_b200 import layers
+    monkeypatch.setattr(layers, "SMALL_PRODUCT", layers.SMALL_PRODUCT if small else 0)
+    for shape, N in (((70, 40), 96), ((2, 64), 4736)):
+        x, w, b, res, dy = make(5, shape, N)
+        check(run(J, x, w, b, "silu", res, dy, offset), reference(x, w, b, "silu", res, dy, U, not small))
+
+
+def test_at_the_border_between_the_products(J):
+    """K = 1024: 512 x 512 outputs are the last on the CUDA cores, 513 the first beyond."""
+    from jax4j_b200 import layers
+    assert layers.SMALL_PRODUCT == 512 * 1024 * 512
+    for M in (512, 513):
+        x, w, b, res, dy = make(M, (M, 1024), 512)
+        check(run(J, x, w, b, "gelu", res, dy), reference(x, w, b, "gelu", res, dy, U, M == 513))
+
+
+@pytest.mark.parametrize("small", [True, False])
+def test_non_finite_values(J, monkeypatch, small):
+    """Infinities and NaN reach exactly the outputs that depend on them."""
+    from jax4j_b200 import layers
+    monkeypatch.setattr(layers, "SMALL_PRODUCT", layers.SMALL_PRODUCT if small else 0)
+    x, w, b, res, dy = make(6, (40, 50), 60)
+    x[3, 4], x[9, 0] = np.inf, np.nan
+    w[7, 11] = -np.inf
+    y = J.Nn.dense(arr(J, x), arr(J, w), arr(J, b), "sigmoid", arr(J, res)).numpy()
+    with np.errstate(invalid="ignore"):
+        z = x.astype(np.float64) @ w.astype(np.float64) + b
+    bad = np.isnan(z)
+    assert np.array_equal(np.isnan(y), bad) and bad.any()
+    np.testing.assert_allclose(y[~bad], (1 / (1 + np.exp(-z)) + res)[~bad], rtol=1e-5, atol=1e-5)
+
+
+def test_line_words_of_the_output(J):
+    """What a later product's split takes instead of a max pass, NaN/Inf flag included."""
+    import torch
+    from jax4j_b200 import _lib
+    for special in (False, True):
+        x, w, b, res, _ = make(7, (513, 1024), 515)
+        if special:
+            res[5, 6] = np.inf
+        for name in ("silu", "none"):
+            out = J.Nn.dense(arr(J, x), arr(J, w), arr(J, b), name, arr(J, res))
+            assert out._lines is not None
+            lines = torch.empty(513 + 515 + 1, dtype=torch.int32, device="cuda")
+            _lib.call("j4c_split_lines", out.data_ptr(), 513, 515, lines.data_ptr(), out._stream())
+            np.testing.assert_array_equal(out._lines.cpu().numpy()[:-1], lines.cpu().numpy()[:-1])
+            assert bool(out._lines[-1].item()) == bool(lines[-1].item()) == special
+
+
+def test_gradient_line_words(J):
+    import torch
+    from jax4j_b200 import _lib
+    r = np.random.default_rng(8)
+    for M, N in ((1, 1), (33, 255), (100, 257), (700, 1028)):
+        dy, z = (r.standard_normal((M, N)).astype(np.float32) for _ in range(2))
+        if M == 100:
+            dy[50, 100] = np.nan
+        DY, Z = arr(J, dy), arr(J, z)
+        dz = torch.empty(M * N, device="cuda")
+        db = torch.empty(N, device="cuda")
+        lines, want = (torch.empty(M + N + 1, dtype=torch.int32, device="cuda") for _ in range(2))
+        need = _lib.lib().j4c_dense_grad_workspace(0, M, N)
+        ws = torch.empty(max(need, 1), dtype=torch.uint8, device="cuda")
+        s = DY._stream()
+        _lib.call("j4c_dense_grad", 0, M, N, DY.data_ptr(), Z.data_ptr(), 5, 0, dz.data_ptr(), db.data_ptr(),
+                  lines.data_ptr(), ws.data_ptr(), need, s)
+        _lib.call("j4c_split_lines", dz.data_ptr(), M, N, want.data_ptr(), s)
+        np.testing.assert_array_equal(lines.cpu().numpy()[:-1], want.cpu().numpy()[:-1])
+        assert bool(lines[-1].item()) == bool(want[-1].item()) == (M == 100)
+
+
+@pytest.mark.parametrize("name", ACTS)
+def test_gradients_against_differences(J, name):
+    x, w, b, res, dy = make(9, (3, 5), 4, np.float64)
+    got = run(J, x, w, b, name, res, dy)
+
+    def f(*a):
+        return float((J.Nn.dense(*[arr(J, t) for t in a[:3]], name, arr(J, a[3])).numpy() * dy).sum())
+
+    step = 1e-5
+    for i, n in enumerate(("dx", "dw", "dbias", "dresidual")):
+        args = [x, w, b, res]
+        for at in np.ndindex(args[i].shape):
+            up, down = ([a.copy() for a in args] for _ in range(2))
+            up[i][at] += step
+            down[i][at] -= step
+            assert abs((f(*up) - f(*down)) / (2 * step) - got[n][at]) <= 1e-7, (n, at)
+
+
+@pytest.mark.parametrize("small", [True, False])
+def test_inside_transformations(J, monkeypatch, small):
+    from jax4j_b200 import layers
+    monkeypatch.setattr(layers, "SMALL_PRODUCT", layers.SMALL_PRODUCT if small else 0)
+    x, w, b, res, _ = make(10, (6, 8, 32), 32)
+    X, W, B, R = (arr(J, a) for a in (x, w, b, res))
+    layer = lambda a: J.Nn.dense(a, W, B, "silu", a)  # noqa: E731
+    direct = layer(X).numpy()
+    np.testing.assert_array_equal(J.JAX.jit(layer)(X).numpy(), direct)
+    loss = lambda a: layer(layer(a)).tanh().sum()  # noqa: E731
+    g = J.JAX.grad(loss)(X).numpy()
+    np.testing.assert_array_equal(J.JAX.grad(J.JAX.checkpoint(loss))(X).numpy(), g)
+    np.testing.assert_array_equal(J.JAX.vmap(layer)(X.reshape(J.Shape(2, 3, 8, 32))).numpy().reshape(6, 8, 32), direct)
+    # the same chain of the framework's own operations
+    two = X.reshape(J.Shape(48, 32))
+    chain = lambda a: [a.dot(W).add(B)][0]  # noqa: E731
+
+    def plain(a):
+        for _ in range(2):
+            z = chain(a)
+            a = z.mul(z.sigmoid()).add(a)
+        return a.tanh().sum()
+
+    np.testing.assert_allclose(g.reshape(48, 32), J.JAX.grad(plain)(two).numpy(), rtol=1e-4, atol=1e-5)
+    devs = [J.Device(None), J.Device(None)]
+    gp = J.JAX.grad(lambda a: J.JAX.pmap(lambda p: loss(p), devs)(a).sum())(X.reshape(J.Shape(2, 3, 8, 32)))
+    np.testing.assert_allclose(gp.numpy().reshape(6, 8, 32), g, rtol=1e-5, atol=1e-6)
+
+
+def test_only_the_wanted_gradients(J):
+    x, w, b, _, dy = make(11, (600, 700), 800, residual=False)
+    X, W, B = arr(J, x), arr(J, w), arr(J, b)
+    full = run(J, x, w, b, "gelu", None, dy)
+    DY = arr(J, dy)
+    for f, arg, n in ((lambda a: J.Nn.dense(a, W, B, "gelu"), X, "dx"), (lambda a: J.Nn.dense(X, a, B, "gelu"), W, "dw"),
+                      (lambda a: J.Nn.dense(X, W, a, "gelu"), B, "dbias")):
+        np.testing.assert_array_equal(J.JAX.vjp(f, arg)[1](DY)[0].numpy(), full[n])
+
+
+@pytest.mark.parametrize("shape,N", [((64, 200), 100), ((512, 1024), 600)])
+def test_recorded_and_on_another_stream(J, shape, N):
+    import torch
+    from jax4j_b200.graphs import CapturedStep
+    x, w, b, res, dy = make(12, shape, N)
+    r = np.random.default_rng(13)
+
+    def step(*a):
+        y, pull = J.JAX.vjp(lambda p, q, s, t: J.Nn.dense(p, q, s, "gelu", t), *a[:4])
+        return [y, *pull(a[4])[:3]]
+
+    args = [arr(J, a) for a in (x, w, b, res, dy)]
+    y, pull = J.JAX.vjp(lambda p, q: J.Nn.dense(p, q, args[2], "gelu"), args[0], args[1])
+    graphs = [CapturedStep(step, [J.ConcreteNDArray(a.tensor().clone(), a.shape()) for a in args]) for _ in range(2)]
+    for _ in range(2):
+        args = [arr(J, r.standard_normal(a.shape().dimensions()).astype(np.float32)) for a in args]
+        want = [a.numpy() for a in step(*args)]
+        for gr in graphs:
+            for i, a in enumerate(args):
+                gr.set_input(i, a)
+        for out in [gr() for gr in graphs]:
+            for a, v in zip(out, want):
+                np.testing.assert_array_equal(a.numpy(), v)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            other = step(*args)
+        side.synchronize()
+        for a, v in zip(other, want):
+            np.testing.assert_array_equal(a.numpy(), v)
+    assert np.isfinite(pull(arr(J, dy))[0].numpy()).all()
+    for gr in graphs:
+        gr.release()

@@ -40,6 +40,49 @@ def test_group_norm_refusals():
             J.Nn.groupNorm(x, 2, eps=eps)
 
 
+def test_dense_refusals():
+    bad = J.IllegalArgumentException
+    x, w = leaf(2, 3, 8), leaf(8, 5)
+    for args, text in (((x, leaf(7, 5)), "inner dimensions"), ((x, leaf(8)), "weight"), ((leaf(), w), "takes"),
+                       ((x, w, leaf(8)), "bias is"), ((x, w, leaf(1, 5)), "bias is"),
+                       ((x, w, None, "none", leaf(2, 3, 8)), "residual is"), ((x, w, None, "none", leaf(5)), "residual is"),
+                       ((x, w, None, "selu"), "activation"), ((leaf(2, 8, dtype=J.DType.INT64), w), "FLOAT32 or FLOAT64"),
+                       ((x, leaf(8, 5, dtype=J.DType.FLOAT64)), "one floating dtype"),
+                       ((x, w, leaf(5, dtype=J.DType.FLOAT64)), "one floating dtype")):
+        with pytest.raises(bad, match=text):
+            J.Nn.dense(*args)
+
+
+def test_vjp_refusals():
+    _, pull = J.JAX.vjp(lambda a: a, leaf(3))
+    for seeds, text in (((), "as many cotangents"), ((leaf(4),), "cotangent"), ((leaf(3, dtype=J.DType.FLOAT64),), "cotangent")):
+        with pytest.raises(J.IllegalArgumentException, match=text):
+            pull(*seeds)
+
+
+def test_dense_c_entries_refuse_bad_arguments():
+    L = _lib.lib()
+    fake = C.c_void_p(0x1000)
+
+    def told(rc, text, code=_lib.E_INVALID):
+        assert rc == code and text in L.j4c_last_error().decode(), (rc, L.j4c_last_error())
+
+    told(L.j4c_dot_act(fake, fake, -1, 2, 3, 0, 0, None, 0, None, None, fake, None), "negative")
+    told(L.j4c_dot_act(fake, fake, 1, 2, 3, 0, 0, None, 6, None, None, fake, None), "activation")
+    told(L.j4c_dot_act(fake, None, 1, 2, 3, 0, 0, None, 0, None, None, fake, None), "NULL")
+    told(L.j4c_dot_act(fake, fake, 1, 2, 3, 0, 0, None, 0, None, None, None, None), "NULL")
+    told(L.j4c_dot_act(fake, fake, 1 << 33, 2, 3, 0, 0, None, 0, None, None, fake, None), "too many", _lib.E_UNSUPPORTED)
+    told(L.j4c_dot_split_act(fake, fake, fake, fake, 2, 0, 3, None, 0, None, None, fake, None, None), "K = 0")
+    told(L.j4c_dot_split_act(fake, None, fake, fake, 2, 4, 3, None, 0, None, None, fake, None, None), "NULL")
+    told(L.j4c_dot_split_act(fake, fake, fake, fake, 2, 4, 3, None, -1, None, None, fake, None, None), "activation")
+    told(L.j4c_dense_finish(2, fake, 2, 3, None, 0, None, fake, None), "FLOAT32 or FLOAT64")
+    told(L.j4c_dense_finish(1, fake, 2, 3, None, 0, None, None, None), "NULL")
+    told(L.j4c_dense_grad(0, 2, 3, fake, None, 3, 0, fake, None, None, None, 0, None), "NULL")
+    told(L.j4c_dense_grad(0, 2, 3, fake, fake, 5, 1, fake, None, None, None, 0, None), "does not tell")
+    told(L.j4c_dense_grad(1, 2, 3, fake, fake, 2, 1, fake, None, fake, None, 0, None), "line words")
+    told(L.j4c_dense_grad(0, 200, 3, fake, fake, 2, 1, fake, fake, None, None, 0, None), "workspace")
+
+
 def test_layers_are_one_equation():
     jaxpr = J.JAX.make_jaxpr(lambda a: J.Nn.groupNorm(a, 2, leaf(8), activation="silu").tanh(), leaf(2, 3, 8))
     kinds = [e.primitive for e in jaxpr.equations]
