@@ -392,11 +392,11 @@ class ConcreteNDArray(NDArray):
 
     def __init__(self, data, shape=None, dtype: DType = None, device: Device = None):
         if device is None:
-            device = Device.defaultDevice()
+            device = Device._default or Device.defaultDevice()
         if isinstance(data, torch.Tensor):
             t = data
             if dtype is None:
-                dtype = _from_torch(t.dtype)
+                dtype = _OF_TORCH.get(t.dtype) or _from_torch(t.dtype)
             if t.dtype is not dtype.torch or not t.is_cuda or t.get_device() != device.ordinal():
                 t = t.to(device=device.torch_device(), dtype=dtype.torch)
             if t.dim() != 1:

@@ -128,78 +128,81 @@ __global__ void __launch_bounds__(kRowsThreads) rows_kernel(const Product p) {
 
 // The general form, op(A) [M, K] . op(B) [K, N] with either operand stored
 // transposed: 64 x 64 tiles of 128 threads (8 x 4 results each), K in steps of
-// 16 through two shared buffers, the next step's values in registers meanwhile.
+// 16 through a ring of four buffers filled by asynchronous copies, three steps
+// ahead: a CTA's share of K is a few steps, each bound by the copies' latency.
 constexpr int kTM = 64, kTN = 64, kTK = 16, kPitch = 68;  // a row of a buffer: padded, 16-byte multiples
+constexpr int kRing = 4;
+struct TileStep {
+    float A[kTK][kPitch], B[kTK][kPitch];
+};
+__device__ __forceinline__ void copy4_async(float *to, const float *from) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from)
+                 : "memory");
+}
 template <bool TA, bool TB>
 __global__ void __launch_bounds__(128) tile_kernel(const Product p) {
-    __shared__ __align__(16) float As[2][kTK][kPitch], Bs[2][kTK][kPitch];
-    __shared__ __align__(16) float part[kTM][kTN];
+    __shared__ __align__(16) TileStep ring[kRing];
+    float(*const part)[kTN] = reinterpret_cast<float(*)[kTN]>(&ring[0]);  // once the ring has been read
+    static_assert(sizeof(ring) >= kTM * kTN * sizeof(float), "the tile's sums take the ring's place");
     const cg::cluster_group cluster = cg::this_cluster();
     const int ranks = cluster.num_blocks(), rank = cluster.block_rank();
     const int tid = threadIdx.x, tx = tid % 16, ty = tid / 16;
     const int64_t n0 = (int64_t)(blockIdx.x / ranks) * kTN, m0 = (int64_t)blockIdx.y * kTM;
     const int64_t k0 = p.K * rank / ranks, k1 = p.K * (rank + 1) / ranks;
-    // value i of this thread's eight of a step: an operand stored along K goes
-    // by rows of 16 K values, one stored across it by rows of 64
-    auto a_at = [&](int i, int &m, int &k) {
-        const int e = tid + 128 * i;
-        if (TA) k = e / kTM, m = e % kTM;
-        else m = e / kTK, k = e % kTK;
-    };
-    auto b_at = [&](int i, int &n, int &k) {
-        const int e = tid + 128 * i;
-        if (TB) n = e / kTK, k = e % kTK;
-        else k = e / kTN, n = e % kTN;
-    };
-    float ra[8], rb[8];
-    auto load = [&](int64_t kb) {
+    const int steps = (int)((k1 - k0 + kTK - 1) / kTK);
+    // This thread copies eight values of each operand a step: of one stored
+    // along K, one K of rows 8 apart; of one stored across, one row of Ks 2 apart.
+    const int am = TA ? tid % kTM : tid / kTK, ak = TA ? tid / kTM : tid % kTK;
+    const int bn = TB ? tid / kTK : tid % kTN, bk = TB ? tid % kTK : tid / kTN;
+    const float *a = p.A + (TA ? (k0 + ak) * p.M + m0 + am : (m0 + am) * p.K + k0 + ak);
+    const float *b = p.B + (TB ? (n0 + bn) * p.K + k0 + bk : (k0 + bk) * p.N + n0 + bn);
+    const int64_t a_next = TA ? 2 * p.M : 8 * p.K, b_next = TB ? 8 * p.K : 2 * p.N;    // to the thread's next value
+    const int64_t a_step = TA ? kTK * p.M : kTK, b_step = TB ? kTK : kTK * p.N;        // to the next step
+    auto fetch = [&](int step) {
+        if (step < steps) {
+            TileStep &to = ring[step % kRing];
+            const int64_t kb = k0 + (int64_t)step * kTK;
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            int m, n, k;
-            a_at(i, m, k);
-            ra[i] = m0 + m < p.M && kb + k < k1 ? p.A[TA ? (kb + k) * p.M + m0 + m : (m0 + m) * p.K + kb + k] : 0.0f;
-            b_at(i, n, k);
-            rb[i] = n0 + n < p.N && kb + k < k1 ? p.B[TB ? (n0 + n) * p.K + kb + k : (kb + k) * p.N + n0 + n] : 0.0f;
-        }
-    };
-    auto store = [&](int buf) {
+            for (int i = 0; i < 8; i++) {
+                const int m = TA ? am : am + 8 * i, k = TA ? ak + 2 * i : ak;
+                if (m0 + m < p.M && kb + k < k1) copy4_async(&to.A[k][m], a + i * a_next);
+                else to.A[k][m] = 0.0f;
+            }
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            int m, n, k;
-            a_at(i, m, k);
-            As[buf][k][m] = ra[i];
-            b_at(i, n, k);
-            Bs[buf][k][n] = rb[i];
+            for (int i = 0; i < 8; i++) {
+                const int n = TB ? bn + 8 * i : bn, k = TB ? bk : bk + 2 * i;
+                if (n0 + n < p.N && kb + k < k1) copy4_async(&to.B[k][n], b + i * b_next);
+                else to.B[k][n] = 0.0f;
+            }
+            a += a_step, b += b_step;
         }
+        asm volatile("cp.async.commit_group;" ::: "memory");
     };
     float acc[8][4];
 #pragma unroll
     for (int i = 0; i < 8; i++)
 #pragma unroll
         for (int j = 0; j < 4; j++) acc[i][j] = 0.0f;
-    if (k0 < k1) {
-        load(k0);
-        store(0);
-    }
-    __syncthreads();
-    int buf = 0;
-    for (int64_t kb = k0; kb < k1; kb += kTK, buf ^= 1) {
-        const bool more = kb + kTK < k1;
-        if (more) load(kb + kTK);
+#pragma unroll
+    for (int i = 0; i < kRing - 1; i++) fetch(i);
+    for (int step = 0; step < steps; step++) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 2) : "memory");
+        __syncthreads();  // this step's copies are everyone's, and the buffer of the step before has been read
+        fetch(step + kRing - 1);
+        const TileStep &at = ring[step % kRing];
 #pragma unroll
         for (int k = 0; k < kTK; k++) {
-            const float4 a0 = *reinterpret_cast<const float4 *>(&As[buf][k][ty * 8]);
-            const float4 a1 = *reinterpret_cast<const float4 *>(&As[buf][k][ty * 8 + 4]);
-            const float4 b0 = *reinterpret_cast<const float4 *>(&Bs[buf][k][tx * 4]);
-            const float a[8] = {a0.x, a0.y, a0.z, a0.w, a1.x, a1.y, a1.z, a1.w}, b[4] = {b0.x, b0.y, b0.z, b0.w};
+            const float4 a0 = *reinterpret_cast<const float4 *>(&at.A[k][ty * 8]);
+            const float4 a1 = *reinterpret_cast<const float4 *>(&at.A[k][ty * 8 + 4]);
+            const float4 b0 = *reinterpret_cast<const float4 *>(&at.B[k][tx * 4]);
+            const float av[8] = {a0.x, a0.y, a0.z, a0.w, a1.x, a1.y, a1.z, a1.w}, bv[4] = {b0.x, b0.y, b0.z, b0.w};
 #pragma unroll
             for (int i = 0; i < 8; i++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) acc[i][j] = fmaf(a[i], b[j], acc[i][j]);
+                for (int j = 0; j < 4; j++) acc[i][j] = fmaf(av[i], bv[j], acc[i][j]);
         }
-        if (more) store(buf ^ 1);
-        __syncthreads();
     }
+    __syncthreads();
 #pragma unroll
     for (int i = 0; i < 8; i++)
         *reinterpret_cast<float4 *>(&part[ty * 8 + i][tx * 4]) = make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
@@ -427,9 +430,13 @@ int dense_grad(int64_t M, int64_t N, const T *dy, const T *u, int act, int from_
     T *sums = dbias ? (groups == 1 ? dbias : static_cast<T *>(ws)) : nullptr;
     const GradArgs<T> a{dy, act == J4C_ACT_NONE ? nullptr : u, dz, sums, lines, M, N, groups, act, from_output};
     constexpr int W = 16 / sizeof(T);
-    const bool vec = N % W == 0 && aligned16(dy) && (!u || aligned16(u)) && (!dz || aligned16(dz));
+    auto fits = [&](int v) {
+        auto ok = [&](const void *p) { return reinterpret_cast<uintptr_t>(p) % (v * sizeof(T)) == 0; };
+        return N % v == 0 && ok(dy) && ok(u) && ok(dz);
+    };
     const dim3 grid((unsigned)ceil_div(N, 256), (unsigned)groups);
-    if (vec) dense_grad_kernel<T, W><<<grid, 256, 0, s>>>(a);
+    if (fits(W)) dense_grad_kernel<T, W><<<grid, 256, 0, s>>>(a);
+    else if (fits(2)) dense_grad_kernel<T, 2><<<grid, 256, 0, s>>>(a);
     else dense_grad_kernel<T, 1><<<grid, 256, 0, s>>>(a);
     J4C_LAUNCH_CHECK("dense_grad_kernel");
     if (dbias && groups > 1) {

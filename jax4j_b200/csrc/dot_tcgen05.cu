@@ -144,6 +144,9 @@ struct Cfg {
     static constexpr int TMEM_COLS = 2 * BN;  // two partial-sum buffers
     static constexpr int COLS_PER_WARP = BN / 2;  // each epilogue warp owns half the columns
     static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 256;
+    // with an activation epilogue, a 32 x 33 staging area of every epilogue warp
+    static constexpr int ACT_SMEM_BYTES = SMEM_BYTES + kEpiWarps * 32 * 33 * 4;
+    static_assert(ACT_SMEM_BYTES <= 232448 || STAGES * STAGE_BYTES > 196608, "shared memory budget");
     static_assert(TMEM_COLS == 256 || TMEM_COLS == 512, "TMEM allocation must be a power of 2");
     static_assert(SMEM_BYTES <= 232448, "shared memory budget");
 };
@@ -920,59 +923,72 @@ gemm_3xtf32_kernel(const __grid_constant__ CUtensorMap tAh, const __grid_constan
             // when act is written; 0 outside C), from which the line maxima are
             // taken.
             if constexpr (ACT) {
-                // eight columns at a time: the activation's branch is taken once
-                // for them, and few values live beside the accumulators
-                const size_t base = (size_t)row * (size_t)N + col0;
+                // The accumulators are a row a lane; the rest of the work is done a
+                // column a lane, 32 columns at a time through the warp's own shared
+                // memory, so that every load and store is a run of 128 bytes
+                // whatever N's alignment (a row a lane: [8192,4096]x[4096,4096] gelu
+                // with a residual 860 us, [4099,1000]x[1000,2050] 260 us).  The next
+                // eight rows' residuals are loaded while eight are worked on.
+                float *const stage = reinterpret_cast<float *>(smem + STAGES * Q::STAGE_BYTES + 256) + ew * (32 * 33);
+                const int row0 = mt * Q::TM + (int)crank * BM + q * 32;
+                const int rows = min(32, M - row0);  // of the warp's 32; may be below 1
+                uint32_t rtop = 0;
+                bool nonfinite = false;
 #pragma unroll
-                for (int c = 0; c < Q::COLS_PER_WARP / 8; c++) {
-                    float x[8];
+                for (int g = 0; g < Q::COLS_PER_WARP / 32; g++) {
+                    const int col = col0 + g * 32 + lane;
+                    __syncwarp();  // the chunk before has been read
 #pragma unroll
-                    for (int e = 0; e < 8; e++) x[e] = acc[8 * c + e];
-                    if (vec_full) {
+                    for (int j = 0; j < 32; j++) stage[lane * 33 + j] = acc[g * 32 + j];
+                    __syncwarp();
+                    const bool col_ok = col < N;
+                    const float b = ep.bias && col_ok ? __ldg(ep.bias + col) : 0.0f;
+                    const size_t base = (size_t)row0 * (size_t)N + col;
+                    uint32_t ctop = 0;
+                    float res[8];
+                    auto residuals = [&](int r0) {
 #pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            float *const xh = x + 4 * h;
-                            if (ep.bias) {
-                                const float4 b = __ldg(reinterpret_cast<const float4 *>(ep.bias + col0) + 2 * c + h);
-                                xh[0] = __fadd_rn(xh[0], b.x); xh[1] = __fadd_rn(xh[1], b.y);
-                                xh[2] = __fadd_rn(xh[2], b.z); xh[3] = __fadd_rn(xh[3], b.w);
-                            }
-                            if (Cb)
-                                reinterpret_cast<float4 *>(Cb + base)[2 * c + h] = make_float4(xh[0], xh[1], xh[2], xh[3]);
+                        for (int i = 0; i < 8; i++)
+                            res[i] = col_ok && r0 + i < rows ? __ldg(ep.residual + base + (size_t)(r0 + i) * N) : 0.0f;
+                    };
+                    if (ep.residual) residuals(0);
+#pragma unroll 1
+                    for (int r0 = 0; r0 < rows; r0 += 8) {
+                        float x[8], add[8];
+#pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            add[i] = res[i];
+                            x[i] = stage[(r0 + i) * 33 + lane];
+                            if (ep.bias) x[i] = __fadd_rn(x[i], b);
+                        }
+                        if (ep.residual && r0 + 8 < rows) residuals(r0 + 8);
+                        if (Cb) {
+#pragma unroll
+                            for (int i = 0; i < 8; i++)
+                                if (col_ok && r0 + i < rows) Cb[base + (size_t)(r0 + i) * N] = x[i];
                         }
                         act_values(ep.act_kind, x);
 #pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            float *const xh = x + 4 * h;
-                            if (ep.residual) {
-                                const float4 r = __ldg(reinterpret_cast<const float4 *>(ep.residual + base) + 2 * c + h);
-                                xh[0] = __fadd_rn(xh[0], r.x); xh[1] = __fadd_rn(xh[1], r.y);
-                                xh[2] = __fadd_rn(xh[2], r.z); xh[3] = __fadd_rn(xh[3], r.w);
-                            }
-                            reinterpret_cast<float4 *>(ep.act + base)[2 * c + h] = make_float4(xh[0], xh[1], xh[2], xh[3]);
-                        }
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 8; e++) {
-                            const int j = 8 * c + e;
-                            if (row_ok && col0 + j < N) {
-                                if (ep.bias) x[e] = __fadd_rn(x[e], __ldg(ep.bias + col0 + j));
-                                if (Cb) Cb[base + j] = x[e];
-                            }
-                        }
-                        act_values(ep.act_kind, x);
-#pragma unroll
-                        for (int e = 0; e < 8; e++) {
-                            const int j = 8 * c + e;
-                            if (row_ok && col0 + j < N) {
-                                if (ep.residual) x[e] = __fadd_rn(x[e], __ldg(ep.residual + base + j));
-                                ep.act[base + j] = x[e];
+                        for (int i = 0; i < 8; i++) {
+                            const bool in = col_ok && r0 + i < rows;
+                            if (ep.residual) x[i] = __fadd_rn(x[i], add[i]);
+                            if (in) ep.act[base + (size_t)(r0 + i) * N] = x[i];
+                            if (ep.out_lines) {
+                                nonfinite |= in && (__float_as_uint(x[i]) & 0x7F800000u) == 0x7F800000u;
+                                const uint32_t m = in ? finite_bits(x[i]) : 0u;
+                                ctop = max(ctop, m);
+                                const uint32_t rm = __reduce_max_sync(0xffffffffu, m);
+                                if (lane == r0 + i) rtop = max(rtop, rm);
                             }
                         }
                     }
-#pragma unroll
-                    for (int e = 0; e < 8; e++) acc[8 * c + e] = x[e];
+                    if (ep.out_lines && col_ok && ctop) atomicMax(ep.out_lines + ep.out_rows + col, ctop);
                 }
+                if (ep.out_lines) {
+                    if (__any_sync(0xffffffffu, nonfinite) && lane == 0) atomicOr(ep.out_flag, 1u);
+                    if (row_ok && rtop) atomicMax(ep.out_lines + row, rtop);
+                }
+                continue;
             } else if (vec_full) {
                 const size_t base = (size_t)row * (size_t)N + col0;
 #pragma unroll
@@ -1696,6 +1712,7 @@ static int launch_gemm(const float *ah, const float *al, const float *bh, const 
                        bool a_bat, bool b_bat, void *tail_ws, cudaStream_t s) {
     using Q = Cfg<BN, STAGES, BK, F16, PAIR>;
     auto kernel = gemm_3xtf32_kernel<BN, STAGES, BK, A_MN, B_MN, F16, PAIR, ACT>;
+    constexpr int smem_bytes = ACT ? Q::ACT_SMEM_BYTES : Q::SMEM_BYTES;
     static std::mutex mu;
     static std::vector<char> configured;
     int dev = 0;
@@ -1704,7 +1721,7 @@ static int launch_gemm(const float *ah, const float *al, const float *bh, const 
         std::lock_guard<std::mutex> lock(mu);
         if ((int)configured.size() <= dev) configured.resize(dev + 1, 0);
         if (!configured[dev]) {
-            J4C_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Q::SMEM_BYTES));
+            J4C_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes));
             configured[dev] = 1;
         }
     }
@@ -1751,7 +1768,7 @@ static int launch_gemm(const float *ah, const float *al, const float *bh, const 
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3((unsigned)grid);
         cfg.blockDim = dim3(kThreads);
-        cfg.dynamicSmemBytes = Q::SMEM_BYTES;
+        cfg.dynamicSmemBytes = smem_bytes;
         cfg.stream = s;
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -1767,7 +1784,7 @@ static int launch_gemm(const float *ah, const float *al, const float *bh, const 
                                     status, wait_limit_ns(), ft, tp.splits, part, arrivals, ahdr, bhdr));
         count_launch();
     } else {
-        kernel<<<grid, kThreads, Q::SMEM_BYTES, s>>>(mAh, mAl, mBh, mBl, c, (int)M, (int)N, (int)K, (int)num_kb,
+        kernel<<<grid, kThreads, smem_bytes, s>>>(mAh, mAl, mBh, mBl, c, (int)M, (int)N, (int)K, (int)num_kb,
                                                      store_t ? 0 : vec, store_t ? 1 : 0, ep, (int)batch,
                                                      a_bat ? 1 : 0, b_bat ? 1 : 0, status, wait_limit_ns(),
                                                      (int)tp.full_tiles, tp.splits, part, arrivals, ahdr, bhdr);

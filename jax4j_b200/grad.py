@@ -518,13 +518,35 @@ def _relu_fed_dots(jaxpr: Jaxpr, need) -> Dict[int, object]:
     return found
 
 
+def _pmap_context():
+    from .pmap import PmapContext
+    return PmapContext.current()
+
+
 def do_backward(jaxpr: Jaxpr, values: Dict[int, NDArray], seeds: List[NDArray]) -> List[NDArray]:
     """Grad.doBackward (Grad.java:154-189)."""
+    if (len(jaxpr.equations) == 1 and jaxpr.equations[0].primitive == Primitive.FFI_CALL and len(seeds) == 1
+            and jaxpr.outVars[0].id == jaxpr.equations[0].outputs[0].id and _pmap_context() is None):
+        return _layer_backward(jaxpr, values, seeds[0])  # one layer: nothing to walk
     _lazy_scope.depth = getattr(_lazy_scope, "depth", 0) + 1
     try:
         return _do_backward(jaxpr, values, seeds)
     finally:
         _lazy_scope.depth -= 1
+
+
+def _layer_backward(jaxpr: Jaxpr, values: Dict[int, NDArray], seed: NDArray) -> List[NDArray]:
+    """do_backward of a Jaxpr that is one FFI_CALL and its output."""
+    eq = jaxpr.equations[0]
+    ids = [v.id for v in jaxpr.inVars]
+    g_ins = eq.metadata.vjp([values[v.id] for v in eq.inputs], values[eq.outputs[0].id], values.get(~eq.outputs[0].id),
+                            materialize(seed), [v.id in ids for v in eq.inputs])
+    grads: Dict[int, NDArray] = {}
+    for v, g in zip(eq.inputs, g_ins):
+        if g is not None:
+            _merge(grads, v.id, g)
+    return [materialize(grads[v.id]) if v.id in grads else zeros(v.shape, v.dtype, _device_of(values.get(v.id)))
+            for v in jaxpr.inVars]
 
 
 def _do_backward(jaxpr: Jaxpr, values: Dict[int, NDArray], seeds: List[NDArray]) -> List[NDArray]:
@@ -537,8 +559,7 @@ def _do_backward(jaxpr: Jaxpr, values: Dict[int, NDArray], seeds: List[NDArray])
     # consumer): inside a pmap there a CUDA event is recorded on the gradient,
     # so a collective over it (Lax.psumTree) can start while the rest of the
     # backward pass still runs.
-    from .pmap import PmapContext
-    overlap = PmapContext.current() is not None
+    overlap = _pmap_context() is not None
     in_ids = {v.id for v in jaxpr.inVars}
     last_use = {}
     for i, e in enumerate(jaxpr.equations):

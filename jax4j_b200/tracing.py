@@ -10,7 +10,7 @@ from __future__ import annotations
 import itertools
 import threading
 from dataclasses import dataclass, field
-from typing import Any, Dict, List, Optional
+from typing import Any, Dict, List, NamedTuple, Optional
 
 from .core import DType, NDArray, Primitive, Shape, UnsupportedOperationException
 
@@ -18,8 +18,7 @@ from .core import DType, NDArray, Primitive, Shape, UnsupportedOperationExceptio
 # ---------------------------------------------------------------------------
 # IR records (ir/Var.java, ir/Equation.java, ir/Jaxpr.java, ir/*Meta.java)
 # ---------------------------------------------------------------------------
-@dataclass(frozen=True)
-class Var:
+class Var(NamedTuple):
     id: int
     shape: Shape
     dtype: DType
