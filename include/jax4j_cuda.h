@@ -723,6 +723,13 @@ J4C_API int j4c_dense_finish(int dtype, void *z, int64_t M, int64_t N, const voi
 J4C_API size_t j4c_dense_grad_workspace(int dtype, int64_t M, int64_t N);
 J4C_API int j4c_dense_grad(int dtype, int64_t M, int64_t N, const void *dy, const void *u, int act, int from_output,
                            void *dz, void *dbias, uint32_t *lines, void *ws, size_t ws_bytes, j4c_stream stream);
+/* The whole gradient of a small FLOAT32 layer (see j4c_dot_act) in two
+ * launches: j4c_dense_grad, then dx = dz . w^T [M, K] and dw = x^T . dz [K, N]
+ * together.  dx or dw, and dbias, may be NULL: not wanted; dz is scratch [M, N]
+ * (NULL where act is J4C_ACT_NONE). */
+J4C_API int j4c_dense_backward(const float *x, const float *w, int64_t M, int64_t K, int64_t N, const float *dy,
+                               const float *u, int act, int from_output, float *dz, float *dx, float *dw, float *dbias,
+                               void *ws, size_t ws_bytes, j4c_stream stream);
 
 #ifdef __cplusplus
 }

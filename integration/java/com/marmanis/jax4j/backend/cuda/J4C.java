@@ -238,6 +238,10 @@ public final class J4C {
         JAVA_INT, JAVA_INT, JAVA_LONG, JAVA_LONG, ADDRESS, ADDRESS, JAVA_INT, JAVA_INT, ADDRESS, ADDRESS, ADDRESS,
         ADDRESS, JAVA_LONG, ADDRESS));
 
+    static final MethodHandle DENSE_BACKWARD = h("j4c_dense_backward", FunctionDescriptor.of(
+        JAVA_INT, ADDRESS, ADDRESS, JAVA_LONG, JAVA_LONG, JAVA_LONG, ADDRESS, ADDRESS, JAVA_INT, JAVA_INT, ADDRESS,
+        ADDRESS, ADDRESS, ADDRESS, ADDRESS, JAVA_LONG, ADDRESS));
+
     // ---- group norm with an activation (group_norm.cu) ----
     static final MethodHandle GROUP_NORM_WORKSPACE = h("j4c_group_norm_workspace", FunctionDescriptor.of(
         JAVA_LONG, JAVA_INT, JAVA_LONG, JAVA_LONG, JAVA_LONG, JAVA_LONG, JAVA_INT));

@@ -134,6 +134,7 @@ SIGNATURES = {
     "j4c_dense_finish": [I32, P, I64, I64, P, I32, P, P, P],
     "j4c_dense_grad_workspace": [I32, I64, I64],
     "j4c_dense_grad": [I32, I64, I64, P, P, I32, I32, P, P, P, P, C.c_size_t, P],
+    "j4c_dense_backward": [P, P, I64, I64, I64, P, P, I32, I32, P, P, P, P, P, C.c_size_t, P],
     "j4c_group_norm_workspace": [I32, I64, I64, I64, I64, I32],
     "j4c_group_norm": [I32, I64, I64, I64, I64, P, P, P, C.c_double, I32, P, P, P, P, C.c_size_t, P],
     "j4c_group_norm_grad": [I32, I64, I64, I64, I64, P, P, P, I32, P, P, P, P, P, P, P, C.c_size_t, P],

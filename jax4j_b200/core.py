@@ -816,7 +816,9 @@ def _make_splits(x: "ConcreteNDArray", kinds) -> None:
     ptrs = []
     for k in ("r", "c", "t"):
         ptrs += [out[k][0].data_ptr(), out[k][1].data_ptr()] if k in out else [None, None]
-    lines = _split_lines(x)
+    # row lines alone need no max pass of their own: the split takes each row's
+    # maximum on the way (j4c_split_f32_ex without lines)
+    lines = _split_lines(x) if x._lines is not None or kinds != ["r"] or cols > 8192 else None
     call("j4c_split_f32_ex", x._t.data_ptr(), rows, cols, *ptrs,
          lines.data_ptr() if lines is not None else None, x._stream())
     if x._split is None:

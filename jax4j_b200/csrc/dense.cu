@@ -4,6 +4,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "act.cuh"
 #include "common.cuh"
@@ -128,10 +129,13 @@ __global__ void __launch_bounds__(kRowsThreads) rows_kernel(const Product p) {
 
 // The general form, op(A) [M, K] . op(B) [K, N] with either operand stored
 // transposed: 64 x 64 tiles of 128 threads (8 x 4 results each), K in steps of
-// 16 through a ring of four buffers filled by asynchronous copies, three steps
+// 16 through a ring of three buffers filled by asynchronous copies, two steps
 // ahead: a CTA's share of K is a few steps, each bound by the copies' latency.
+// Also measured, and no faster at [256,784]x[784,512] (13.4 us) to 1024^3 (81
+// us): rings of four and six buffers, 8 x 8 results a thread, and two or four
+// shares of K within a CTA.
 constexpr int kTM = 64, kTN = 64, kTK = 16, kPitch = 68;  // a row of a buffer: padded, 16-byte multiples
-constexpr int kRing = 4;
+constexpr int kRing = 3, kTileThreads = 128;
 struct TileStep {
     float A[kTK][kPitch], B[kTK][kPitch];
 };
@@ -140,38 +144,46 @@ __device__ __forceinline__ void copy4_async(float *to, const float *from) {
                  : "memory");
 }
 template <bool TA, bool TB>
-__global__ void __launch_bounds__(128) tile_kernel(const Product p) {
-    __shared__ __align__(16) TileStep ring[kRing];
-    float(*const part)[kTN] = reinterpret_cast<float(*)[kTN]>(&ring[0]);  // once the ring has been read
-    static_assert(sizeof(ring) >= kTM * kTN * sizeof(float), "the tile's sums take the ring's place");
+__device__ __forceinline__ void tile_product(const Product &p, int64_t tile_m, int64_t tile_n, TileStep *ring) {
+    // the tile's sums take the ring's place once it has been read
+    float(*const part)[kTN] = reinterpret_cast<float(*)[kTN]>(ring);
+    static_assert(kRing * sizeof(TileStep) >= kTM * kTN * sizeof(float), "the tile's sums take the ring's place");
     const cg::cluster_group cluster = cg::this_cluster();
     const int ranks = cluster.num_blocks(), rank = cluster.block_rank();
     const int tid = threadIdx.x, tx = tid % 16, ty = tid / 16;
-    const int64_t n0 = (int64_t)(blockIdx.x / ranks) * kTN, m0 = (int64_t)blockIdx.y * kTM;
+    const int64_t n0 = tile_n * kTN, m0 = tile_m * kTM;
     const int64_t k0 = p.K * rank / ranks, k1 = p.K * (rank + 1) / ranks;
     const int steps = (int)((k1 - k0 + kTK - 1) / kTK);
     // This thread copies eight values of each operand a step: of one stored
-    // along K, one K of rows 8 apart; of one stored across, one row of Ks 2 apart.
+    // along K, one K of every eighth row; of one stored across, every second K
+    // of a row.  Bit i of the masks: its i-th row (or its row) is in the operand.
     const int am = TA ? tid % kTM : tid / kTK, ak = TA ? tid / kTM : tid % kTK;
     const int bn = TB ? tid / kTK : tid % kTN, bk = TB ? tid % kTK : tid / kTN;
     const float *a = p.A + (TA ? (k0 + ak) * p.M + m0 + am : (m0 + am) * p.K + k0 + ak);
     const float *b = p.B + (TB ? (n0 + bn) * p.K + k0 + bk : (k0 + bk) * p.N + n0 + bn);
-    const int64_t a_next = TA ? 2 * p.M : 8 * p.K, b_next = TB ? 8 * p.K : 2 * p.N;    // to the thread's next value
-    const int64_t a_step = TA ? kTK * p.M : kTK, b_step = TB ? kTK : kTK * p.N;        // to the next step
+    const int64_t a_next = TA ? 2 * p.M : 8 * p.K, b_next = TB ? 8 * p.K : 2 * p.N;  // to the thread's next value
+    const int64_t a_step = TA ? kTK * p.M : kTK, b_step = TB ? kTK : kTK * p.N;      // to the next step
+    uint32_t a_in = 0, b_in = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        a_in |= (m0 + am + (TA ? 0 : 8 * i) < p.M ? 1u : 0u) << i;
+        b_in |= (n0 + bn + (TB ? 8 * i : 0) < p.N ? 1u : 0u) << i;
+    }
     auto fetch = [&](int step) {
         if (step < steps) {
             TileStep &to = ring[step % kRing];
-            const int64_t kb = k0 + (int64_t)step * kTK;
+            const int left = (int)min((int64_t)kTK, k1 - k0 - (int64_t)step * kTK);  // Ks of this step
+            const float *pa = a, *pb = b;
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
+            for (int i = 0; i < 8; i++, pa += a_next) {
                 const int m = TA ? am : am + 8 * i, k = TA ? ak + 2 * i : ak;
-                if (m0 + m < p.M && kb + k < k1) copy4_async(&to.A[k][m], a + i * a_next);
+                if ((a_in >> i & 1u) && k < left) copy4_async(&to.A[k][m], pa);
                 else to.A[k][m] = 0.0f;
             }
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
+            for (int i = 0; i < 8; i++, pb += b_next) {
                 const int n = TB ? bn + 8 * i : bn, k = TB ? bk : bk + 2 * i;
-                if (n0 + n < p.N && kb + k < k1) copy4_async(&to.B[k][n], b + i * b_next);
+                if ((b_in >> i & 1u) && k < left) copy4_async(&to.B[k][n], pb);
                 else to.B[k][n] = 0.0f;
             }
             a += a_step, b += b_step;
@@ -207,8 +219,8 @@ __global__ void __launch_bounds__(128) tile_kernel(const Product p) {
     for (int i = 0; i < 8; i++)
         *reinterpret_cast<float4 *>(&part[ty * 8 + i][tx * 4]) = make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
     cluster.sync();
-    // rank r finishes rows r, r + ranks, ... of the tile
-    for (int e = tid; e < kTM / ranks * kTN; e += 128) {
+    // rank r finishes rows r, r + ranks, ... of the tile; shares in order
+    for (int e = tid; e < kTM / ranks * kTN; e += kTileThreads) {
         const int m = e / kTN * ranks + rank, n = e % kTN;
         if (m0 + m >= p.M || n0 + n >= p.N) continue;
         float v = 0.0f;
@@ -218,8 +230,35 @@ __global__ void __launch_bounds__(128) tile_kernel(const Product p) {
     cluster.sync();
 }
 
-template <typename Kernel>
-int launch_cluster(Kernel kernel, dim3 grid, int threads, size_t smem, int ranks, const Product &p, cudaStream_t s) {
+template <bool TA, bool TB>
+__global__ void __launch_bounds__(kTileThreads) tile_kernel(const Product p) {
+    __shared__ __align__(16) TileStep ring[kRing];
+    const int64_t tile = blockIdx.x / cg::this_cluster().num_blocks(), tiles_n = (p.N + kTN - 1) / kTN;
+    tile_product<TA, TB>(p, tile / tiles_n, tile % tiles_n, ring);
+}
+
+// Two products in one launch, x's gradient dz . w^T and w's x^T . dz: neither
+// fills the GPU, and together they cost one launch.
+struct TwoProducts {
+    Product dx, dw;
+    int64_t dx_tiles;
+};
+__global__ void __launch_bounds__(kTileThreads) two_products_kernel(const TwoProducts p) {
+    __shared__ __align__(16) TileStep ring[kRing];
+    const int64_t tile = blockIdx.x / cg::this_cluster().num_blocks();
+    if (tile < p.dx_tiles) {
+        const int64_t tiles_n = (p.dx.N + kTN - 1) / kTN;
+        tile_product<false, true>(p.dx, tile / tiles_n, tile % tiles_n, ring);
+    } else {
+        const int64_t tiles_n = (p.dw.N + kTN - 1) / kTN, t = tile - p.dx_tiles;
+        tile_product<true, false>(p.dw, t / tiles_n, t % tiles_n, ring);
+    }
+}
+
+template <typename Kernel, typename Arg>
+int launch_cluster(Kernel kernel, dim3 grid, int threads, size_t smem, int ranks, const Arg &p, cudaStream_t s) {
+    if (smem > 48 * 1024)
+        J4C_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid.x * ranks, grid.y);
     cfg.blockDim = dim3(threads);
@@ -247,8 +286,6 @@ template <int MT, int V>
 int launch_rows(const Product &p, cudaStream_t s) {
     constexpr size_t smem = std::max<size_t>(8 * MT * 32 * V, kRowsK * MT) * sizeof(float);
     const dim3 grid((unsigned)ceil_div(p.N, 32 * V), (unsigned)ceil_div(p.M, MT));
-    if (smem > 48 * 1024)
-        J4C_CUDA(cudaFuncSetAttribute(rows_kernel<MT, V>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     return launch_cluster(rows_kernel<MT, V>, grid, kRowsThreads, smem, ranks_for((int64_t)grid.x * grid.y, p.K, 64), p, s);
 }
 template <int V>
@@ -260,7 +297,10 @@ int launch_rows_m(const Product &p, cudaStream_t s) {
     return launch_rows<16, V>(p, s);
 }
 
-int small_product(const Product &p, int ta, int tb, cudaStream_t s) {
+int64_t tiles_of(const Product &p) { return ceil_div(p.M, kTM) * ceil_div(p.N, kTN); }
+
+// ranks: CTAs along K of the tile form (0: by the product's own size).
+int small_product(const Product &p, int ta, int tb, int ranks, cudaStream_t s) {
     if (p.M <= 16 && !ta && !tb) {
         // the widest loads that still give every SM a strip of columns
         auto fits = [&](int v) {
@@ -268,12 +308,13 @@ int small_product(const Product &p, int ta, int tb, cudaStream_t s) {
         };
         return fits(4) ? launch_rows_m<4>(p, s) : fits(2) ? launch_rows_m<2>(p, s) : launch_rows_m<1>(p, s);
     }
-    const dim3 grid((unsigned)ceil_div(p.N, kTN), (unsigned)ceil_div(p.M, kTM));
-    const int ranks = ranks_for((int64_t)grid.x * grid.y, p.K, 64);
-    if (ta) return tb ? launch_cluster(tile_kernel<true, true>, grid, 128, 0, ranks, p, s)
-                      : launch_cluster(tile_kernel<true, false>, grid, 128, 0, ranks, p, s);
-    return tb ? launch_cluster(tile_kernel<false, true>, grid, 128, 0, ranks, p, s)
-              : launch_cluster(tile_kernel<false, false>, grid, 128, 0, ranks, p, s);
+    const int64_t tiles = tiles_of(p);
+    if (!ranks) ranks = ranks_for(tiles, p.K, 64);
+    auto launch = [&](auto kernel) {
+        return launch_cluster(kernel, dim3((unsigned)tiles), kTileThreads, 0, ranks, p, s);
+    };
+    if (ta) return tb ? launch(tile_kernel<true, true>) : launch(tile_kernel<true, false>);
+    return tb ? launch(tile_kernel<false, true>) : launch(tile_kernel<false, false>);
 }
 
 // ---- the elementwise part alone (FLOAT64, whose product is the DMMA kernel's) ---------
@@ -335,7 +376,9 @@ struct alignas(sizeof(T) * V) Vec {
     T e[V];
 };
 
-template <typename T, int V>
+// CLUSTER: the groups of rows of a strip are one cluster, which adds its column
+// sums through distributed shared memory: a.sums is the bias's gradient itself.
+template <typename T, int V, bool CLUSTER>
 __global__ void __launch_bounds__(256) dense_grad_kernel(const GradArgs<T> a) {
     __shared__ T sums[8][256];
     __shared__ uint32_t tops[8][256];
@@ -411,15 +454,31 @@ __global__ void __launch_bounds__(256) dense_grad_kernel(const GradArgs<T> a) {
         uint32_t m = tops[0][c];
 #pragma unroll
         for (int w = 1; w < 8; w++) v += sums[w][c], m = max(m, tops[w][c]);
-        if (a.sums) a.sums[g * a.N + c0 + c] = v;
+        if (CLUSTER) sums[0][c] = v;
+        else if (a.sums) a.sums[g * a.N + c0 + c] = v;
         if (a.lines && m) atomicMax(a.lines + a.M + c0 + c, m);
+    }
+    if constexpr (CLUSTER) {
+        const cg::cluster_group cluster = cg::this_cluster();
+        cluster.sync();
+        // rank r takes columns r, r + ranks, ...
+        const int ranks = cluster.num_blocks();
+        for (int cc = cluster.block_rank() + threadIdx.x * ranks; cc < 256 && c0 + cc < a.N; cc += 256 * ranks) {
+            T v = T(0);
+            for (int r = 0; r < ranks; r++) v += *cluster.map_shared_rank(&sums[0][cc], r);
+            a.sums[c0 + cc] = v;
+        }
+        cluster.sync();
     }
     if (a.lines && __any_sync(0xffffffffu, bad) && lane == 0) atomicOr(a.lines + a.M + a.N, 1u);
 }
 
-// Groups of rows: four CTAs an SM, at least 32 rows each.
+// Groups of rows: four CTAs an SM, at least 32 rows each; where eight are
+// enough for that, or for 512 rows, they are a cluster and need no second launch.
 int64_t grad_groups(int64_t M, int64_t N) {
-    return std::max<int64_t>(1, std::min(ceil_div(M, 32), ceil_div((int64_t)sm_count() * 4, ceil_div(N, 256))));
+    const int64_t groups = std::max<int64_t>(
+        1, std::min(ceil_div(M, 32), ceil_div((int64_t)sm_count() * 4, ceil_div(N, 256))));
+    return M <= 512 ? std::min<int64_t>(groups, 8) : groups;
 }
 
 template <typename T>
@@ -427,19 +486,36 @@ int dense_grad(int64_t M, int64_t N, const T *dy, const T *u, int act, int from_
                void *ws, cudaStream_t s) {
     const int64_t groups = grad_groups(M, N);
     if (lines) J4C_CUDA(cudaMemsetAsync(lines, 0, (size_t)(M + N + 1) * sizeof(uint32_t), s));
-    T *sums = dbias ? (groups == 1 ? dbias : static_cast<T *>(ws)) : nullptr;
+    const bool cluster = dbias && groups > 1 && groups <= 8;
+    T *sums = !dbias ? nullptr : groups <= 8 ? dbias : static_cast<T *>(ws);
     const GradArgs<T> a{dy, act == J4C_ACT_NONE ? nullptr : u, dz, sums, lines, M, N, groups, act, from_output};
     constexpr int W = 16 / sizeof(T);
     auto fits = [&](int v) {
         auto ok = [&](const void *p) { return reinterpret_cast<uintptr_t>(p) % (v * sizeof(T)) == 0; };
         return N % v == 0 && ok(dy) && ok(u) && ok(dz);
     };
-    const dim3 grid((unsigned)ceil_div(N, 256), (unsigned)groups);
-    if (fits(W)) dense_grad_kernel<T, W><<<grid, 256, 0, s>>>(a);
-    else if (fits(2)) dense_grad_kernel<T, 2><<<grid, 256, 0, s>>>(a);
-    else dense_grad_kernel<T, 1><<<grid, 256, 0, s>>>(a);
-    J4C_LAUNCH_CHECK("dense_grad_kernel");
-    if (dbias && groups > 1) {
+    auto launch = [&](auto vec) {
+        constexpr int V = decltype(vec)::value;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)ceil_div(N, 256), (unsigned)groups);
+        cfg.blockDim = dim3(256);
+        cfg.stream = s;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = attr[0].val.clusterDim.z = 1;
+        attr[0].val.clusterDim.y = (unsigned)groups;
+        cfg.attrs = attr;
+        cfg.numAttrs = cluster ? 1 : 0;
+        J4C_CUDA(cluster ? cudaLaunchKernelEx(&cfg, dense_grad_kernel<T, V, true>, a)
+                         : cudaLaunchKernelEx(&cfg, dense_grad_kernel<T, V, false>, a));
+        count_launch();
+        return (int)J4C_OK;
+    };
+    if (int rc = fits(W)   ? launch(std::integral_constant<int, W>{})
+                 : fits(2) ? launch(std::integral_constant<int, 2>{})
+                           : launch(std::integral_constant<int, 1>{}))
+        return rc;
+    if (dbias && groups > 8) {
         sum_rows_kernel<T><<<(unsigned)ceil_div(N, 32), 1024, 0, s>>>(sums, groups, N, dbias, nullptr);
         J4C_LAUNCH_CHECK("sum_rows_kernel");
     }
@@ -451,6 +527,11 @@ int dense_grad(int64_t M, int64_t N, const T *dy, const T *u, int act, int from_
 
 using namespace j4c;
 
+// More tiles (eight CTAs each) than a grid takes.
+static bool too_many(int64_t M, int64_t N) {
+    return M >= (1ll << 40) || N >= (1ll << 33) || ceil_div(M, kTM) * ceil_div(N, 32) >= (1ll << 27);
+}
+
 extern "C" {
 
 int j4c_dot_act(const float *a, const float *b, int64_t M, int64_t K, int64_t N, int trans_a, int trans_b,
@@ -459,9 +540,9 @@ int j4c_dot_act(const float *a, const float *b, int64_t M, int64_t K, int64_t N,
     J4C_REQUIRE(act_known(act), "j4c_dot_act: unknown activation %d", act);
     if (M == 0 || N == 0) return J4C_OK;
     J4C_REQUIRE(y && (K == 0 || (a && b)), "j4c_dot_act: NULL pointer");
-    if (ceil_div(M, kTM) > 65535 || ceil_div(N, 32) * 8 >= (1ll << 31))
+    if (too_many(M, N))
         return set_error(J4C_E_UNSUPPORTED, "j4c_dot_act: %lld x %lld results are too many", (long long)M, (long long)N);
-    return small_product(Product{a, b, bias, residual, z, y, M, K, N, act}, trans_a, trans_b, as_stream(stream));
+    return small_product(Product{a, b, bias, residual, z, y, M, K, N, act}, trans_a, trans_b, 0, as_stream(stream));
 }
 
 int j4c_dot_split_act(const float *a_hi, const float *a_lo, const float *bt_hi, const float *bt_lo, int64_t M, int64_t K,
@@ -503,7 +584,7 @@ int j4c_dense_finish(int dtype, void *z, int64_t M, int64_t N, const void *bias,
 size_t j4c_dense_grad_workspace(int dtype, int64_t M, int64_t N) {
     if (M <= 0 || N <= 0) return 0;
     const int64_t groups = grad_groups(M, N);
-    return groups == 1 ? 0 : (size_t)(groups * N) * dtype_size(dtype);
+    return groups <= 8 ? 0 : (size_t)(groups * N) * dtype_size(dtype);
 }
 
 int j4c_dense_grad(int dtype, int64_t M, int64_t N, const void *dy, const void *u, int act, int from_output, void *dz,
@@ -530,6 +611,36 @@ int j4c_dense_grad(int dtype, int64_t M, int64_t N, const void *dy, const void *
         return dense_grad<T>(M, N, (const T *)dy, (const T *)u, act, from_output, (T *)dz, (T *)dbias, lines, ws, s);
     };
     return dtype == J4C_FLOAT64 ? run(0.0) : run(0.0f);
+}
+
+int j4c_dense_backward(const float *x, const float *w, int64_t M, int64_t K, int64_t N, const float *dy, const float *u,
+                       int act, int from_output, float *dz, float *dx, float *dw, float *dbias, void *ws, size_t ws_bytes,
+                       j4c_stream stream) {
+    J4C_REQUIRE(M >= 0 && K >= 0 && N >= 0, "j4c_dense_backward: negative dimension");
+    J4C_REQUIRE(dx || dw || K == 0 || (M == 0 && N == 0),
+                "j4c_dense_backward: neither product is wanted (j4c_dense_grad gives dbias alone)");
+    const float *d = dy;
+    if (dbias || act != J4C_ACT_NONE) {
+        if (int rc = j4c_dense_grad(J4C_FLOAT32, M, N, dy, u, act, from_output, dz, dbias, nullptr, ws, ws_bytes, stream))
+            return rc;
+        if (act != J4C_ACT_NONE) d = dz;
+    }
+    const bool dx_too = dx && M && K, dw_too = dw && K && N;
+    J4C_REQUIRE((!dx_too || N == 0 || (d && w)) && (!dw_too || M == 0 || (d && x)), "j4c_dense_backward: NULL pointer");
+    const Product px{d, w, nullptr, nullptr, nullptr, dx, M, N, K, J4C_ACT_NONE};
+    const Product pw{x, d, nullptr, nullptr, nullptr, dw, K, M, N, J4C_ACT_NONE};
+    if ((dx_too && too_many(M, K)) || (dw_too && too_many(K, N)))
+        return set_error(J4C_E_UNSUPPORTED, "j4c_dense_backward: %lld x %lld x %lld is too large", (long long)M,
+                         (long long)K, (long long)N);
+    cudaStream_t s = as_stream(stream);
+    // the same cut of K whether one product is wanted or both: the same bits
+    const int64_t tx = tiles_of(px), tw = tiles_of(pw);
+    const int ranks = ranks_for(tx + tw, std::max(M, N), 64);
+    if (dx_too && dw_too)
+        return launch_cluster(two_products_kernel, dim3((unsigned)(tx + tw)), kTileThreads, 0, ranks,
+                              TwoProducts{px, pw, tx}, s);
+    if (dx_too) return small_product(px, 0, 1, ranks, s);
+    return dw_too ? small_product(pw, 1, 0, ranks, s) : (int)J4C_OK;
 }
 
 }  // extern "C"

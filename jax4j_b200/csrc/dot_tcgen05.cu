@@ -820,6 +820,18 @@ gemm_3xtf32_kernel(const __grid_constant__ CUtensorMap tAh, const __grid_constan
             float *const Cb = C ? C + boff : nullptr;  // NULL: only the relu output is stored
             const float *const mask_b = ep.mask ? ep.mask + boff : nullptr;
             float *const act_b = ep.act ? ep.act + boff : nullptr;
+            if constexpr (ACT) {
+                // the residual's lines to L2 while the MMAs of the tile run
+                const int row = mt * Q::TM + (int)crank * BM + q * 32 + lane;
+                if (ep.residual && row < M) {
+#pragma unroll
+                    for (int g = 0; g < Q::COLS_PER_WARP / 32; g++) {
+                        const int col = nt * BN + cbase + g * 32;
+                        if (col < N)
+                            asm volatile("prefetch.global.L2 [%0];" ::"l"(ep.residual + (size_t)row * N + col));
+                    }
+                }
+            }
             float acc[Q::COLS_PER_WARP];
 #pragma unroll
             for (int j = 0; j < Q::COLS_PER_WARP; j++) acc[j] = 0.0f;
@@ -1509,6 +1521,76 @@ __global__ void __launch_bounds__(256) split16_kernel(const float *__restrict__ 
     flag_nonfinite(bad, hdr_r, hdr_c, nf);
 }
 
+// The row-line split alone, of an X whose maxima nobody has computed: WARPS
+// warps hold a row of up to 1024 WARPS columns in registers, so its maximum
+// and its split come from one read of X -- 8 B per element instead of the max
+// pass's 4 and the split's 8 ([8192, 4096]: 100 us for those two, see the
+// launch's figure).  The same bits as split16_kernel's.  hdr starts zeroed.
+constexpr int kSplitRowCols = 8 * 1024;
+template <int WARPS>
+__global__ void __launch_bounds__(256) split16_rows_kernel(const float *__restrict__ src, int64_t rows, int64_t cols,
+                                                           int64_t pitch, int vec, __half *__restrict__ hr,
+                                                           __half *__restrict__ lr, SplitHeader *hdr) {
+    constexpr int SETS = 8 / WARPS, THREADS = 32 * WARPS;
+    __shared__ uint32_t tops[2][8];  // two rows' take turns: one barrier a row
+    const int set = threadIdx.x / THREADS, t = threadIdx.x % THREADS;
+    uint32_t *lines = reinterpret_cast<uint32_t *>(hdr + 1);
+    if (blockIdx.x == 0 && threadIdx.x == 0) {  // not `nonfinite`, which any CTA may be setting
+        hdr->src = (unsigned long long)src;
+        hdr->layout = 0;
+        hdr->lines = (uint32_t)rows;
+        hdr->magic = kSplitMagic;
+    }
+    bool bad = false;
+    int turn = 0;
+    for (int64_t r = (int64_t)blockIdx.x * SETS + set; r < rows; r += (int64_t)gridDim.x * SETS, turn ^= 1) {
+        const float *p = src + r * cols;
+        float x[4][8];
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int64_t k = (int64_t)(t + i * THREADS) * 8;
+            if (vec && k + 8 <= cols) {
+                const float4 a = __ldg(reinterpret_cast<const float4 *>(p + k));
+                const float4 b = __ldg(reinterpret_cast<const float4 *>(p + k) + 1);
+                x[i][0] = a.x; x[i][1] = a.y; x[i][2] = a.z; x[i][3] = a.w;
+                x[i][4] = b.x; x[i][5] = b.y; x[i][6] = b.z; x[i][7] = b.w;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; j++) x[i][j] = k + j < cols ? __ldg(p + k + j) : 0.0f;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                x[i][j] = finite_or_zero(x[i][j], bad);
+                top = max(top, __float_as_uint(x[i][j]) & 0x7FFFFFFFu);
+            }
+        top = __reduce_max_sync(0xffffffffu, top);
+        if constexpr (WARPS > 1) {
+            if (threadIdx.x % 32 == 0) tops[turn][threadIdx.x / 32] = top;
+            asm volatile("bar.sync %0, %1;" ::"r"(1 + set), "n"(THREADS) : "memory");
+#pragma unroll
+            for (int w = 0; w < WARPS; w++) top = max(top, tops[turn][set * WARPS + w]);
+        }
+        if (t == 0) lines[r] = top;
+        const float sc = pow2f(split_exp(top));
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int64_t k = (int64_t)(t + i * THREADS) * 8;
+            if (k < pitch) {
+                uint32_t hw[4], lw[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) hw[j] = split2_f16(x[i][2 * j], x[i][2 * j + 1], sc, sc, lw[j]);
+                *reinterpret_cast<uint4 *>(hr + r * pitch + k) = make_uint4(hw[0], hw[1], hw[2], hw[3]);
+                *reinterpret_cast<uint4 *>(lr + r * pitch + k) = make_uint4(lw[0], lw[1], lw[2], lw[3]);
+            }
+        }
+    }
+    if (bad) atomicOr(&hdr->nonfinite, 1u);
+}
+
 // The fp16 split of X^T ([cols, pitch], pitch = rows rounded up to 8; its
 // rows are X's columns, scaled by cmax) and, with phi / plo set, the
 // row-scaled split of X in its stored layout ([rows, ppitch], ppitch = cols
@@ -1880,6 +1962,19 @@ int split_any(const float *src, int64_t rows, int64_t cols, float *hr, float *lr
                             : (hdr_t ? reinterpret_cast<uint32_t *>(hdr_t + 1) : nullptr);
     const uint32_t *rmax = nullptr, *cmax = nullptr, *nf = nullptr;
     uint32_t *copy_r = nullptr, *copy_c = nullptr;
+    if (f16 && hr && !hc && !ht && !lines_in && cols <= kSplitRowCols) {
+        J4C_CUDA(cudaMemsetAsync(hdr_r, 0, sizeof(SplitHeader), s));
+        const int64_t pitch = split_pitch(cols);
+        const int vec = (cols % 4 == 0) && aligned16(src);
+        const int warps = cols <= 1024 ? 1 : cols <= 4096 ? 4 : 8;
+        const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(rows, 8 / warps), (int64_t)sm_count() * 16);
+        auto *h = reinterpret_cast<__half *>(hr), *l = reinterpret_cast<__half *>(lr);
+        if (warps == 1) split16_rows_kernel<1><<<grid, 256, 0, s>>>(src, rows, cols, pitch, vec, h, l, hdr_r);
+        else if (warps == 4) split16_rows_kernel<4><<<grid, 256, 0, s>>>(src, rows, cols, pitch, vec, h, l, hdr_r);
+        else split16_rows_kernel<8><<<grid, 256, 0, s>>>(src, rows, cols, pitch, vec, h, l, hdr_r);
+        J4C_LAUNCH_CHECK("split16_rows_kernel");
+        return J4C_OK;
+    }
     if (lines_in) {
         // the maxima and the NaN/Inf flag came with the call: the kernels
         // copy them into the outputs and write whole headers, nothing to zero

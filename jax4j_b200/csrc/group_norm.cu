@@ -15,8 +15,8 @@
 // All of it is bound by HBM: x in, y out (8 B per FLOAT32 value) forward; x and
 // dy in, dx out backward (12 B).  Two forms:
 //  * Groups of at most 8192 values (rows of features are S = 1, G = 1: layer
-//    norm) are held in registers, eight values a thread, by 1 to 32 warps:
-//    every value is read once, and while a group is worked on the thread's
+//    norm) are held in registers by 1 to 32 warps, sixteen values a thread where
+//    they come four at a time, else eight: every value is read once, and while a group is worked on the thread's
 //    values of the next one are on their way to shared memory (cp.async).
 //    Backward a warp set keeps its group and walks over samples, so dgamma and
 //    dbeta gather in registers too.
@@ -36,8 +36,9 @@
 namespace j4c {
 namespace {
 
-constexpr int kHeld = 8;             // values a thread holds
-constexpr int64_t kMaxHeld = 32 * 32 * kHeld;
+template <typename T, int V>
+constexpr int kHeld = sizeof(T) * V == 16 && V == 4 ? 16 : 8;  // values a thread holds
+constexpr int64_t kMaxHeld = 8192;
 constexpr int kTileThreads = 512;    // at most: a tile's CTA has whole rows of columns
 constexpr int kTileChannels = 2048;  // channels of a tile at most
 constexpr int64_t kL2Part = 40ll << 20;
@@ -84,6 +85,11 @@ struct Held {
     static constexpr int THREADS = 32 * WARPS;  // of a set
 };
 
+// Threads an SM: 64 registers each, and 128 where two arrays and their sums of
+// sixteen values are held.
+template <typename T, int V, bool BACKWARD>
+constexpr int kResident = kHeld<T, V> == 16 && BACKWARD ? 512 : 1024;
+
 // The sum over a set.  Consecutive sums alternate between two buffers: a
 // barrier of the second is behind every read of the first.
 template <typename T, int WARPS>
@@ -93,18 +99,18 @@ __device__ __forceinline__ T set_sum(T v, T *buf, int set) {
         const int warp = (threadIdx.x / 32) % WARPS;
         if (threadIdx.x % 32 == 0) buf[set * WARPS + warp] = v;
         asm volatile("bar.sync %0, %1;" ::"r"(1 + set), "n"(32 * WARPS) : "memory");
-        v = T(0);
+        v = buf[set * WARPS + threadIdx.x % WARPS];
 #pragma unroll
-        for (int w = 0; w < WARPS; w++) v += buf[set * WARPS + w];
+        for (int o = WARPS / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     }
     return v;
 }
 
-// Where thread t of a set finds its values: value i * V + e of its kHeld is
+// Where thread t of a set finds its values: value i * V + e of those it holds is
 // channel col[i] + e of the group, off[i] + e elements behind the group's first.
 template <int V, int WARPS, int NV>
 struct Place {
-    int64_t off[NV];
+    uint32_t off[NV];
     int col[NV];
     __device__ __forceinline__ Place(int t, int64_t S, int64_t C, int64_t D) {
         const int per_row = (int)(D / V), all = (int)(S * per_row);
@@ -113,7 +119,7 @@ struct Place {
             const int v = t + i * Held<WARPS>::THREADS;
             const int s = v / per_row;
             col[i] = v < all ? (v - s * per_row) * V : -1;
-            off[i] = (int64_t)s * C + col[i];
+            off[i] = (uint32_t)((int64_t)s * C + col[i]);
         }
     }
 };
@@ -133,7 +139,7 @@ __device__ __forceinline__ void fetch(Vec<T, V> *slots, const T *from, const Pla
             copy_async(slots + i * blockDim.x + threadIdx.x, reinterpret_cast<const Vec<T, V> *>(from + at.off[i]));
 }
 template <typename T, int V, int WARPS, int NV>
-__device__ __forceinline__ void take(const Vec<T, V> *slots, T (&x)[kHeld], const Place<V, WARPS, NV> &at) {
+__device__ __forceinline__ void take(const Vec<T, V> *slots, T (&x)[kHeld<T, V>], const Place<V, WARPS, NV> &at) {
 #pragma unroll
     for (int i = 0; i < NV; i++)
         if (at.col[i] >= 0) {
@@ -146,7 +152,7 @@ __device__ __forceinline__ void take(const Vec<T, V> *slots, T (&x)[kHeld], cons
         }
 }
 template <typename T, int V, int WARPS, int NV>
-__device__ __forceinline__ void put(T *to, const T (&x)[kHeld], const Place<V, WARPS, NV> &at) {
+__device__ __forceinline__ void put(T *to, const T (&x)[kHeld<T, V>], const Place<V, WARPS, NV> &at) {
 #pragma unroll
     for (int i = 0; i < NV; i++)
         if (at.col[i] >= 0) {
@@ -158,7 +164,7 @@ __device__ __forceinline__ void put(T *to, const T (&x)[kHeld], const Place<V, W
 }
 // The group's parameters of the thread's values (from L1 after the first item).
 template <typename T, int V, int WARPS, int NV>
-__device__ __forceinline__ void params(const T *p, int64_t c0, T (&v)[kHeld], const Place<V, WARPS, NV> &at) {
+__device__ __forceinline__ void params(const T *p, int64_t c0, T (&v)[kHeld<T, V>], const Place<V, WARPS, NV> &at) {
 #pragma unroll
     for (int i = 0; i < NV; i++)
         if (at.col[i] >= 0) {
@@ -172,10 +178,10 @@ __device__ __forceinline__ void params(const T *p, int64_t c0, T (&v)[kHeld], co
 }
 
 template <typename T, int V, int WARPS>
-__global__ void __launch_bounds__(32 * Held<WARPS>::CTA, 1024 / (32 * Held<WARPS>::CTA))
+__global__ void __launch_bounds__(32 * Held<WARPS>::CTA, kResident<T, V, false> / (32 * Held<WARPS>::CTA))
 held_forward_kernel(const Args<T> a) {
     using H = Held<WARPS>;
-    constexpr int NV = kHeld / V;
+    constexpr int NV = kHeld<T, V> / V;
     __shared__ T sums[2][H::CTA];
     extern __shared__ __align__(16) unsigned char raw[];
     Vec<T, V> *slots = reinterpret_cast<Vec<T, V> *>(raw);
@@ -191,7 +197,7 @@ held_forward_kernel(const Args<T> a) {
     copies_commit();
     for (int now = 0; item < items; item += step, now ^= 1) {
         const int64_t base = b * sample + g * a.D, c0 = g * a.D;
-        T x[kHeld], p[kHeld];
+        T x[kHeld<T, V>], p[kHeld<T, V>];
         b += b_step, g += g_step;  // the next item's, without a division
         if (g >= a.G) b++, g -= a.G;
         if (item + step < items) fetch(slots + (now ^ 1) * turn, a.x + b * sample + g * a.D, at);
@@ -200,11 +206,11 @@ held_forward_kernel(const Args<T> a) {
         take(slots + now * turn, x, at);
         T sum = T(0);
 #pragma unroll
-        for (int i = 0; i < kHeld; i++) sum += x[i];
+        for (int i = 0; i < kHeld<T, V>; i++) sum += x[i];
         const T mean = set_sum<T, WARPS>(sum, sums[0], set) / n;
         T sq = T(0);
 #pragma unroll
-        for (int i = 0; i < kHeld; i++)
+        for (int i = 0; i < kHeld<T, V>; i++)
             if (at.col[i / V] >= 0) {
                 x[i] -= mean;
                 sq += x[i] * x[i];
@@ -215,16 +221,16 @@ held_forward_kernel(const Args<T> a) {
             a.rstd[item] = rstd;
         }
 #pragma unroll
-        for (int i = 0; i < kHeld; i++) x[i] *= rstd;
+        for (int i = 0; i < kHeld<T, V>; i++) x[i] *= rstd;
         if (a.gamma) {
             params(a.gamma, c0, p, at);
 #pragma unroll
-            for (int i = 0; i < kHeld; i++) x[i] *= p[i];
+            for (int i = 0; i < kHeld<T, V>; i++) x[i] *= p[i];
         }
         if (a.beta) {
             params(a.beta, c0, p, at);
 #pragma unroll
-            for (int i = 0; i < kHeld; i++) x[i] += p[i];
+            for (int i = 0; i < kHeld<T, V>; i++) x[i] += p[i];
         }
         act_values(a.act, x);
         put(a.y + base, x, at);
@@ -235,10 +241,10 @@ held_forward_kernel(const Args<T> a) {
 // (nb sets for every group).  a.dpart, unless NULL, gets its sums over samples
 // and positions: [nb, C] of du, then [nb, C] of du xhat.
 template <typename T, int V, int WARPS>
-__global__ void __launch_bounds__(32 * Held<WARPS>::CTA, 1024 / (32 * Held<WARPS>::CTA))
+__global__ void __launch_bounds__(32 * Held<WARPS>::CTA, kResident<T, V, true> / (32 * Held<WARPS>::CTA))
 held_backward_kernel(const Args<T> a, int64_t nb) {
     using H = Held<WARPS>;
-    constexpr int NV = kHeld / V;
+    constexpr int NV = kHeld<T, V> / V;
     __shared__ T sums[2][H::CTA];
     extern __shared__ __align__(16) unsigned char raw[];
     constexpr int AHEAD = kAhead<T, true>;
@@ -250,9 +256,9 @@ held_backward_kernel(const Args<T> a, int64_t nb) {
     const bool on = k < nb * a.G;  // a whole set: the barriers in the loop are the set's own
     const int64_t g = k % a.G, sample = a.S * a.C;
     const T n = (T)(a.S * a.D);
-    T du_sum[kHeld], dux_sum[kHeld];
+    T du_sum[kHeld<T, V>], dux_sum[kHeld<T, V>];
 #pragma unroll
-    for (int i = 0; i < kHeld; i++) du_sum[i] = dux_sum[i] = T(0);
+    for (int i = 0; i < kHeld<T, V>; i++) du_sum[i] = dux_sum[i] = T(0);
     auto fetch_both = [&](int64_t sb, int to) {
         if (sb < a.B) {
             fetch(xs + to * turn, a.x + sb * sample + g * a.D, at);
@@ -265,47 +271,47 @@ held_backward_kernel(const Args<T> a, int64_t nb) {
     for (int now = 0; b < a.B; b += nb, now ^= AHEAD) {
         fetch_both(b + AHEAD * nb, now ^ AHEAD);
         const T mean = a.mean[b * a.G + g], rstd = a.rstd[b * a.G + g];
-        T x[kHeld], h[kHeld], u[kHeld], p[kHeld];
+        T x[kHeld<T, V>], h[kHeld<T, V>], u[kHeld<T, V>], p[kHeld<T, V>];
         copies_done<AHEAD>();
         take(xs + now * turn, x, at);
         take(ds + now * turn, h, at);
 #pragma unroll
-        for (int i = 0; i < kHeld; i++) x[i] = at.col[i / V] >= 0 ? (x[i] - mean) * rstd : T(0);
+        for (int i = 0; i < kHeld<T, V>; i++) x[i] = at.col[i / V] >= 0 ? (x[i] - mean) * rstd : T(0);
         if (a.act != J4C_ACT_NONE) {
 #pragma unroll
-            for (int i = 0; i < kHeld; i++) u[i] = x[i];
+            for (int i = 0; i < kHeld<T, V>; i++) u[i] = x[i];
             if (a.gamma) {
                 params(a.gamma, g * a.D, p, at);
 #pragma unroll
-                for (int i = 0; i < kHeld; i++) u[i] *= p[i];
+                for (int i = 0; i < kHeld<T, V>; i++) u[i] *= p[i];
             }
             if (a.beta) {
                 params(a.beta, g * a.D, p, at);
 #pragma unroll
-                for (int i = 0; i < kHeld; i++) u[i] += p[i];
+                for (int i = 0; i < kHeld<T, V>; i++) u[i] += p[i];
             }
             act_slopes(a.act, u, h);
         }
 #pragma unroll
-        for (int i = 0; i < kHeld; i++) {
+        for (int i = 0; i < kHeld<T, V>; i++) {
             du_sum[i] += h[i];
             dux_sum[i] += h[i] * x[i];
         }
         if (a.gamma) {
             params(a.gamma, g * a.D, p, at);
 #pragma unroll
-            for (int i = 0; i < kHeld; i++) h[i] *= p[i];
+            for (int i = 0; i < kHeld<T, V>; i++) h[i] *= p[i];
         }
         T s1 = T(0), s2 = T(0);
 #pragma unroll
-        for (int i = 0; i < kHeld; i++) {
+        for (int i = 0; i < kHeld<T, V>; i++) {
             s1 += h[i];
             s2 += h[i] * x[i];
         }
         s1 = set_sum<T, WARPS>(s1, sums[0], set) / n;
         s2 = set_sum<T, WARPS>(s2, sums[1], set) / n;
 #pragma unroll
-        for (int i = 0; i < kHeld; i++) x[i] = rstd * (h[i] - s1 - x[i] * s2);
+        for (int i = 0; i < kHeld<T, V>; i++) x[i] = rstd * (h[i] - s1 - x[i] * s2);
         put(a.y + b * sample + g * a.D, x, at);
     }
     if (!a.dpart) return;
@@ -313,12 +319,12 @@ held_backward_kernel(const Args<T> a, int64_t nb) {
     // memory (the slots' space: every set's copies have been read)
     copies_done<0>();
     __syncthreads();
-    T *buf = reinterpret_cast<T *>(raw) + (size_t)set * H::THREADS * kHeld;
+    T *buf = reinterpret_cast<T *>(raw) + (size_t)set * H::THREADS * kHeld<T, V>;
     for (int which = 0; which < 2; which++) {
 #pragma unroll
-        for (int i = 0; i < kHeld; i++)
+        for (int i = 0; i < kHeld<T, V>; i++)
             if (at.col[i / V] >= 0) {
-                const int64_t s = (at.off[i / V] - at.col[i / V]) / a.C;
+                const int64_t s = (at.off[i / V] - (uint32_t)at.col[i / V]) / (uint32_t)a.C;
                 buf[s * a.D + at.col[i / V] + i % V] = which ? dux_sum[i] : du_sum[i];
             }
         __syncthreads();
@@ -721,7 +727,10 @@ __global__ void __launch_bounds__(kTileThreads, 2) tile_grad_kernel(const Args<T
 }
 
 // ---- host ----------------------------------------------------------------------------
-inline bool held(int64_t S, int64_t D) { return D <= kMaxHeld && S <= kMaxHeld && S * D <= kMaxHeld; }
+inline bool held(int64_t S, int64_t C, int64_t G) {
+    const int64_t D = C / G;
+    return D <= kMaxHeld && S <= kMaxHeld && S * D <= kMaxHeld && S * C < (1ll << 32);
+}
 
 template <typename T>
 Geo make_geo(int64_t B, int64_t S, int64_t C, int64_t G) {
@@ -754,24 +763,31 @@ int64_t samples_of_part(int64_t B, int64_t bytes_per_sample) {
     return std::max<int64_t>(1, std::min(B, kL2Part / std::max<int64_t>(1, bytes_per_sample)));
 }
 
-// Warps that hold a group of n values, eight values a thread.
-inline int held_warps(int64_t n) {
+// Warps that hold a group of n values.
+template <typename T, int V>
+int held_warps(int64_t n) {
     int warps = 1;
-    while (warps * 32 * kHeld < n) warps *= 2;
+    while (warps * 32 * kHeld<T, V> < n) warps *= 2;
     return warps;
 }
 
-// Backward, the sets that share a group's samples: two CTAs of 512 threads an
-// SM (64 registers each) or as many threads in smaller ones, no more than samples.
-inline int64_t held_sets(int64_t B, int64_t G, int warps) {
+// Backward, the sets that share a group's samples: as many as are resident, no
+// more than samples.
+template <typename T, int V>
+int64_t held_sets(int64_t B, int64_t G, int warps) {
     const int cta = std::max(8, warps);
-    return std::min(B, std::max<int64_t>(1, ceil_div((int64_t)sm_count() * (32 / cta) * (cta / warps), G)));
+    return std::min(B, std::max<int64_t>(1, ceil_div((int64_t)sm_count() * (kResident<T, V, true> / 32 / cta) * (cta / warps), G)));
 }
 
 template <typename T>
 size_t workspace(int64_t B, int64_t S, int64_t C, int64_t G, bool backward) {
     const int64_t es = sizeof(T);
-    if (held(S, C / G)) return backward ? (size_t)(2 * es * C * held_sets(B, G, held_warps(S * (C / G)))) : 0;
+    if (held(S, C, G)) {
+        // with either width of vector
+        const int64_t n = S * (C / G);
+        const int64_t sets = std::max(held_sets<T, 1>(B, G, held_warps<T, 1>(n)), held_sets<T, 4>(B, G, held_warps<T, 4>(n)));
+        return backward ? (size_t)(2 * es * C * sets) : 0;
+    }
     const int64_t part = samples_of_part(B, (backward ? 2 : 1) * S * C * es);
     const Geo q = make_geo<T>(part, S, C, G);
     // the parts' statistics, and backward the tiles' sums of every channel
@@ -782,7 +798,7 @@ template <typename T, int V, int WARPS>
 int launch_held(const Args<T> &a, bool backward, T *dgamma, T *dbeta, cudaStream_t s) {
     using H = Held<WARPS>;
     const int threads = 32 * H::CTA;
-    const size_t smem = (size_t)threads * kHeld * sizeof(T) *
+    const size_t smem = (size_t)threads * kHeld<T, V> * sizeof(T) *
                         (backward ? 2 * (1 + kAhead<T, true>) : 1 + kAhead<T, false>);
     auto allow = [&](auto kernel) {
         return smem > 48 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)
@@ -790,13 +806,13 @@ int launch_held(const Args<T> &a, bool backward, T *dgamma, T *dbeta, cudaStream
     };
     if (!backward) {
         const int64_t ctas = ceil_div(a.B * a.G, H::SETS);
-        const unsigned grid = (unsigned)std::min<int64_t>(ctas, (int64_t)sm_count() * (1024 / threads));
+        const unsigned grid = (unsigned)std::min<int64_t>(ctas, (int64_t)sm_count() * (kResident<T, V, false> / threads));
         J4C_CUDA(allow(held_forward_kernel<T, V, WARPS>));
         held_forward_kernel<T, V, WARPS><<<grid, threads, smem, s>>>(a);
         J4C_LAUNCH_CHECK("held_forward_kernel");
         return J4C_OK;
     }
-    const int64_t nb = held_sets(a.B, a.G, WARPS);
+    const int64_t nb = held_sets<T, V>(a.B, a.G, WARPS);
     if (ceil_div(nb * a.G, H::SETS) >= (1ll << 31)) return set_error(J4C_E_UNSUPPORTED, "j4c_group_norm: too many groups");
     J4C_CUDA(allow(held_backward_kernel<T, V, WARPS>));
     held_backward_kernel<T, V, WARPS><<<(unsigned)ceil_div(nb * a.G, H::SETS), threads, smem, s>>>(a, nb);
@@ -810,13 +826,15 @@ int launch_held(const Args<T> &a, bool backward, T *dgamma, T *dbeta, cudaStream
 
 template <typename T, int V>
 int run_held(const Args<T> &a, bool backward, T *dgamma, T *dbeta, cudaStream_t s) {
-    switch (held_warps(a.S * a.D)) {
+    switch (held_warps<T, V>(a.S * a.D)) {
     case 1: return launch_held<T, V, 1>(a, backward, dgamma, dbeta, s);
     case 2: return launch_held<T, V, 2>(a, backward, dgamma, dbeta, s);
     case 4: return launch_held<T, V, 4>(a, backward, dgamma, dbeta, s);
     case 8: return launch_held<T, V, 8>(a, backward, dgamma, dbeta, s);
     case 16: return launch_held<T, V, 16>(a, backward, dgamma, dbeta, s);
-    default: return launch_held<T, V, 32>(a, backward, dgamma, dbeta, s);
+    default:
+        if constexpr (kHeld<T, V> == 8) return launch_held<T, V, 32>(a, backward, dgamma, dbeta, s);
+        return set_error(J4C_E_UNSUPPORTED, "j4c_group_norm: a group of %lld values", (long long)(a.S * a.D));  // > kMaxHeld
     }
 }
 
@@ -871,7 +889,7 @@ int group_norm(const Args<T> &a, bool backward, T *dgamma, T *dbeta, void *ws, c
         return a.D % v == 0 && ok(a.x) && ok(a.y) && ok(a.dy) && ok(a.gamma) && ok(a.beta);
     };
     const int v = fits(W) ? W : W > 2 && fits(2) ? 2 : 1;
-    const bool small = held(a.S, a.D);
+    const bool small = held(a.S, a.C, a.G);
     auto run = [&](auto vec) {
         constexpr int V = decltype(vec)::value;
         return small ? run_held<T, V>(a, backward, dgamma, dbeta, s) : run_tiles<T, V>(a, backward, dgamma, dbeta, ws, s);

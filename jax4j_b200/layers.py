@@ -163,9 +163,10 @@ class _GroupNorm(FfiMeta):
 # ---------------------------------------------------------------------------
 # FLOAT32 products of at most this many multiply-adds run on the CUDA cores
 # straight from their arrays (j4c_dot_act); the tensor-core product first
-# splits both operands (eight launches with the line maxima), which larger ones
-# win back.
-SMALL_PRODUCT = 1 << 28
+# splits both operands (five launches more), which larger ones win back: forward
+# and gradients of [1024,1024]x[1024,512] 161 against 188 us, of [1024,1024]x
+# [1024,1024] 260 against 204.
+SMALL_PRODUCT = 1 << 29
 
 
 def _small(M: int, K: int, N: int) -> bool:
@@ -268,33 +269,34 @@ class _Dense(FfiMeta):
         f32 = dt == DType.FLOAT32
         small = f32 and (_small(M, K, N) or not (M and N and K))
         dz, dbias, lines = t, None, None
-        if want_bias or (products and (self.act or (f32 and not small))):
-            L = _lib.lib()
-            if self.act:
-                dz = torch.empty(M * N, dtype=t.dtype, device=t.device)
-            if want_bias:
-                dbias = torch.empty(N, dtype=t.dtype, device=t.device)
-            if f32 and not small and products:
-                lines = torch.empty(M + N + 1, dtype=torch.int32, device=t.device)
-            need = L.j4c_dense_grad_workspace(dt.ordinal, M, N) if want_bias else 0
-            ws = torch.empty(need, dtype=torch.uint8, device=t.device) if need else None
-            u = z if z is not None else out._t
-            call("j4c_dense_grad", dt.ordinal, M, N, t.data_ptr(), u.data_ptr() if self.act else None, self.act,
-                 int(z is None), dz.data_ptr() if self.act else None, dbias.data_ptr() if want_bias else None,
-                 lines.data_ptr() if lines is not None else None, ws.data_ptr() if need else None, need, stream)
         grads: List[Optional[ConcreteNDArray]] = [None, None]
-        if small:
-            if wanted[0]:
-                dx = torch.empty(M * K, dtype=t.dtype, device=t.device)
-                call("j4c_dot_act", dz.data_ptr(), w._t.data_ptr(), M, N, K, 0, 1, None, 0, None, None, dx.data_ptr(),
-                     stream)
-                grads[0] = ConcreteNDArray._wrap(dx, x._shape, dt, dev)
-            if wanted[1]:
-                dw = torch.empty(K * N, dtype=t.dtype, device=t.device)
-                call("j4c_dot_act", x2._t.data_ptr(), dz.data_ptr(), K, M, N, 1, 0, None, 0, None, None, dw.data_ptr(),
-                     stream)
-                grads[1] = ConcreteNDArray._wrap(dw, w._shape, dt, dev)
-        elif products:
+        if want_bias or products:
+            # the pass over g, and for small products all of the gradient
+            dev_t = t.device
+            pass_over = want_bias or self.act or (f32 and not small)
+            need = _lib.lib().j4c_dense_grad_workspace(dt.ordinal, M, N) if want_bias else 0
+            ws = torch.empty(need, dtype=torch.uint8, device=dev_t) if need else None
+            wp = ws.data_ptr() if need else None
+            if self.act:
+                dz = torch.empty(M * N, dtype=t.dtype, device=dev_t)
+            if want_bias:
+                dbias = torch.empty(N, dtype=t.dtype, device=dev_t)
+            up = (z if z is not None else out._t).data_ptr() if self.act else None
+            zp, bp = dz.data_ptr() if self.act else None, dbias.data_ptr() if want_bias else None
+            if small and products:
+                dx = torch.empty(M * K, dtype=t.dtype, device=dev_t) if wanted[0] else None
+                dw = torch.empty(K * N, dtype=t.dtype, device=dev_t) if wanted[1] else None
+                call("j4c_dense_backward", x2._t.data_ptr(), w._t.data_ptr(), M, K, N, t.data_ptr(), up, self.act,
+                     int(z is None), zp, dx.data_ptr() if wanted[0] else None, dw.data_ptr() if wanted[1] else None, bp,
+                     wp, need, stream)
+                grads = [ConcreteNDArray._wrap(dx, x._shape, dt, dev) if wanted[0] else None,
+                         ConcreteNDArray._wrap(dw, w._shape, dt, dev) if wanted[1] else None]
+            elif pass_over:
+                if f32 and products:
+                    lines = torch.empty(M + N + 1, dtype=torch.int32, device=dev_t)
+                call("j4c_dense_grad", dt.ordinal, M, N, t.data_ptr(), up, self.act, int(z is None), zp, bp,
+                     lines.data_ptr() if lines is not None else None, wp, need, stream)
+        if products and not small:
             d = ConcreteNDArray._wrap(dz, Shape(M, N), dt, dev)
             if f32:
                 d._lines = lines

@@ -75,7 +75,7 @@ class AdamWState:
         for i, a in enumerate(arrays):
             l = leaves[i // per]
             dt, n = (DType.INT32, _q8_words(l.size)) if stateBits == 8 else (l.dtype, l.size)
-            if a.dtype() != dt or a.shape().size() != n:
+            if a.dtype() is not dt or a.shape().size() != n:
                 raise IllegalArgumentException(f"AdamW: array {i} of the state is {a.shape()} {a.dtype()}, "
                                                f"parameter {i // per} {l.shape} takes {n} x {dt}")
         self._set(PyTrees.unflatten(params, leaves), leaves, stateBits, step, arrays)
@@ -131,18 +131,19 @@ def _pointers(arrays) -> C.Array:
 def _carve(sizes: List[int], dtype: torch.dtype, device) -> List[torch.Tensor]:
     """Uninitialised flat tensors of these sizes from one allocation, each on
     a 256-byte boundary (one allocator call and one view call for a tree)."""
-    unit = 256 // torch.empty(0, dtype=dtype).element_size()
+    unit = 256 // dtype.itemsize
     cuts = []
     for n in sizes:
-        cuts += [n, -n % unit]
-    return list(torch.empty(sum(cuts), dtype=dtype, device=device).split(cuts)[0::2])
+        cuts += (n, -n % unit)
+    return torch.split_with_sizes(torch.empty(sum(cuts), dtype=dtype, device=device), cuts)[0::2]
 
 
 def _one_gpu(arrays) -> None:
-    first = arrays[0]._t.device
+    first = arrays[0]._t.get_device()
     for a in arrays:
-        if a._t.device != first:
-            raise IllegalStateException(f"AdamW: the tree's arrays lie on different GPUs ({first} and {a._t.device})")
+        if a._t.get_device() != first:
+            raise IllegalStateException(f"AdamW: the tree's arrays lie on different GPUs ({arrays[0]._t.device} and "
+                                        f"{a._t.device})")
 
 
 class Optim:
@@ -189,7 +190,8 @@ class Optim:
         for w, g, l in zip(pl, gl, ls):
             if not (isinstance(w, ConcreteNDArray) and isinstance(g, ConcreteNDArray)):
                 raise UnsupportedOperationException("AdamW takes concrete arrays, not traced ones")
-            if w._shape != g._shape or w._dtype != g._dtype or w._shape != l.shape or w._dtype != l.dtype:
+            d, dt = w._shape._d, w._dtype
+            if g._shape._d != d or l.shape._d != d or g._dtype is not dt or l.dtype is not dt:
                 raise IllegalArgumentException(f"adamW: parameter {w._shape} {w._dtype}, gradient {g._shape} {g._dtype} "
                                                f"and state {l.shape} {l.dtype} do not match")
         if not (0.0 <= beta1 < 1.0 and 0.0 <= beta2 < 1.0):
@@ -204,7 +206,7 @@ class Optim:
             if not isinstance(lr, ConcreteNDArray) or lr.dtype() != DType.FLOAT32 or lr.shape().size() != 1:
                 raise IllegalArgumentException("adamW: lr is a number or one FLOAT32 value")
             lr_dev, lr = lr, 0.0
-        _one_gpu(pl + gl + state.arrays() + ([lr_dev] if lr_dev is not None else []))
+        _one_gpu([state._step, *pl, *gl, *state._arrays] + ([lr_dev] if lr_dev is not None else []))
         dev = state._step._t.device
         stream = stream_of(dev.index)
         step = torch.empty(3, dtype=torch.float64, device=dev)
@@ -215,28 +217,25 @@ class Optim:
         kinds = [(dt, [i for i in range(n) if pl[i]._dtype is dt]) for dt in (DType.FLOAT32, DType.FLOAT64)]
         kinds = [k for k in kinds if k[1]] or [(DType.FLOAT32, [])]
         steps_out = step.data_ptr()
+        wrap = ConcreteNDArray._wrap
         for dt, idx in kinds:
+            k, all_of = len(idx), len(idx) == n
             sizes = [ls[i].size for i in idx]
             ws = _carve(sizes, dt.torch, dev)
-            if per == 1:
-                ss = _carve([_q8_words(s) for s in sizes], torch.int32, dev)
-            else:
-                ss = _carve([s for s in sizes for _ in range(2)], dt.torch, dev)
-            k = len(idx)
-            old = [state._arrays[per * i + j] for i in idx for j in range(per)]
-            call("j4c_adamw_step", dt.ordinal, state._bits, k, (C.c_int64 * k)(*sizes),
-                 _pointers([pl[i] for i in idx]), _pointers([gl[i] for i in idx]), _pointers(old),
-                 (C.c_void_p * k)(*[t.data_ptr() for t in ws]), (C.c_void_p * (per * k))(*[t.data_ptr() for t in ss]),
-                 (C.c_double * k)(*[wd[i] for i in idx]), state._step._t.data_ptr(), steps_out,
-                 lr_dev._t.data_ptr() if lr_dev is not None else None, float(lr), float(scale), float(beta1),
-                 float(beta2), float(eps), stream)
+            ss = (_carve([_q8_words(s) for s in sizes], torch.int32, dev) if per == 1 else
+                  _carve([s for s in sizes for _ in range(2)], dt.torch, dev))
+            pk, gk = (pl, gl) if all_of else ([pl[i] for i in idx], [gl[i] for i in idx])
+            old = state._arrays if all_of else [state._arrays[per * i + j] for i in idx for j in range(per)]
+            call("j4c_adamw_step", dt.ordinal, state._bits, k, (C.c_int64 * k)(*sizes), _pointers(pk), _pointers(gk),
+                 _pointers(old), (C.c_void_p * k)(*[t.data_ptr() for t in ws]),
+                 (C.c_void_p * (per * k))(*[t.data_ptr() for t in ss]), (C.c_double * k)(*[wd[i] for i in idx]),
+                 state._step._t.data_ptr(), steps_out, lr_dev._t.data_ptr() if lr_dev is not None else None, float(lr),
+                 float(scale), float(beta1), float(beta2), float(eps), stream)
             steps_out = None
-            for j, i in enumerate(idx):
-                w = pl[i]
-                new_w[i] = ConcreteNDArray._wrap(ws[j], w._shape, dt, w._device)
-                for p in range(per):
-                    a = old[per * j + p]
-                    new_s[per * i + p] = ConcreteNDArray._wrap(ss[per * j + p], a._shape, a._dtype, a._device)
+            for i, w, t in zip(idx, pk, ws):
+                new_w[i] = wrap(t, w._shape, dt, w._device)
+            for j, (a, t) in enumerate(zip(old, ss)):
+                new_s[per * idx[j // per] + j % per] = wrap(t, a._shape, a._dtype, a._device)
         new_step = ConcreteNDArray._wrap(step, state._step._shape, DType.FLOAT64, state._step._device)
         return (PyTrees.unflatten(params, new_w),
                 AdamWState.__new__(AdamWState)._set(state._tree, ls, state._bits, new_step, new_s))

@@ -150,12 +150,38 @@ def test_unaligned_arrays(J, monkeypatch, small, offset):
 
 
 def test_at_the_border_between_the_products(J):
-    """K = 1024: 512 x 512 outputs are the last on the CUDA cores, 513 the first beyond."""
+    """K = 1024: 1024 x 512 outputs are the last on the CUDA cores, 1025 x 512 the first beyond."""
     from jax4j_b200 import layers
-    assert layers.SMALL_PRODUCT == 512 * 1024 * 512
-    for M in (512, 513):
+    assert layers.SMALL_PRODUCT == 1024 * 1024 * 512
+    for M in (1024, 1025):
         x, w, b, res, dy = make(M, (M, 1024), 512)
-        check(run(J, x, w, b, "gelu", res, dy), reference(x, w, b, "gelu", res, dy, U, M == 513))
+        check(run(J, x, w, b, "gelu", res, dy), reference(x, w, b, "gelu", res, dy, U, M == 1025))
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 1), (7, 100), (33, 1024), (40, 1028), (5, 4097), (9, 8192), (300, 512), (3, 8195)])
+def test_row_splits_without_a_max_pass(J, rows, cols):
+    """The split that takes its maxima on the way is, bit for bit, the one that is given them."""
+    import torch
+    from jax4j_b200 import _lib
+    r = np.random.default_rng(rows + cols)
+    x = (r.standard_normal((rows, cols)) * 10.0 ** r.integers(-30, 30, (rows, 1))).astype(np.float32)
+    for special in (False, True):
+        if special:
+            x[rows // 2, cols // 2] = np.nan
+            x[0, 0] = -np.inf
+        for offset in (0, 1):
+            X = arr(J, x, offset)
+            n = _lib.lib().j4c_split_floats(rows, cols)
+            out = [torch.zeros(n, dtype=torch.int32, device="cuda") for _ in range(4)]
+            lines = torch.empty(rows + cols + 1, dtype=torch.int32, device="cuda")
+            s = X._stream()
+            _lib.call("j4c_split_lines", X.data_ptr(), rows, cols, lines.data_ptr(), s)
+            _lib.call("j4c_split_f32_ex", X.data_ptr(), rows, cols, out[0].data_ptr(), out[1].data_ptr(), None, None, None,
+                      None, lines.data_ptr(), s)
+            _lib.call("j4c_split_f32_ex", X.data_ptr(), rows, cols, out[2].data_ptr(), out[3].data_ptr(), None, None, None,
+                      None, None, s)
+            for a, b in ((out[0], out[2]), (out[1], out[3])):
+                np.testing.assert_array_equal(a.cpu().numpy(), b.cpu().numpy())
 
 
 @pytest.mark.parametrize("small", [True, False])
@@ -174,10 +200,11 @@ def test_non_finite_values(J, monkeypatch, small):
     np.testing.assert_allclose(y[~bad], (1 / (1 + np.exp(-z)) + res)[~bad], rtol=1e-5, atol=1e-5)
 
 
-def test_line_words_of_the_output(J):
+def test_line_words_of_the_output(J, monkeypatch):
     """What a later product's split takes instead of a max pass, NaN/Inf flag included."""
     import torch
-    from jax4j_b200 import _lib
+    from jax4j_b200 import _lib, layers
+    monkeypatch.setattr(layers, "SMALL_PRODUCT", 0)
     for special in (False, True):
         x, w, b, res, _ = make(7, (513, 1024), 515)
         if special:
@@ -260,7 +287,10 @@ def test_inside_transformations(J, monkeypatch, small):
     np.testing.assert_allclose(gp.numpy().reshape(6, 8, 32), g, rtol=1e-5, atol=1e-6)
 
 
-def test_only_the_wanted_gradients(J):
+@pytest.mark.parametrize("small", [True, False])
+def test_only_the_wanted_gradients(J, monkeypatch, small):
+    from jax4j_b200 import layers
+    monkeypatch.setattr(layers, "SMALL_PRODUCT", layers.SMALL_PRODUCT if small else 0)
     x, w, b, _, dy = make(11, (600, 700), 800, residual=False)
     X, W, B = arr(J, x), arr(J, w), arr(J, b)
     full = run(J, x, w, b, "gelu", None, dy)
@@ -270,9 +300,11 @@ def test_only_the_wanted_gradients(J):
         np.testing.assert_array_equal(J.JAX.vjp(f, arg)[1](DY)[0].numpy(), full[n])
 
 
-@pytest.mark.parametrize("shape,N", [((64, 200), 100), ((512, 1024), 600)])
-def test_recorded_and_on_another_stream(J, shape, N):
+@pytest.mark.parametrize("shape,N,small", [((64, 200), 100, True), ((512, 1024), 600, False)])
+def test_recorded_and_on_another_stream(J, monkeypatch, shape, N, small):
     import torch
+    from jax4j_b200 import layers
+    monkeypatch.setattr(layers, "SMALL_PRODUCT", layers.SMALL_PRODUCT if small else 0)
     from jax4j_b200.graphs import CapturedStep
     x, w, b, res, dy = make(12, shape, N)
     r = np.random.default_rng(13)

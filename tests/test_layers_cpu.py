@@ -80,7 +80,10 @@ def test_dense_c_entries_refuse_bad_arguments():
     told(L.j4c_dense_grad(0, 2, 3, fake, None, 3, 0, fake, None, None, None, 0, None), "NULL")
     told(L.j4c_dense_grad(0, 2, 3, fake, fake, 5, 1, fake, None, None, None, 0, None), "does not tell")
     told(L.j4c_dense_grad(1, 2, 3, fake, fake, 2, 1, fake, None, fake, None, 0, None), "line words")
-    told(L.j4c_dense_grad(0, 200, 3, fake, fake, 2, 1, fake, fake, None, None, 0, None), "workspace")
+    told(L.j4c_dense_backward(fake, fake, 2, 3, 4, fake, None, 0, 0, None, None, None, fake, None, 0, None), "neither product")
+    told(L.j4c_dense_backward(fake, fake, 2, 3, 4, fake, fake, 5, 0, None, fake, fake, None, None, 0, None), "NULL")
+    told(L.j4c_dense_backward(fake, None, 2, 3, 4, fake, None, 0, 0, None, fake, fake, None, None, 0, None), "NULL")
+    told(L.j4c_dense_grad(0, 2000, 3, fake, fake, 2, 1, fake, fake, None, None, 0, None), "workspace")
 
 
 def test_layers_are_one_equation():
