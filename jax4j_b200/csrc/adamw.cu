@@ -7,17 +7,21 @@
 // b = 1 / sqrt(1 - beta2^t) computed in FP64 from the running powers of the
 // betas that travel with the state (no host knows t, so a recorded graph
 // counts on).  Every product and sum is rounded on its own (no FMA), so an
-// elementwise evaluation of the same expressions gives the same bits.
+// elementwise evaluation of the same expressions gives the same bits (with
+// moments in 8 bits the quotient is within 2 ulp).
 //
-// The step is bound by HBM: 28 B per FLOAT32 element (w, g, m, v read; w, m, v
-// written), 16.1 B with moments in 8 bits.  All tensors of a tree share one
+// Bound by HBM with moments in the tensors' type: 28 B per FLOAT32 element (w,
+// g, m, v read; w, m, v written), 41.9 M elements in 209 us = 5.6 TB/s.  With
+// moments in 8 bits 16.1 B, and bound by instructions (some 100 an element, a
+// third of them the IEEE root and quotient and the root's encoding): 190 us =
+// 3.6 TB/s; four elements a lane and an IEEE quotient took 207.  All tensors of a tree share one
 // launch: the table of pointers travels in the kernel's parameters (no copy to
 // the device, nothing a captured graph would have to keep alive), and a CTA
 // takes chunks of consecutive elements, finding a chunk's tensor by bisection.
 //
-// Moments in 8 bits.  A tensor is cut into blocks of 128 elements, one warp's
-// four elements per lane, so a block's largest value is one warp reduction of
-// registers.  First moments are e4m3 floats; of the second moment the root is
+// Moments in 8 bits.  A tensor is cut into blocks of 128 elements, half a
+// warp's eight elements per lane, so a block's largest value is one reduction
+// of registers.  First moments are e4m3 floats; of the second moment the root is
 // held (the update needs the root anyway, and it has half the range), in
 // unsigned floats of 4 exponent and 4 fraction bits, whose smallest value a
 // non-zero root never falls below -- a zero would divide by eps alone.  Each
@@ -84,6 +88,9 @@ __device__ __forceinline__ double r_sqrt(double x) { return __dsqrt_rn(x); }
 // r_div without its shortcut for zero dividends, which are rare here
 __device__ __forceinline__ float q_div(float a, float b) { return __fdiv_rn(a, b); }
 __device__ __forceinline__ double q_div(double a, double b) { return __ddiv_rn(a, b); }
+// Within 2 ulp for divisors below 2^126 and 0 above (the divisor is a root, at
+// most 2^64, times b, plus eps): no branch, so eight of them overlap.
+__device__ __forceinline__ float fast_div(float a, float b) { return __fdividef(a, b); }
 
 // What a step needs beside the elements, in the elements' type.
 template <typename T>
@@ -115,14 +122,18 @@ struct Coef {
     }
 };
 
-// m, v in: the old moments; out: the new ones and the root of v.
-template <typename T>
+// m, v in: the old moments; out: the new ones and the root of v.  FAST: the
+// update's quotient within 2 ulp.
+template <typename T, bool FAST = false>
 __device__ __forceinline__ T adamw_element(const Coef<T> &k, T decay, T w, T g, T &m, T &v, T &root) {
     if (k.scaled) g = r_mul(g, k.scale);
     m = r_add(r_mul(m, k.b1), r_mul(g, k.c1));
     v = r_add(r_mul(v, k.b2), r_mul(r_mul(g, g), k.c2));
     root = r_sqrt(v);
-    const T update = q_div(r_mul(m, k.a), r_add(r_mul(root, k.b), k.eps));
+    const T up = r_mul(m, k.a), down = r_add(r_mul(root, k.b), k.eps);
+    T update;
+    if constexpr (FAST) update = fast_div(up, down);
+    else update = q_div(up, down);
     return r_sub(r_sub(w, r_mul(w, decay)), r_mul(update, k.lr));
 }
 
@@ -189,8 +200,8 @@ __global__ void __launch_bounds__(kThreads, kCtas) adamw_kernel(const __grid_con
 // ---- moments in 8 bits -----------------------------------------------------------
 // A packed state of nb blocks: nb * 32 words of first-moment codes, nb * 32 of
 // root codes, nb steps of the first moments, nb steps of the roots.
-// Four codes of a word each way; the codes of four elements are one register.
-__device__ __forceinline__ void decode_m(uint32_t codes, float step, float (&x)[4]) {
+// Four codes of a word each way.
+__device__ __forceinline__ void decode_m(uint32_t codes, float step, float *x) {
 #pragma unroll
     for (int p = 0; p < 2; p++) {
         const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(codes >> (16 * p)), __NV_E4M3);
@@ -202,7 +213,7 @@ __device__ __forceinline__ void decode_m(uint32_t codes, float step, float (&x)[
 // Bits 7..4 the exponent, 3..0 the fraction: read as an FP32 number's (its
 // subnormals included) and scaled by 2^120, exponent 0 is 2^-6 and below it
 // the code counts 2^-10s.  0xFF is NaN.
-__device__ __forceinline__ void decode_r(uint32_t codes, float step, float (&x)[4]) {
+__device__ __forceinline__ void decode_r(uint32_t codes, float step, float *x) {
 #pragma unroll
     for (int e = 0; e < 4; e++) {
         const uint32_t at = e < 3 ? codes << (19 - 8 * e) : codes >> 5;  // this code's bits at 26..19
@@ -215,7 +226,7 @@ __device__ __forceinline__ void decode_r(uint32_t codes, float step, float (&x)[
             if (((codes >> (8 * e)) & 0xFFu) == 0xFFu) x[e] = __int_as_float(0x7FC00000);
     }
 }
-__device__ __forceinline__ uint32_t encode_m(const float (&y)[4]) {
+__device__ __forceinline__ uint32_t encode_m(const float *y) {
     uint32_t c = 0;
 #pragma unroll
     for (int p = 0; p < 2; p++)
@@ -244,9 +255,54 @@ __device__ __forceinline__ void block_scale(uint32_t top_bits, float top_code, f
     step = held ? r_mul(top, 1.0f / top_code) : 0.0f;
 }
 
+// A warp takes two neighbouring blocks, half a warp each and eight elements a
+// lane: what a lane computes for its block (addresses, the step, its inverse)
+// is shared by eight.
+__device__ __forceinline__ uint32_t half_max(uint32_t v) {
+    return __reduce_max_sync(threadIdx.x % 32 < 16 ? 0x0000FFFFu : 0xFFFF0000u, v);
+}
+struct Packed {  // a packed state's parts
+    uint32_t *m, *r;
+    float *steps_m, *steps_r;
+    __device__ __forceinline__ Packed(const void *q, int64_t nb) {
+        m = static_cast<uint32_t *>(const_cast<void *>(q));
+        r = m + nb * 32;
+        steps_m = reinterpret_cast<float *>(r + nb * 32);
+        steps_r = steps_m + nb;
+    }
+};
+// Eight codes of a lane, at word `at`: one load where the state is 8-byte aligned.
+__device__ __forceinline__ uint2 load_codes(const uint32_t *p, int64_t at, bool vec) {
+    return vec ? *reinterpret_cast<const uint2 *>(p + at) : make_uint2(p[at], p[at + 1]);
+}
+__device__ __forceinline__ void store_codes(uint32_t *p, int64_t at, bool vec, uint2 c) {
+    if (vec) *reinterpret_cast<uint2 *>(p + at) = c;
+    else p[at] = c.x, p[at + 1] = c.y;
+}
+// Eight values at p, those from `left` on behind the tensor.
+__device__ __forceinline__ void load8(const float *p, bool whole, int left, float (&x)[8]) {
+    if (whole) {
+        const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 4);
+        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = e < left ? p[e] : 0.0f;
+    }
+}
+__device__ __forceinline__ void store8(float *p, bool whole, int left, const float (&x)[8]) {
+    if (whole) {
+        *reinterpret_cast<float4 *>(p) = make_float4(x[0], x[1], x[2], x[3]);
+        *reinterpret_cast<float4 *>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            if (e < left) p[e] = x[e];
+    }
+}
+
 template <int N>
 __global__ void __launch_bounds__(kThreads, kCtas) adamw_q8_kernel(const __grid_constant__ Table<N> tab,
-                                                            const __grid_constant__ Hyper h) {
+                                                                   const __grid_constant__ Hyper h) {
     const Coef<float> k(h);
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     for (int chunk = blockIdx.x; chunk < tab.chunks; chunk += gridDim.x) {
@@ -256,106 +312,77 @@ __global__ void __launch_bounds__(kThreads, kCtas) adamw_q8_kernel(const __grid_
         const int per = tab.chunk_elems / kQBlock;  // blocks of a chunk
         const int64_t b0 = (int64_t)(chunk - t.first) * per, b1 = min(nb, b0 + per);
         const float *w = static_cast<const float *>(t.w), *g = static_cast<const float *>(t.g);
-        const uint32_t *q = static_cast<const uint32_t *>(t.m);
-        uint32_t *qo = static_cast<uint32_t *>(t.m_out);
         float *wo = static_cast<float *>(t.w_out);
-        const float *steps = reinterpret_cast<const float *>(q + nb * 64);
-        float *steps_out = reinterpret_cast<float *>(qo + nb * 64);
+        const Packed q(t.m, nb), qo(t.m_out, nb);
         const float decay = k.decay(h, t.wd);
-        for (int64_t b = b0 + warp; b < b1; b += 2 * (kThreads / 32)) {
-            // two blocks of a warp in flight (see adamw_kernel)
-            const int64_t blk[2] = {b, b + kThreads / 32};
-            const bool both = blk[1] < b1;
-            float ww[2][4], gg[2][4], sm[2], sr[2];
-            uint32_t cm[2], cr[2];
-            int left[2];  // of the lane's four elements, those inside the tensor
+        for (int64_t b = b0 + 2 * warp + lane / 16; b < b1; b += 2 * (kThreads / 32)) {  // a half warp's block
+            const int64_t i = b * kQBlock + (lane % 16) * 8, at = b * 32 + (lane % 16) * 2;
+            const int left = (int)max((int64_t)0, min((int64_t)8, n - i));  // of the lane's elements, those in the tensor
+            const bool whole = vec && left == 8;
+            float ww[8], gg[8], mm[8], rr[8];
+            load8(w + i, whole, left, ww);
+            load8(g + i, whole, left, gg);
+            const uint2 cm = load_codes(q.m, at, vec), cr = load_codes(q.r, at, vec);
+            const float sm = q.steps_m[b], sr = q.steps_r[b];
+            decode_m(cm.x, sm, mm);
+            decode_m(cm.y, sm, mm + 4);
+            decode_r(cr.x, sr, rr);
+            decode_r(cr.y, sr, rr + 4);
+            uint32_t top_m = 0, top_r = 0;
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
-                if (u == 1 && !both) break;
-                const int64_t i = blk[u] * kQBlock + lane * 4;
-                left[u] = (int)max((int64_t)0, min((int64_t)4, n - i));
-                if (vec && left[u] == 4) {
-                    const float4 a = *reinterpret_cast<const float4 *>(w + i);
-                    const float4 c = *reinterpret_cast<const float4 *>(g + i);
-                    ww[u][0] = a.x, ww[u][1] = a.y, ww[u][2] = a.z, ww[u][3] = a.w;
-                    gg[u][0] = c.x, gg[u][1] = c.y, gg[u][2] = c.z, gg[u][3] = c.w;
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        ww[u][e] = e < left[u] ? w[i + e] : 0.0f;
-                        gg[u][e] = e < left[u] ? g[i + e] : 0.0f;
-                    }
-                }
-                cm[u] = q[blk[u] * 32 + lane], cr[u] = q[(nb + blk[u]) * 32 + lane];
-                sm[u] = steps[blk[u]], sr[u] = steps[nb + blk[u]];
+            for (int e = 0; e < 8; e++) {
+                float v = r_mul(rr[e], rr[e]);
+                ww[e] = adamw_element<float, true>(k, decay, ww[e], gg[e], mm[e], v, rr[e]);
             }
+            if (left < 8) {  // behind the tensor: zeros
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
-                if (u == 1 && !both) break;  // the same for the whole warp
-                const int64_t i = blk[u] * kQBlock + lane * 4;
-                float mm[4], rr[4];
-                decode_m(cm[u], sm[u], mm);
-                decode_r(cr[u], sr[u], rr);
-                uint32_t top_m = 0, top_r = 0;
+                for (int e = 0; e < 8; e++)
+                    if (e >= left) mm[e] = rr[e] = 0.0f;
+            }
+            store8(wo + i, whole, left, ww);
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    float v = r_mul(rr[e], rr[e]);
-                    ww[u][e] = adamw_element(k, decay, ww[u][e], gg[u][e], mm[e], v, rr[e]);
-                }
-                if (left[u] < 4) {  // behind the tensor: zeros
+            for (int e = 0; e < 8; e++) {
+                top_m = max(top_m, abs_bits(mm[e]));
+                top_r = max(top_r, abs_bits(rr[e]));
+            }
+            top_m = half_max(top_m);
+            top_r = half_max(top_r);
+            const bool odd = max(top_m, top_r) >= kInfBits;  // of the whole block: a value is not finite
+            if (odd) {
+                top_m = top_r = 0;
 #pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        if (e >= left[u]) mm[e] = rr[e] = 0.0f;
+                for (int e = 0; e < 8; e++) {
+                    if (abs_bits(mm[e]) < kInfBits) top_m = max(top_m, abs_bits(mm[e]));
+                    if (abs_bits(rr[e]) < kInfBits) top_r = max(top_r, abs_bits(rr[e]));
                 }
+                top_m = half_max(top_m);
+                top_r = half_max(top_r);
+            }
+            float inv_m, inv_r, step_m, step_r;
+            block_scale(top_m, kTopM, inv_m, step_m);
+            block_scale(top_r, kTopR, inv_r, step_r);
+            float ym[8];
+            uint32_t om[2], orr[2] = {0, 0};
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    top_m = max(top_m, abs_bits(mm[e]));
-                    top_r = max(top_r, abs_bits(rr[e]));
-                }
-                top_m = __reduce_max_sync(0xffffffffu, top_m);
-                top_r = __reduce_max_sync(0xffffffffu, top_r);
-                const bool odd = max(top_m, top_r) >= kInfBits;  // of the whole warp: a value is not finite
-                if (odd) {
-                    top_m = top_r = 0;
+            for (int e = 0; e < 8; e++) {
+                ym[e] = r_mul(mm[e], inv_m);
+                orr[e / 4] |= encode_r(r_mul(rr[e], inv_r)) << (8 * (e % 4));
+            }
+            om[0] = encode_m(ym);
+            om[1] = encode_m(ym + 4);
+            if (odd) {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        if (abs_bits(mm[e]) < kInfBits) top_m = max(top_m, abs_bits(mm[e]));
-                        if (abs_bits(rr[e]) < kInfBits) top_r = max(top_r, abs_bits(rr[e]));
-                    }
-                    top_m = __reduce_max_sync(0xffffffffu, top_m);
-                    top_r = __reduce_max_sync(0xffffffffu, top_r);
+                for (int e = 0; e < 8; e++) {
+                    const int s = 8 * (e % 4);
+                    if (abs_bits(mm[e]) >= kInfBits) om[e / 4] = (om[e / 4] & ~(0xFFu << s)) | 0x7Fu << s;
+                    if (abs_bits(rr[e]) >= kInfBits) orr[e / 4] |= 0xFFu << s;
                 }
-                float inv_m, inv_r, step_m, step_r;
-                block_scale(top_m, kTopM, inv_m, step_m);
-                block_scale(top_r, kTopR, inv_r, step_r);
-                float ym[4];
-                uint32_t orr = 0;
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    ym[e] = r_mul(mm[e], inv_m);
-                    orr |= encode_r(r_mul(rr[e], inv_r)) << (8 * e);
-                }
-                uint32_t om = encode_m(ym);
-                if (odd) {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        if (abs_bits(mm[e]) >= kInfBits) om = (om & ~(0xFFu << (8 * e))) | 0x7Fu << (8 * e);
-                        if (abs_bits(rr[e]) >= kInfBits) orr |= 0xFFu << (8 * e);
-                    }
-                }
-                qo[blk[u] * 32 + lane] = om;
-                qo[(nb + blk[u]) * 32 + lane] = orr;
-                if (lane == 0) {
-                    steps_out[blk[u]] = step_m;
-                    steps_out[nb + blk[u]] = step_r;
-                }
-                if (vec && left[u] == 4) {
-                    *reinterpret_cast<float4 *>(wo + i) = make_float4(ww[u][0], ww[u][1], ww[u][2], ww[u][3]);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        if (e < left[u]) wo[i + e] = ww[u][e];
-                }
+            }
+            store_codes(qo.m, at, vec, make_uint2(om[0], om[1]));
+            store_codes(qo.r, at, vec, make_uint2(orr[0], orr[1]));
+            if (lane % 16 == 0) {
+                qo.steps_m[b] = step_m;
+                qo.steps_r[b] = step_r;
             }
         }
     }
@@ -368,48 +395,32 @@ __global__ void __launch_bounds__(kThreads, kCtas) adamw_moments_kernel(const __
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     for (int chunk = blockIdx.x; chunk < tab.chunks; chunk += gridDim.x) {
         const Tensor &t = tensor_of(tab, chunk);
-        const int64_t nb = (t.n + kQBlock - 1) / kQBlock;
+        const int64_t n = t.n, nb = (n + kQBlock - 1) / kQBlock;
+        const bool vec = t.vec;
         const int per = tab.chunk_elems / kQBlock;
         const int64_t b0 = (int64_t)(chunk - t.first) * per, b1 = min(nb, b0 + per);
-        const uint32_t *q = static_cast<const uint32_t *>(t.m);
-        const float *steps = reinterpret_cast<const float *>(q + nb * 64);
+        const Packed q(t.m, nb);
         float *mo = static_cast<float *>(t.m_out), *vo = static_cast<float *>(t.v_out);
-        const int64_t n = t.n;
-        const bool vec = t.vec;
-        for (int64_t b = b0 + warp; b < b1; b += 2 * (kThreads / 32)) {
-            const int64_t blk[2] = {b, b + kThreads / 32};  // two blocks of a warp in flight
-            uint32_t cm[2], cr[2];
-            float sm[2], sr[2];
+        for (int64_t b = b0 + 2 * warp + lane / 16; b < b1; b += 2 * (kThreads / 32)) {
+            const int64_t i = b * kQBlock + (lane % 16) * 8, at = b * 32 + (lane % 16) * 2;
+            const int left = (int)max((int64_t)0, min((int64_t)8, n - i));
+            const bool whole = vec && left == 8;
+            const uint2 cm = load_codes(q.m, at, vec), cr = load_codes(q.r, at, vec);
+            const float sm = q.steps_m[b], sr = q.steps_r[b];
+            float m[8], r[8];
+            decode_m(cm.x, sm, m);
+            decode_m(cm.y, sm, m + 4);
+            decode_r(cr.x, sr, r);
+            decode_r(cr.y, sr, r + 4);
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
-                if (blk[u] >= b1) break;
-                cm[u] = q[blk[u] * 32 + lane], cr[u] = q[(nb + blk[u]) * 32 + lane];
-                sm[u] = steps[blk[u]], sr[u] = steps[nb + blk[u]];
-            }
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                if (blk[u] >= b1) break;
-                const int64_t i = blk[u] * kQBlock + lane * 4;
-                float m[4], r[4];
-                decode_m(cm[u], sm[u], m);
-                decode_r(cr[u], sr[u], r);
-#pragma unroll
-                for (int e = 0; e < 4; e++) r[e] = r_mul(r[e], r[e]);
-                if (vec && i + 4 <= n) {
-                    *reinterpret_cast<float4 *>(mo + i) = make_float4(m[0], m[1], m[2], m[3]);
-                    *reinterpret_cast<float4 *>(vo + i) = make_float4(r[0], r[1], r[2], r[3]);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        if (i + e < n) {
-                            mo[i + e] = m[e];
-                            vo[i + e] = r[e];
-                        }
-                }
-            }
+            for (int e = 0; e < 8; e++) r[e] = r_mul(r[e], r[e]);
+            store8(mo + i, whole, left, m);
+            store8(vo + i, whole, left, r);
         }
     }
 }
+
+bool aligned8(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0; }
 
 // Lays the tensors' chunks out and launches; chunks of 2048 elements (two
 // vectors of every thread), or of 1024 when that leaves SMs without one.
@@ -496,6 +507,7 @@ int j4c_adamw_step(int dtype, int state_bits, int ntensors, const int64_t *numel
         t.w = w[i], t.g = g[i], t.w_out = w_out[i], t.wd = weight_decay[i];
         t.m = state[per * i], t.m_out = state_out[per * i];
         t.vec = aligned16(t.w) && aligned16(t.g) && aligned16(t.w_out);
+        if (per == 1) t.vec = t.vec && aligned8(t.m) && aligned8(t.m_out);
         if (per == 2) {
             t.v = state[2 * i + 1], t.v_out = state_out[2 * i + 1];
             t.vec = t.vec && aligned16(t.m) && aligned16(t.v) && aligned16(t.m_out) && aligned16(t.v_out);
@@ -532,7 +544,7 @@ int j4c_adamw_moments(int ntensors, const int64_t *numel, const void *const *sta
     cudaStream_t s = as_stream(stream);
     auto fill = [&](int i, Tensor &t) {
         t.m = state[i], t.m_out = m_out[i], t.v_out = v_out[i];
-        t.vec = aligned16(t.m_out) && aligned16(t.v_out);
+        t.vec = aligned16(t.m_out) && aligned16(t.v_out) && aligned8(t.m);
     };
     auto launch = [&](auto &tab, unsigned grid) {
         constexpr int N = sizeof(tab.t) / sizeof(tab.t[0]);

@@ -153,7 +153,8 @@ def test_eight_bit_steps(J, offset):
             with np.errstate(divide="ignore", invalid="ignore"):
                 up = np.abs(1e-2 * m1 / (1 - 0.9 ** t) / (np.sqrt(v1 / (1 - 0.999 ** t)) + 1e-8))
             mag = np.abs(0.9 * m0) / np.maximum(np.abs(m1), 1e-300)
-            assert np.all(np.abs(got_w[i] - w1) <= ew + up * U * (2 + mag)), (i, t)
+            # the quotient is off by up to 2 ulp (4 U), of which ref_step counts one rounding
+            assert np.all(np.abs(got_w[i] - w1) <= ew + up * U * (5 + mag)), (i, t)
             m, r, sm, sr = after[i]
             r1 = np.sqrt(v1)
             # half a step of the code (2^-4 and 2^-5 relative, 2^-10 and 2^-11 of the block's step below the
