@@ -82,13 +82,13 @@ __global__ void __launch_bounds__(kRowsThreads) rows_kernel(const Product p) {
                     const float *at = w + (int64_t)(k + 8 * u) * p.N;
                     const bool in = k + 8 * u < len;
                     if constexpr (V == 4) {
-                        const float4 t = in ? __ldcs(reinterpret_cast<const float4 *>(at)) : float4{0, 0, 0, 0};
+                        const float4 t = in ? __ldg(reinterpret_cast<const float4 *>(at)) : float4{0, 0, 0, 0};
                         b[u][0] = t.x, b[u][1] = t.y, b[u][2] = t.z, b[u][3] = t.w;
                     } else if constexpr (V == 2) {
-                        const float2 t = in ? __ldcs(reinterpret_cast<const float2 *>(at)) : float2{0, 0};
+                        const float2 t = in ? __ldg(reinterpret_cast<const float2 *>(at)) : float2{0, 0};
                         b[u][0] = t.x, b[u][1] = t.y;
                     } else {
-                        b[u][0] = in ? __ldcs(at) : 0.0f;
+                        b[u][0] = in ? __ldg(at) : 0.0f;
                     }
                 }
 #pragma unroll

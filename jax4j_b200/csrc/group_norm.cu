@@ -916,11 +916,14 @@ static int check_shape(const char *name, int dtype, int64_t B, int64_t S, int64_
     J4C_REQUIRE(eps >= 0.0, "%s: negative eps", name);
     J4C_REQUIRE(act_known(act), "%s: unknown activation %d", name, act);
     J4C_REQUIRE(S < (1ll << 31) && C < (1ll << 31), "%s: extents of 2^31 and more are not supported", name);
+    J4C_REQUIRE((double)B * (double)S * (double)C < 1e18, "%s: [%lld, %lld, %lld] is too large", name, (long long)B,
+                (long long)S, (long long)C);
     return J4C_OK;
 }
 
 size_t j4c_group_norm_workspace(int dtype, int64_t B, int64_t S, int64_t C, int64_t groups, int backward) {
     if (B <= 0 || S <= 0 || C < 1 || groups < 1 || C % groups) return 0;
+    if ((double)B * (double)S * (double)C >= 1e18) return 0;  // refused by the calls
     return dtype == J4C_FLOAT64 ? workspace<double>(B, S, C, groups, backward != 0)
                                 : workspace<float>(B, S, C, groups, backward != 0);
 }

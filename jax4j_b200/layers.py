@@ -169,8 +169,13 @@ class _GroupNorm(FfiMeta):
 SMALL_PRODUCT = 1 << 29
 
 
+# As many rows or fewer run there whatever the weight's size: they are bound by
+# reading it once, which the splits read, write and read again.
+FEW_ROWS = 16
+
+
 def _small(M: int, K: int, N: int) -> bool:
-    return M * K * N <= SMALL_PRODUCT
+    return M * K * N <= SMALL_PRODUCT or not (M and N and K)
 
 
 def dense(x: NDArray, w: NDArray, bias: Optional[NDArray], activation: Optional[str],
@@ -236,7 +241,7 @@ class _Dense(FfiMeta):
         rp = residual._t.data_ptr() if residual is not None else None
         zp = z.data_ptr() if z is not None else None
         lines = None
-        if f32 and (_small(M, K, N) or not (M and N and K)):
+        if f32 and (M <= FEW_ROWS or _small(M, K, N)):
             call("j4c_dot_act", t.data_ptr(), w._t.data_ptr(), M, K, N, 0, 0, bp, self.act, rp, zp, y.data_ptr(), stream)
         elif f32:
             if keep:  # with those that the gradient's products take, each operand's in one pass
@@ -267,7 +272,7 @@ class _Dense(FfiMeta):
         want_bias = self.has_bias and wanted[2]
         products = wanted[0] or wanted[1]
         f32 = dt == DType.FLOAT32
-        small = f32 and (_small(M, K, N) or not (M and N and K))
+        small = f32 and _small(M, K, N)
         dz, dbias, lines = t, None, None
         grads: List[Optional[ConcreteNDArray]] = [None, None]
         if want_bias or products:

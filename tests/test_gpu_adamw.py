@@ -203,6 +203,18 @@ def test_many_leaves(J, count, bits):
     assert state.step().numpy()[0] == 1.0
 
 
+@pytest.mark.parametrize("bits", [8, 32])
+def test_empty_trees_and_leaves(J, bits):
+    """Nothing to update: the count still advances."""
+    for arrays in ([], [arr(J, np.zeros(0, np.float32))], [arr(J, np.zeros((0, 4), np.float32))] * 2):
+        params = tree(J, arrays)
+        p, s = J.Optim.adamW(params, params, J.Optim.adamWInit(params, bits), 1e-2, beta2=0.5)
+        assert len(J.PyTrees.flatten(p)) == len(arrays)
+        np.testing.assert_array_equal(s.step().numpy(), [1.0, 0.9, 0.5])
+        m, _ = s.moments()
+        assert [a.numpy().shape for a in J.PyTrees.flatten(m)] == [a.shape().dimensions() for a in arrays]
+
+
 def test_mixed_dtypes_take_one_count(J):
     w32, g32 = make(5, [300])
     w64, g64 = make(6, [200], np.float64)

@@ -25,9 +25,10 @@ def arr(J, x, offset=0):
 def steps(K, tensor):
     """Error of a K-term product, in half steps of sum |a||b|.  CUDA cores: K
     roundings of mean zero, 8 standard deviations of their sum.  Tensor cores:
-    48 truncating MMAs of a 256-deep chunk at 3.6e-8 (29 U), the splits' 2^-22
-    (4 U) and K / 256 additions of chunks."""
-    return 33 + K / 256 + 8 if tensor else 8 * np.sqrt(K) + 8
+    48 truncating MMAs of a 256-deep chunk at 3.6e-8 (29 U; 3xTF32: 96 of them),
+    the splits' 2^-22 (4 U) and K / 128 additions of chunks."""
+    from jax4j_b200 import core
+    return (29 if core.split_kind() == 1 else 58) + 4 + K / 128 + 8 if tensor else 8 * np.sqrt(K) + 8
 
 
 def reference(x, w, bias, name, residual, dy, unit, tensor):
@@ -112,7 +113,7 @@ def test_small_products(J, shape, N, f64):
     check(run(J, x, w, b, name, res, dy), reference(x, w, b, name, res, dy, 2.0 ** -53 if f64 else U, False))
 
 
-LARGE = [((1, 5), 3), ((128, 64), 256), ((130, 64), 260), ((257, 1000), 513), ((300, 513), 1000), ((3, 100, 48), 77),
+LARGE = [((17, 5), 3), ((128, 64), 256), ((130, 64), 260), ((257, 1000), 513), ((300, 513), 1000), ((3, 100, 48), 77),
          ((1024, 300), 1000), ((600, 2048), 512)]
 
 
@@ -156,6 +157,34 @@ def test_at_the_border_between_the_products(J):
     for M in (1024, 1025):
         x, w, b, res, dy = make(M, (M, 1024), 512)
         check(run(J, x, w, b, "gelu", res, dy), reference(x, w, b, "gelu", res, dy, U, M == 1025))
+
+
+def test_few_rows_of_a_large_weight(J):
+    """Up to 16 rows stay on the CUDA cores forward, whatever the weight; their
+    gradients take the tensor cores beyond SMALL_PRODUCT."""
+    from jax4j_b200 import layers
+    assert layers.FEW_ROWS == 16
+    x, w, b, res, dy = make(14, (16, 6000), 6004)
+    assert 16 * 6000 * 6004 > layers.SMALL_PRODUCT
+    ref = reference(x, w, b, "silu", res, dy, U, True)
+    small = reference(x, w, b, "silu", res, dy, U, False)["y"]
+    got = run(J, x, w, b, "silu", res, dy)
+    check({"y": got.pop("y")}, {"y": small})
+    # the pre-activation's error is the larger of the two forms'
+    check(got, {n: (v, np.maximum(e, reference(x, w, b, "silu", res, dy, U, False)[n][1])) for n, (v, e) in ref.items()})
+
+
+@pytest.mark.parametrize("env", [{"J4C_GEMM_SPLIT": "tf32"}, {"J4C_GEMM_PAIR": "0"}])
+def test_other_gemm_variants(env):
+    """The tensor-core layers under 3xTF32 and with single-CTA tiles (both are fixed for a process)."""
+    import os
+    import subprocess
+    import sys
+    r = subprocess.run([sys.executable, "-m", "pytest", "-q", "-x", "tests/test_gpu_dense.py", "-k",
+                        "tensor_core or line_words or non_finite or border"], env={**os.environ, **env},
+                       capture_output=True, text=True, timeout=600,
+                       cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert r.returncode == 0, r.stdout[-3000:] + r.stderr[-2000:]
 
 
 @pytest.mark.parametrize("rows,cols", [(1, 1), (7, 100), (33, 1024), (40, 1028), (5, 4097), (9, 8192), (300, 512), (3, 8195)])

@@ -104,7 +104,7 @@ SHAPES = [((1, 1), 1), ((3, 7), 7), ((2, 16), 4), ((5, 3, 10), 5), ((4, 17, 24),
           ((2, 8, 8, 64), 8), ((2, 100, 96), 6), ((3, 127, 32), 1), ((600, 4096), 1), ((3, 4095), 1), ((2, 5, 5000), 4),
           ((5, 8192), 1),
           ((1, 8193, 1), 1), ((2, 1000, 20), 2), ((3, 700, 250), 10), ((1, 9000), 1), ((2, 5, 12300), 3),
-          ((2, 3, 40000), 4), ((1, 20000, 6), 2), ((2, 33, 33, 320), 32), ((1, 4097, 2052), 1), ((41, 1024, 512), 8)]
+          ((2, 3, 40000), 4), ((1, 20000, 6), 2), ((2, 33, 33, 320), 32), ((1, 4097, 2052), 1), ((2, 9000, 40), 40), ((2, 100, 4096), 32), ((41, 1024, 512), 8)]
 
 
 @pytest.mark.parametrize("shape,G", SHAPES, ids=[f"{'x'.join(map(str, s))}g{g}" for s, g in SHAPES])
