@@ -702,11 +702,10 @@ J4C_API int j4c_group_norm_grad(int dtype, int64_t B, int64_t S, int64_t C, int6
 /* A dense layer, y = act(x . w + bias) + residual (bias [N], residual [M, N]
  * and the pre-activation z [M, N] may each be NULL), FLOAT32:
  * from splits, x's by rows (j4c_split_f32) and w's transposed
- * (j4c_split_f32_transposed), on the tensor cores, with the line words of y in
- * out_lines ([M + N + 1], may be NULL) as j4c_dot_split_ep_bits leaves them; */
+ * (j4c_split_f32_transposed), on the tensor cores; */
 J4C_API int j4c_dot_split_act(const float *x_hi, const float *x_lo, const float *wt_hi, const float *wt_lo, int64_t M,
                               int64_t K, int64_t N, const float *bias, int act, const float *residual, float *z,
-                              float *y, uint32_t *out_lines, j4c_stream stream);
+                              float *y, j4c_stream stream);
 /* and from the arrays themselves, op(A) . op(B) in FP32 FMAs in one launch, for
  * products too small for the splits to pay (K = 0: the sum is 0). */
 J4C_API int j4c_dot_act(const float *a, const float *b, int64_t M, int64_t K, int64_t N, int trans_a, int trans_b,

@@ -226,7 +226,7 @@ public final class J4C {
     // ---- dense layers (dense.cu) ----
     static final MethodHandle DOT_SPLIT_ACT = h("j4c_dot_split_act", FunctionDescriptor.of(
         JAVA_INT, ADDRESS, ADDRESS, ADDRESS, ADDRESS, JAVA_LONG, JAVA_LONG, JAVA_LONG, ADDRESS, JAVA_INT, ADDRESS,
-        ADDRESS, ADDRESS, ADDRESS, ADDRESS));
+        ADDRESS, ADDRESS, ADDRESS));
     static final MethodHandle DOT_ACT = h("j4c_dot_act", FunctionDescriptor.of(
         JAVA_INT, ADDRESS, ADDRESS, JAVA_LONG, JAVA_LONG, JAVA_LONG, JAVA_INT, JAVA_INT, ADDRESS, JAVA_INT, ADDRESS,
         ADDRESS, ADDRESS, ADDRESS));

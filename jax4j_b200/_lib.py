@@ -129,7 +129,7 @@ SIGNATURES = {
     "j4c_adamw_step": [I32, I32, I32, P, P, P, P, P, P, P, P, P, P, C.c_double, C.c_double, C.c_double, C.c_double,
                        C.c_double, P],
     "j4c_adamw_moments": [I32, P, P, P, P, P],
-    "j4c_dot_split_act": [P, P, P, P, I64, I64, I64, P, I32, P, P, P, P, P],
+    "j4c_dot_split_act": [P, P, P, P, I64, I64, I64, P, I32, P, P, P, P],
     "j4c_dot_act": [P, P, I64, I64, I64, I32, I32, P, I32, P, P, P, P],
     "j4c_dense_finish": [I32, P, I64, I64, P, I32, P, P, P],
     "j4c_dense_grad_workspace": [I32, I64, I64],

@@ -15,8 +15,7 @@ namespace cg = cooperative_groups;
 namespace j4c {
 
 int tc_gemm_act(const float *ah, const float *al, const float *bh, const float *bl, int64_t M, int64_t K, int64_t N,
-                const float *bias, int act, const float *residual, float *z, float *y, uint32_t *out_lines,
-                cudaStream_t s);
+                const float *bias, int act, const float *residual, float *z, float *y, cudaStream_t s);
 bool tc_gemm_supported(int64_t M, int64_t K, int64_t N);
 
 namespace {
@@ -547,20 +546,16 @@ int j4c_dot_act(const float *a, const float *b, int64_t M, int64_t K, int64_t N,
 
 int j4c_dot_split_act(const float *a_hi, const float *a_lo, const float *bt_hi, const float *bt_lo, int64_t M, int64_t K,
                       int64_t N, const float *bias, int act, const float *residual, float *z, float *y,
-                      uint32_t *out_lines, j4c_stream stream) {
+                      j4c_stream stream) {
     J4C_REQUIRE(M >= 0 && K >= 0 && N >= 0, "j4c_dot_split_act: negative dimension");
     J4C_REQUIRE(act_known(act), "j4c_dot_split_act: unknown activation %d", act);
-    J4C_REQUIRE(M == 0 || N == 0 || (y && a_hi && a_lo && bt_hi && bt_lo), "j4c_dot_split_act: NULL pointer");
-    J4C_REQUIRE(M == 0 || N == 0 || K > 0, "j4c_dot_split_act: K = 0");
-    if (M == 0 || N == 0) {
-        if (out_lines)
-            J4C_CUDA(cudaMemsetAsync(out_lines, 0, (size_t)(M + N + 1) * sizeof(uint32_t), as_stream(stream)));
-        return J4C_OK;
-    }
+    if (M == 0 || N == 0) return J4C_OK;
+    J4C_REQUIRE(y && a_hi && a_lo && bt_hi && bt_lo, "j4c_dot_split_act: NULL pointer");
+    J4C_REQUIRE(K > 0, "j4c_dot_split_act: K = 0");
     if (!tc_gemm_supported(M, K, N))
         return set_error(J4C_E_UNSUPPORTED, "j4c_dot_split_act: shape %lld x %lld x %lld is too large", (long long)M,
                          (long long)K, (long long)N);
-    return tc_gemm_act(a_hi, a_lo, bt_hi, bt_lo, M, K, N, bias, act, residual, z, y, out_lines, as_stream(stream));
+    return tc_gemm_act(a_hi, a_lo, bt_hi, bt_lo, M, K, N, bias, act, residual, z, y, as_stream(stream));
 }
 
 int j4c_dense_finish(int dtype, void *z, int64_t M, int64_t N, const void *bias, int act, const void *residual, void *y,

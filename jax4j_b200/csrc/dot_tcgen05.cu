@@ -144,8 +144,8 @@ struct Cfg {
     static constexpr int TMEM_COLS = 2 * BN;  // two partial-sum buffers
     static constexpr int COLS_PER_WARP = BN / 2;  // each epilogue warp owns half the columns
     static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 256;
-    // with an activation epilogue, a 32 x 33 staging area of every epilogue warp
-    static constexpr int ACT_SMEM_BYTES = SMEM_BYTES + kEpiWarps * 32 * 33 * 4;
+    // with an activation epilogue, a 32 x 32 staging area of every epilogue warp
+    static constexpr int ACT_SMEM_BYTES = SMEM_BYTES + kEpiWarps * 32 * 32 * 4;
     static_assert(ACT_SMEM_BYTES <= 232448 || STAGES * STAGE_BYTES > 196608, "shared memory budget");
     static_assert(TMEM_COLS == 256 || TMEM_COLS == 512, "TMEM allocation must be a power of 2");
     static_assert(SMEM_BYTES <= 232448, "shared memory budget");
@@ -473,7 +473,8 @@ __device__ __forceinline__ Unit unit_of(int u, int full_tiles, int splits, int n
 // With ACT (a template parameter of the kernel; operands both K-major, C
 // untransposed, one batch entry) instead:
 //   v = acc + bias[col],  C[row][col] = v,  act[row][col] = act_kind(v) + residual[row][col]
-// (C and residual may be NULL) and the line words of act.
+// (C and residual may be NULL); no line words: they cost this store what a
+// max pass over its output costs, and a row split needs none.
 struct Epilogue {
     const float *bias;
     const float *mask;
@@ -541,14 +542,6 @@ __device__ void exact_tiles(const float *__restrict__ A, bool a_col, const float
                 act_values(ep.act_kind, o);
                 if (ep.residual) o[0] = __fadd_rn(o[0], __ldg(ep.residual + idx));
                 ep.act[idx] = o[0];
-                if (ep.out_lines) {
-                    const uint32_t m = finite_bits(o[0]);
-                    if (m) {
-                        atomicMax(ep.out_lines + i, m);
-                        atomicMax(ep.out_lines + ep.out_rows + j, m);
-                    }
-                    if ((__float_as_uint(o[0]) & 0x7F800000u) == 0x7F800000u) atomicOr(ep.out_flag, 1u);
-                }
                 continue;
             }
             if (ep.mask_bits)
@@ -935,70 +928,115 @@ gemm_3xtf32_kernel(const __grid_constant__ CUtensorMap tAh, const __grid_constan
             // when act is written; 0 outside C), from which the line maxima are
             // taken.
             if constexpr (ACT) {
-                // The accumulators are a row a lane; the rest of the work is done a
-                // column a lane, 32 columns at a time through the warp's own shared
-                // memory, so that every load and store is a run of 128 bytes
-                // whatever N's alignment (a row a lane: [8192,4096]x[4096,4096] gelu
-                // with a residual 860 us, [4099,1000]x[1000,2050] 260 us).  The next
-                // eight rows' residuals are loaded while eight are worked on.
-                float *const stage = reinterpret_cast<float *>(smem + STAGES * Q::STAGE_BYTES + 256) + ew * (32 * 33);
+                // The accumulators are a row a lane.  32 columns at a time they go
+                // through the warp's own shared memory (rows of eight 16-byte slots,
+                // slot i of row r at i ^ (r & 7): no bank conflicts either way) and
+                // come back as eight lanes a row, so that loads and stores are whole
+                // 128-byte runs: 16 bytes a lane where everything is 16-byte aligned,
+                // else 4 and a row a time.  Eight values of a lane are worked on
+                // together, the residuals of the next eight on their way.
+                float4 *const stage = reinterpret_cast<float4 *>(smem + STAGES * Q::STAGE_BYTES + 256) + ew * 256;
                 const int row0 = mt * Q::TM + (int)crank * BM + q * 32;
                 const int rows = min(32, M - row0);  // of the warp's 32; may be below 1
-                uint32_t rtop = 0;
-                bool nonfinite = false;
+                const size_t first = (size_t)row0 * (size_t)N;
 #pragma unroll
                 for (int g = 0; g < Q::COLS_PER_WARP / 32; g++) {
-                    const int col = col0 + g * 32 + lane;
                     __syncwarp();  // the chunk before has been read
 #pragma unroll
-                    for (int j = 0; j < 32; j++) stage[lane * 33 + j] = acc[g * 32 + j];
+                    for (int j = 0; j < 8; j++)
+                        stage[lane * 8 + (j ^ (lane & 7))] = make_float4(acc[g * 32 + 4 * j], acc[g * 32 + 4 * j + 1],
+                                                                        acc[g * 32 + 4 * j + 2], acc[g * 32 + 4 * j + 3]);
                     __syncwarp();
-                    const bool col_ok = col < N;
-                    const float b = ep.bias && col_ok ? __ldg(ep.bias + col) : 0.0f;
-                    const size_t base = (size_t)row0 * (size_t)N + col;
-                    uint32_t ctop = 0;
-                    float res[8];
-                    auto residuals = [&](int r0) {
+                    const int c0 = col0 + g * 32;
+                    if (vec_store) {  // N % 4 == 0
+                        const int sub = lane >> 3, slot = lane & 7, col = c0 + 4 * slot;
+                        const bool col_ok = col < N;
+                        float4 b = make_float4(0.0f, 0.0f, 0.0f, 0.0f), res[2];
+                        if (ep.bias && col_ok) b = __ldg(reinterpret_cast<const float4 *>(ep.bias + col));
+                        const size_t base = first + col;
+                        auto residuals = [&](int r0) {
 #pragma unroll
-                        for (int i = 0; i < 8; i++)
-                            res[i] = col_ok && r0 + i < rows ? __ldg(ep.residual + base + (size_t)(r0 + i) * N) : 0.0f;
-                    };
-                    if (ep.residual) residuals(0);
+                            for (int i = 0; i < 2; i++) {
+                                const int r = r0 + 4 * i + sub;
+                                res[i] = col_ok && r < rows
+                                             ? __ldg(reinterpret_cast<const float4 *>(ep.residual + base + (size_t)r * N))
+                                             : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                            }
+                        };
+                        if (ep.residual) residuals(0);
 #pragma unroll 1
-                    for (int r0 = 0; r0 < rows; r0 += 8) {
-                        float x[8], add[8];
+                        for (int r0 = 0; r0 < rows; r0 += 8) {  // two rows of each lane
+                            float x[8];
+                            float4 add[2] = {res[0], res[1]};
 #pragma unroll
-                        for (int i = 0; i < 8; i++) {
-                            add[i] = res[i];
-                            x[i] = stage[(r0 + i) * 33 + lane];
-                            if (ep.bias) x[i] = __fadd_rn(x[i], b);
+                            for (int i = 0; i < 2; i++) {
+                                const int r = r0 + 4 * i + sub;
+                                const float4 v = stage[r * 8 + (slot ^ (r & 7))];
+                                x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
+                                if (ep.bias) {
+                                    x[4 * i] = __fadd_rn(v.x, b.x), x[4 * i + 1] = __fadd_rn(v.y, b.y);
+                                    x[4 * i + 2] = __fadd_rn(v.z, b.z), x[4 * i + 3] = __fadd_rn(v.w, b.w);
+                                }
+                            }
+                            if (ep.residual && r0 + 8 < rows) residuals(r0 + 8);
+                            auto put = [&](float *to) {
+#pragma unroll
+                                for (int i = 0; i < 2; i++) {
+                                    const int r = r0 + 4 * i + sub;
+                                    if (col_ok && r < rows)
+                                        *reinterpret_cast<float4 *>(to + base + (size_t)r * N) =
+                                            make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+                                }
+                            };
+                            if (Cb) put(Cb);
+                            act_values(ep.act_kind, x);
+                            if (ep.residual) {
+#pragma unroll
+                                for (int i = 0; i < 2; i++) {
+                                    x[4 * i] = __fadd_rn(x[4 * i], add[i].x);
+                                    x[4 * i + 1] = __fadd_rn(x[4 * i + 1], add[i].y);
+                                    x[4 * i + 2] = __fadd_rn(x[4 * i + 2], add[i].z);
+                                    x[4 * i + 3] = __fadd_rn(x[4 * i + 3], add[i].w);
+                                }
+                            }
+                            put(ep.act);
                         }
-                        if (ep.residual && r0 + 8 < rows) residuals(r0 + 8);
-                        if (Cb) {
+                    } else {
+                        const int col = c0 + lane;
+                        const bool col_ok = col < N;
+                        const float b = ep.bias && col_ok ? __ldg(ep.bias + col) : 0.0f;
+                        const size_t base = first + col;
+                        float res[8];
+                        auto residuals = [&](int r0) {
 #pragma unroll
                             for (int i = 0; i < 8; i++)
-                                if (col_ok && r0 + i < rows) Cb[base + (size_t)(r0 + i) * N] = x[i];
-                        }
-                        act_values(ep.act_kind, x);
+                                res[i] = col_ok && r0 + i < rows ? __ldg(ep.residual + base + (size_t)(r0 + i) * N) : 0.0f;
+                        };
+                        if (ep.residual) residuals(0);
+#pragma unroll 1
+                        for (int r0 = 0; r0 < rows; r0 += 8) {
+                            float x[8], add[8];
 #pragma unroll
-                        for (int i = 0; i < 8; i++) {
-                            const bool in = col_ok && r0 + i < rows;
-                            if (ep.residual) x[i] = __fadd_rn(x[i], add[i]);
-                            if (in) ep.act[base + (size_t)(r0 + i) * N] = x[i];
-                            if (ep.out_lines) {
-                                nonfinite |= in && (__float_as_uint(x[i]) & 0x7F800000u) == 0x7F800000u;
-                                const uint32_t m = in ? finite_bits(x[i]) : 0u;
-                                ctop = max(ctop, m);
-                                const uint32_t rm = __reduce_max_sync(0xffffffffu, m);
-                                if (lane == r0 + i) rtop = max(rtop, rm);
+                            for (int i = 0; i < 8; i++) {
+                                add[i] = res[i];
+                                x[i] = reinterpret_cast<const float *>(stage + (r0 + i) * 8 + ((lane >> 2) ^ ((r0 + i) & 7)))[lane & 3];
+                                if (ep.bias) x[i] = __fadd_rn(x[i], b);
                             }
+                            if (ep.residual && r0 + 8 < rows) residuals(r0 + 8);
+                            auto put = [&](float *to) {
+#pragma unroll
+                                for (int i = 0; i < 8; i++)
+                                    if (col_ok && r0 + i < rows) to[base + (size_t)(r0 + i) * N] = x[i];
+                            };
+                            if (Cb) put(Cb);
+                            act_values(ep.act_kind, x);
+                            if (ep.residual) {
+#pragma unroll
+                                for (int i = 0; i < 8; i++) x[i] = __fadd_rn(x[i], add[i]);
+                            }
+                            put(ep.act);
                         }
                     }
-                    if (ep.out_lines && col_ok && ctop) atomicMax(ep.out_lines + ep.out_rows + col, ctop);
-                }
-                if (ep.out_lines) {
-                    if (__any_sync(0xffffffffu, nonfinite) && lane == 0) atomicOr(ep.out_flag, 1u);
-                    if (row_ok && rtop) atomicMax(ep.out_lines + row, rtop);
                 }
                 continue;
             } else if (vec_full) {
@@ -2123,12 +2161,10 @@ static int gemm_presplit_ws(const float *ah, const float *al, const float *bh, c
 // y = act(A . B + bias) + residual from A's row-line split and B's transposed
 // split (both K-major); z, unless NULL, the pre-activation.
 int tc_gemm_act(const float *ah, const float *al, const float *bh, const float *bl, int64_t M, int64_t K, int64_t N,
-                const float *bias, int act, const float *residual, float *z, float *y, uint32_t *out_lines,
-                cudaStream_t s) {
+                const float *bias, int act, const float *residual, float *z, float *y, cudaStream_t s) {
     J4C_REQUIRE(aligned16(ah) && aligned16(al) && aligned16(bh) && aligned16(bl),
                 "dot: split operands must be 16-byte aligned");
-    const tc::Epilogue ep{bias,    nullptr, y, out_lines, (int)M, out_lines ? out_lines + M + N : nullptr,
-                          nullptr, nullptr, 0, act,       residual};
+    const tc::Epilogue ep{bias, nullptr, y, nullptr, (int)M, nullptr, nullptr, nullptr, 0, act, residual};
     static const bool pair = [] {
         const char *v = getenv("J4C_GEMM_PAIR");
         return !(v && v[0] == '0');

@@ -240,7 +240,6 @@ class _Dense(FfiMeta):
         bp = bias._t.data_ptr() if bias is not None else None
         rp = residual._t.data_ptr() if residual is not None else None
         zp = z.data_ptr() if z is not None else None
-        lines = None
         if f32 and (M <= FEW_ROWS or _small(M, K, N)):
             call("j4c_dot_act", t.data_ptr(), w._t.data_ptr(), M, K, N, 0, 0, bp, self.act, rp, zp, y.data_ptr(), stream)
         elif f32:
@@ -248,9 +247,8 @@ class _Dense(FfiMeta):
                 _make_splits(x2, ["r", "t" if K < N else "c"])
                 _make_splits(w, ["t", "r"])
             (xh, xl), (wh, wl) = _split_of(x2, "r"), _split_of(w, "t")
-            lines = torch.empty(M + N + 1, dtype=torch.int32, device=t.device)
             call("j4c_dot_split_act", xh.data_ptr(), xl.data_ptr(), wh.data_ptr(), wl.data_ptr(), M, K, N, bp, self.act,
-                 rp, zp, y.data_ptr(), lines.data_ptr(), stream)
+                 rp, zp, y.data_ptr(), stream)
         else:
             c = _product(x2, w, False, False, dev)._t  # FLOAT64: the product, then the rest in place or beside it
             if keep_z:
@@ -258,10 +256,7 @@ class _Dense(FfiMeta):
             else:
                 y = c
             call("j4c_dense_finish", dt.ordinal, c.data_ptr(), M, N, bp, self.act, rp, y.data_ptr(), stream)
-        out = ConcreteNDArray._wrap(y, out_shape, dt, dev)
-        if lines is not None and len(out_shape) == 2:
-            out._lines = lines
-        return out, ((x2, z) if keep else None)
+        return ConcreteNDArray._wrap(y, out_shape, dt, dev), ((x2, z) if keep else None)
 
     def vjp(self, inputs, out, saved, g, wanted):
         x, w = inputs[0], inputs[1]

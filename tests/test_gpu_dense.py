@@ -181,7 +181,7 @@ def test_other_gemm_variants(env):
     import subprocess
     import sys
     r = subprocess.run([sys.executable, "-m", "pytest", "-q", "-x", "tests/test_gpu_dense.py", "-k",
-                        "tensor_core or line_words or non_finite or border"], env={**os.environ, **env},
+                        "tensor_core or line_words or non_finite or border or unaligned"], env={**os.environ, **env},
                        capture_output=True, text=True, timeout=600,
                        cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
     assert r.returncode == 0, r.stdout[-3000:] + r.stderr[-2000:]
@@ -227,24 +227,6 @@ def test_non_finite_values(J, monkeypatch, small):
     bad = np.isnan(z)
     assert np.array_equal(np.isnan(y), bad) and bad.any()
     np.testing.assert_allclose(y[~bad], (1 / (1 + np.exp(-z)) + res)[~bad], rtol=1e-5, atol=1e-5)
-
-
-def test_line_words_of_the_output(J, monkeypatch):
-    """What a later product's split takes instead of a max pass, NaN/Inf flag included."""
-    import torch
-    from jax4j_b200 import _lib, layers
-    monkeypatch.setattr(layers, "SMALL_PRODUCT", 0)
-    for special in (False, True):
-        x, w, b, res, _ = make(7, (513, 1024), 515)
-        if special:
-            res[5, 6] = np.inf
-        for name in ("silu", "none"):
-            out = J.Nn.dense(arr(J, x), arr(J, w), arr(J, b), name, arr(J, res))
-            assert out._lines is not None
-            lines = torch.empty(513 + 515 + 1, dtype=torch.int32, device="cuda")
-            _lib.call("j4c_split_lines", out.data_ptr(), 513, 515, lines.data_ptr(), out._stream())
-            np.testing.assert_array_equal(out._lines.cpu().numpy()[:-1], lines.cpu().numpy()[:-1])
-            assert bool(out._lines[-1].item()) == bool(lines[-1].item()) == special
 
 
 def test_gradient_line_words(J):

@@ -72,9 +72,9 @@ def test_dense_c_entries_refuse_bad_arguments():
     told(L.j4c_dot_act(fake, None, 1, 2, 3, 0, 0, None, 0, None, None, fake, None), "NULL")
     told(L.j4c_dot_act(fake, fake, 1, 2, 3, 0, 0, None, 0, None, None, None, None), "NULL")
     told(L.j4c_dot_act(fake, fake, 1 << 33, 2, 3, 0, 0, None, 0, None, None, fake, None), "too many", _lib.E_UNSUPPORTED)
-    told(L.j4c_dot_split_act(fake, fake, fake, fake, 2, 0, 3, None, 0, None, None, fake, None, None), "K = 0")
-    told(L.j4c_dot_split_act(fake, None, fake, fake, 2, 4, 3, None, 0, None, None, fake, None, None), "NULL")
-    told(L.j4c_dot_split_act(fake, fake, fake, fake, 2, 4, 3, None, -1, None, None, fake, None, None), "activation")
+    told(L.j4c_dot_split_act(fake, fake, fake, fake, 2, 0, 3, None, 0, None, None, fake, None), "K = 0")
+    told(L.j4c_dot_split_act(fake, None, fake, fake, 2, 4, 3, None, 0, None, None, fake, None), "NULL")
+    told(L.j4c_dot_split_act(fake, fake, fake, fake, 2, 4, 3, None, -1, None, None, fake, None), "activation")
     told(L.j4c_dense_finish(2, fake, 2, 3, None, 0, None, fake, None), "FLOAT32 or FLOAT64")
     told(L.j4c_dense_finish(1, fake, 2, 3, None, 0, None, None, None), "NULL")
     told(L.j4c_dense_grad(0, 2, 3, fake, None, 3, 0, fake, None, None, None, 0, None), "NULL")
