@@ -144,9 +144,9 @@ struct Cfg {
     static constexpr int TMEM_COLS = 2 * BN;  // two partial-sum buffers
     static constexpr int COLS_PER_WARP = BN / 2;  // each epilogue warp owns half the columns
     static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 256;
-    // with an activation epilogue, a 32 x 32 staging area of every epilogue warp
-    static constexpr int ACT_SMEM_BYTES = SMEM_BYTES + kEpiWarps * 32 * 32 * 4;
-    static_assert(ACT_SMEM_BYTES <= 232448 || STAGES * STAGE_BYTES > 196608, "shared memory budget");
+    // with an activation epilogue, two 32 x 32 areas of every epilogue warp: the
+    // results on their way to the store, and the residuals
+    static constexpr int ACT_SMEM_BYTES = SMEM_BYTES + 2 * kEpiWarps * 32 * 32 * 4;
     static_assert(TMEM_COLS == 256 || TMEM_COLS == 512, "TMEM allocation must be a power of 2");
     static_assert(SMEM_BYTES <= 232448, "shared memory budget");
 };
@@ -813,17 +813,41 @@ gemm_3xtf32_kernel(const __grid_constant__ CUtensorMap tAh, const __grid_constan
             float *const Cb = C ? C + boff : nullptr;  // NULL: only the relu output is stored
             const float *const mask_b = ep.mask ? ep.mask + boff : nullptr;
             float *const act_b = ep.act ? ep.act + boff : nullptr;
-            if constexpr (ACT) {
-                // the residual's lines to L2 while the MMAs of the tile run
-                const int row = mt * Q::TM + (int)crank * BM + q * 32 + lane;
-                if (ep.residual && row < M) {
+            // ACT: the residuals of the warp's first 32 columns come to its own shared
+            // memory while the MMAs of the tile run, those of the next 32 as these are
+            // used up; a lane copies and reads its own slots, a place in the chunk each.
+            const int row0 = mt * Q::TM + (int)crank * BM + q * 32;
+            const int rows = min(32, M - row0);  // of the warp's 32; may be below 1
+            float4 *const stage = reinterpret_cast<float4 *>(smem + STAGES * Q::STAGE_BYTES + 256) + ew * 256;
+            float4 *const kept = stage + kEpiWarps * 256;
+            // rows r0..r0+7 of the chunk that starts at column c0
+            auto fetch_residual = [&](int r0, int c0) {
+                if constexpr (ACT) {
+                    if (vec_store) {
+                        const int slot = lane & 7, col = c0 + 4 * slot;
 #pragma unroll
-                    for (int g = 0; g < Q::COLS_PER_WARP / 32; g++) {
-                        const int col = nt * BN + cbase + g * 32;
-                        if (col < N)
-                            asm volatile("prefetch.global.L2 [%0];" ::"l"(ep.residual + (size_t)row * N + col));
+                        for (int i = 0; i < 2; i++) {
+                            const int r = r0 + 4 * i + (lane >> 3);
+                            if (col < N && r < rows)
+                                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(kept + r * 8 + slot)),
+                                             "l"(ep.residual + (size_t)(row0 + r) * N + col)
+                                             : "memory");
+                        }
+                    } else if (c0 + lane < N) {
+#pragma unroll
+                        for (int i = 0; i < 8; i++)
+                            if (r0 + i < rows)
+                                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(
+                                                 smem_u32(reinterpret_cast<float *>(kept + (r0 + i) * 8) + lane)),
+                                             "l"(ep.residual + (size_t)(row0 + r0 + i) * N + c0 + lane)
+                                             : "memory");
                     }
+                    asm volatile("cp.async.commit_group;" ::: "memory");
                 }
+            };
+            if (ACT && ep.residual) {
+#pragma unroll 1
+                for (int r0 = 0; r0 < 32; r0 += 8) fetch_residual(r0, nt * BN + cbase);
             }
             float acc[Q::COLS_PER_WARP];
 #pragma unroll
@@ -868,7 +892,11 @@ gemm_3xtf32_kernel(const __grid_constant__ CUtensorMap tAh, const __grid_constan
                 int before = 0;
                 if (lane == 0) before = atomicAdd(arrivals + (tix * NPAIR + crank) * kEpiWarps + ew, 1);
                 before = __shfl_sync(0xffffffffu, before, 0);
-                if (before != splits - 1) continue;  // a later part settles the region
+                if (before != splits - 1) {  // a later part settles the region
+                    // the residuals' copies end before the next unit's start into the same place
+                    if constexpr (ACT) asm volatile("cp.async.wait_group 0;" ::: "memory");
+                    continue;
+                }
                 __threadfence();
                 // every partial (this part's too) is read back through L2
                 const float *rp = part + ((tix * splits * NPAIR + crank) * kEpiWarps + ew) * (size_t)RF + lane;
@@ -934,10 +962,9 @@ gemm_3xtf32_kernel(const __grid_constant__ CUtensorMap tAh, const __grid_constan
                 // come back as eight lanes a row, so that loads and stores are whole
                 // 128-byte runs: 16 bytes a lane where everything is 16-byte aligned,
                 // else 4 and a row a time.  Eight values of a lane are worked on
-                // together, the residuals of the next eight on their way.
-                float4 *const stage = reinterpret_cast<float4 *>(smem + STAGES * Q::STAGE_BYTES + 256) + ew * 256;
-                const int row0 = mt * Q::TM + (int)crank * BM + q * 32;
-                const int rows = min(32, M - row0);  // of the warp's 32; may be below 1
+                // together.  ([8192,4096]x[4096,4096]: 570 us, 600 with gelu and a
+                // residual, 613 with the pre-activation kept too; the plain product,
+                // whose store is a row a lane, 587.)
                 const size_t first = (size_t)row0 * (size_t)N;
 #pragma unroll
                 for (int g = 0; g < Q::COLS_PER_WARP / 32; g++) {
@@ -951,23 +978,12 @@ gemm_3xtf32_kernel(const __grid_constant__ CUtensorMap tAh, const __grid_constan
                     if (vec_store) {  // N % 4 == 0
                         const int sub = lane >> 3, slot = lane & 7, col = c0 + 4 * slot;
                         const bool col_ok = col < N;
-                        float4 b = make_float4(0.0f, 0.0f, 0.0f, 0.0f), res[2];
+                        float4 b = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                         if (ep.bias && col_ok) b = __ldg(reinterpret_cast<const float4 *>(ep.bias + col));
                         const size_t base = first + col;
-                        auto residuals = [&](int r0) {
-#pragma unroll
-                            for (int i = 0; i < 2; i++) {
-                                const int r = r0 + 4 * i + sub;
-                                res[i] = col_ok && r < rows
-                                             ? __ldg(reinterpret_cast<const float4 *>(ep.residual + base + (size_t)r * N))
-                                             : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                            }
-                        };
-                        if (ep.residual) residuals(0);
 #pragma unroll 1
-                        for (int r0 = 0; r0 < rows; r0 += 8) {  // two rows of each lane
+                        for (int r0 = 0; r0 < 32; r0 += 8) {  // two rows of each lane
                             float x[8];
-                            float4 add[2] = {res[0], res[1]};
 #pragma unroll
                             for (int i = 0; i < 2; i++) {
                                 const int r = r0 + 4 * i + sub;
@@ -978,7 +994,6 @@ gemm_3xtf32_kernel(const __grid_constant__ CUtensorMap tAh, const __grid_constan
                                     x[4 * i + 2] = __fadd_rn(v.z, b.z), x[4 * i + 3] = __fadd_rn(v.w, b.w);
                                 }
                             }
-                            if (ep.residual && r0 + 8 < rows) residuals(r0 + 8);
                             auto put = [&](float *to) {
 #pragma unroll
                                 for (int i = 0; i < 2; i++) {
@@ -991,38 +1006,32 @@ gemm_3xtf32_kernel(const __grid_constant__ CUtensorMap tAh, const __grid_constan
                             if (Cb) put(Cb);
                             act_values(ep.act_kind, x);
                             if (ep.residual) {
+                                asm volatile("cp.async.wait_group 3;" ::: "memory");  // four fetches a chunk: the oldest
 #pragma unroll
                                 for (int i = 0; i < 2; i++) {
-                                    x[4 * i] = __fadd_rn(x[4 * i], add[i].x);
-                                    x[4 * i + 1] = __fadd_rn(x[4 * i + 1], add[i].y);
-                                    x[4 * i + 2] = __fadd_rn(x[4 * i + 2], add[i].z);
-                                    x[4 * i + 3] = __fadd_rn(x[4 * i + 3], add[i].w);
+                                    const float4 add = kept[(r0 + 4 * i + sub) * 8 + slot];
+                                    x[4 * i] = __fadd_rn(x[4 * i], add.x);
+                                    x[4 * i + 1] = __fadd_rn(x[4 * i + 1], add.y);
+                                    x[4 * i + 2] = __fadd_rn(x[4 * i + 2], add.z);
+                                    x[4 * i + 3] = __fadd_rn(x[4 * i + 3], add.w);
                                 }
                             }
                             put(ep.act);
+                            if (ep.residual) fetch_residual(r0, g < Q::COLS_PER_WARP / 32 - 1 ? c0 + 32 : N);
                         }
                     } else {
                         const int col = c0 + lane;
                         const bool col_ok = col < N;
                         const float b = ep.bias && col_ok ? __ldg(ep.bias + col) : 0.0f;
                         const size_t base = first + col;
-                        float res[8];
-                        auto residuals = [&](int r0) {
-#pragma unroll
-                            for (int i = 0; i < 8; i++)
-                                res[i] = col_ok && r0 + i < rows ? __ldg(ep.residual + base + (size_t)(r0 + i) * N) : 0.0f;
-                        };
-                        if (ep.residual) residuals(0);
 #pragma unroll 1
-                        for (int r0 = 0; r0 < rows; r0 += 8) {
-                            float x[8], add[8];
+                        for (int r0 = 0; r0 < 32; r0 += 8) {
+                            float x[8];
 #pragma unroll
                             for (int i = 0; i < 8; i++) {
-                                add[i] = res[i];
                                 x[i] = reinterpret_cast<const float *>(stage + (r0 + i) * 8 + ((lane >> 2) ^ ((r0 + i) & 7)))[lane & 3];
                                 if (ep.bias) x[i] = __fadd_rn(x[i], b);
                             }
-                            if (ep.residual && r0 + 8 < rows) residuals(r0 + 8);
                             auto put = [&](float *to) {
 #pragma unroll
                                 for (int i = 0; i < 8; i++)
@@ -1031,10 +1040,13 @@ gemm_3xtf32_kernel(const __grid_constant__ CUtensorMap tAh, const __grid_constan
                             if (Cb) put(Cb);
                             act_values(ep.act_kind, x);
                             if (ep.residual) {
+                                asm volatile("cp.async.wait_group 3;" ::: "memory");
 #pragma unroll
-                                for (int i = 0; i < 8; i++) x[i] = __fadd_rn(x[i], add[i]);
+                                for (int i = 0; i < 8; i++)
+                                    x[i] = __fadd_rn(x[i], reinterpret_cast<const float *>(kept + (r0 + i) * 8)[lane]);
                             }
                             put(ep.act);
+                            if (ep.residual) fetch_residual(r0, g < Q::COLS_PER_WARP / 32 - 1 ? c0 + 32 : N);
                         }
                     }
                 }
@@ -1152,6 +1164,7 @@ gemm_3xtf32_kernel(const __grid_constant__ CUtensorMap tAh, const __grid_constan
             }
             if (ep.out_lines && row_ok && rmax) atomicMax(ep.out_lines + (store_t ? ep.out_rows + row : row), rmax);
         }
+        if constexpr (ACT) asm volatile("cp.async.wait_group 0;" ::: "memory");  // where a wait ran out
     }
 
     tc_fence_before();
@@ -1833,6 +1846,7 @@ static int launch_gemm(const float *ah, const float *al, const float *bh, const 
     using Q = Cfg<BN, STAGES, BK, F16, PAIR>;
     auto kernel = gemm_3xtf32_kernel<BN, STAGES, BK, A_MN, B_MN, F16, PAIR, ACT>;
     constexpr int smem_bytes = ACT ? Q::ACT_SMEM_BYTES : Q::SMEM_BYTES;
+    static_assert(smem_bytes <= 232448, "shared memory budget");
     static std::mutex mu;
     static std::vector<char> configured;
     int dev = 0;
@@ -2169,14 +2183,14 @@ int tc_gemm_act(const float *ah, const float *al, const float *bh, const float *
         const char *v = getenv("J4C_GEMM_PAIR");
         return !(v && v[0] == '0');
     }();
-    // the variants of gemm_presplit_ws
+    // the variants of gemm_presplit_ws, with a stage less for the epilogue's areas
     if (tc::split_fp16() && pair && M >= 2 * tc::BM)
-        return tc::launch_gemm<256, 6, 16, false, false, true, true, true>(ah, al, bh, bl, z, M, N, K, false, ep, 1, false,
+        return tc::launch_gemm<256, 5, 16, false, false, true, true, true>(ah, al, bh, bl, z, M, N, K, false, ep, 1, false,
                                                                            false, nullptr, s);
     if (tc::split_fp16())
-        return tc::launch_gemm<256, 4, 16, false, false, true, false, true>(ah, al, bh, bl, z, M, N, K, false, ep, 1, false,
+        return tc::launch_gemm<256, 3, 16, false, false, true, false, true>(ah, al, bh, bl, z, M, N, K, false, ep, 1, false,
                                                                             false, nullptr, s);
-    return tc::launch_gemm<256, 4, 16, false, false, false, false, true>(ah, al, bh, bl, z, M, N, K, false, ep, 1, false,
+    return tc::launch_gemm<256, 3, 16, false, false, false, false, true>(ah, al, bh, bl, z, M, N, K, false, ep, 1, false,
                                                                          false, nullptr, s);
 }
 
