@@ -359,6 +359,9 @@ J4C_API int j4c_split_f32_both(const float *x, int64_t rows, int64_t cols, float
  * leave them; it replaces the split's own max pass. */
 J4C_API int j4c_split_f32_ex(const float *x, int64_t rows, int64_t cols, float *hi, float *lo, float *hi_c,
                              float *lo_c, float *hi_t, float *lo_t, const uint32_t *lines, j4c_stream stream);
+/* j4c_split_lines and then j4c_split_f32_ex with its lines. */
+J4C_API int j4c_split_f32_lines(const float *x, int64_t rows, int64_t cols, float *hi, float *lo, float *hi_c,
+                                float *lo_c, float *hi_t, float *lo_t, uint32_t *lines, j4c_stream stream);
 /* lines [rows + cols + 1] (device): the line maxima of x (rows, then
  * columns) and its NaN/Inf flag in one pass, for several later
  * j4c_split_f32_ex calls. */

@@ -126,6 +126,9 @@ public final class J4C {
     static final MethodHandle SPLIT_F32_EX = h("j4c_split_f32_ex", FunctionDescriptor.of(
         JAVA_INT, ADDRESS, JAVA_LONG, JAVA_LONG, ADDRESS, ADDRESS, ADDRESS, ADDRESS, ADDRESS, ADDRESS, ADDRESS,
         ADDRESS));
+    static final MethodHandle SPLIT_F32_LINES = h("j4c_split_f32_lines", FunctionDescriptor.of(
+        JAVA_INT, ADDRESS, JAVA_LONG, JAVA_LONG, ADDRESS, ADDRESS, ADDRESS, ADDRESS, ADDRESS, ADDRESS, ADDRESS,
+        ADDRESS));
     static final MethodHandle SPLIT_LINES = h("j4c_split_lines", FunctionDescriptor.of(
         JAVA_INT, ADDRESS, JAVA_LONG, JAVA_LONG, ADDRESS, ADDRESS));
     static final MethodHandle SGD_UPDATE_LINES = h("j4c_sgd_update_lines", FunctionDescriptor.of(

@@ -84,6 +84,7 @@ SIGNATURES = {
     "j4c_dot_split_ep": [P, P, P, P, P, I64, I64, I64, I32, I32, P, P, P, P],
     "j4c_split_f32_both": [P, I64, I64, P, P, P, P, P],
     "j4c_split_f32_ex": [P, I64, I64, P, P, P, P, P, P, P, P],
+    "j4c_split_f32_lines": [P, I64, I64, P, P, P, P, P, P, P, P],
     "j4c_split_f32_cols": [P, I64, I64, P, P, P],
     "j4c_split_lines": [P, I64, I64, P, P],
     "j4c_split_floats": [I64, I64],

@@ -11,6 +11,7 @@ GPU stream.  There is no host compute path.
 from __future__ import annotations
 
 import enum
+import functools
 import threading
 from typing import Optional, Sequence
 
@@ -786,15 +787,10 @@ def _kind(kind: str) -> str:
     return kind
 
 
-def _split_lines(x: "ConcreteNDArray"):
-    """x's line maxima (rows then columns), from the GEMM that wrote x or one
-    max pass, kept on the array for every split of it."""
-    if x._lines is None:
-        rows, cols = x._shape.dimensions()
-        lines = torch.empty(rows + cols + 1, dtype=torch.int32, device=x._t.device)
-        call("j4c_split_lines", x._t.data_ptr(), rows, cols, lines.data_ptr(), x._stream())
-        x._lines = lines
-    return x._lines
+@functools.lru_cache(maxsize=4096)
+def _split_floats(rows: int, cols: int) -> int:
+    """j4c_split_floats, rounded up to 256 bytes."""
+    return -(-int(_lib.lib().j4c_split_floats(rows, cols)) // 64) * 64
 
 
 def _make_splits(x: "ConcreteNDArray", kinds) -> None:
@@ -807,20 +803,29 @@ def _make_splits(x: "ConcreteNDArray", kinds) -> None:
         _make_splits(x, ["t"])
         kinds.remove("t")
     rows, cols = x._shape.dimensions()
-    L = _lib.lib()
-    out = {}
+    # every hi and lo array, and the line words where they are computed here,
+    # from one allocation
+    sizes = []
     for k in kinds:
-        n = L.j4c_split_floats(cols, rows) if k == "t" else L.j4c_split_floats(rows, cols)
-        out[k] = (torch.empty(n, dtype=torch.float32, device=x._t.device),
-                  torch.empty(n, dtype=torch.float32, device=x._t.device))
-    ptrs = []
-    for k in ("r", "c", "t"):
-        ptrs += [out[k][0].data_ptr(), out[k][1].data_ptr()] if k in out else [None, None]
+        n = _split_floats(cols, rows) if k == "t" else _split_floats(rows, cols)
+        sizes += (n, n)
     # row lines alone need no max pass of their own: the split takes each row's
     # maximum on the way (j4c_split_f32_ex without lines)
-    lines = _split_lines(x) if x._lines is not None or kinds != ["r"] or cols > 8192 else None
-    call("j4c_split_f32_ex", x._t.data_ptr(), rows, cols, *ptrs,
-         lines.data_ptr() if lines is not None else None, x._stream())
+    new_lines = x._lines is None and (kinds != ["r"] or cols > 8192)
+    if new_lines:
+        sizes.append(-(-(rows + cols + 1) // 64) * 64)
+    parts = torch.split_with_sizes(torch.empty(sum(sizes), dtype=torch.float32, device=x._t.device), sizes)
+    out = {k: (parts[2 * i], parts[2 * i + 1]) for i, k in enumerate(kinds)}
+    ptrs = []
+    for k in ("r", "c", "t"):
+        ptrs += (out[k][0].data_ptr(), out[k][1].data_ptr()) if k in out else (None, None)
+    if new_lines:
+        lines = parts[-1].view(torch.int32)[:rows + cols + 1]
+        call("j4c_split_f32_lines", x._t.data_ptr(), rows, cols, *ptrs, lines.data_ptr(), x._stream())
+        x._lines = lines
+    else:
+        call("j4c_split_f32_ex", x._t.data_ptr(), rows, cols, *ptrs,
+             x._lines.data_ptr() if x._lines is not None else None, x._stream())
     if x._split is None:
         x._split = {}
     x._split.update(out)

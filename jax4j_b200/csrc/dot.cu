@@ -127,6 +127,13 @@ int j4c_split_f32_ex(const float *x, int64_t rows, int64_t cols, float *hi, floa
     return split_entry("j4c_split_f32_ex", x, rows, cols, hi, lo, hi_c, lo_c, hi_t, lo_t, lines, stream);
 }
 
+int j4c_split_f32_lines(const float *x, int64_t rows, int64_t cols, float *hi, float *lo, float *hi_c, float *lo_c,
+                        float *hi_t, float *lo_t, uint32_t *lines, j4c_stream stream) {
+    J4C_REQUIRE(lines, "j4c_split_f32_lines: NULL pointer");
+    if (int rc = j4c_split_lines(x, rows, cols, lines, stream)) return rc;
+    return split_entry("j4c_split_f32_lines", x, rows, cols, hi, lo, hi_c, lo_c, hi_t, lo_t, lines, stream);
+}
+
 int j4c_split_lines(const float *x, int64_t rows, int64_t cols, uint32_t *lines, j4c_stream stream) {
     J4C_REQUIRE(rows >= 0 && cols >= 0, "j4c_split_lines: negative extent");
     J4C_REQUIRE(lines && (x || rows == 0 || cols == 0), "j4c_split_lines: NULL pointer");
