@@ -185,4 +185,7 @@ def kernel_launches() -> int:
 
 
 def call(name: str, *args) -> None:
-    check(getattr(lib(), name)(*args), name)
+    L = _lib if _lib is not None else lib()
+    rc = getattr(L, name)(*args)
+    if rc != OK:
+        check(rc, name)

@@ -398,7 +398,7 @@ class ConcreteNDArray(NDArray):
             t = data
             if dtype is None:
                 dtype = _OF_TORCH.get(t.dtype) or _from_torch(t.dtype)
-            if t.dtype is not dtype.torch or not t.is_cuda or t.get_device() != device.ordinal():
+            if t.dtype is not dtype.torch or t.get_device() != device.ordinal():  # -1: not on a GPU
                 t = t.to(device=device.torch_device(), dtype=dtype.torch)
             if t.dim() != 1:
                 t = t.reshape(-1)

@@ -218,13 +218,37 @@ __device__ __forceinline__ void tile_product(const Product &p, int64_t tile_m, i
     for (int i = 0; i < 8; i++)
         *reinterpret_cast<float4 *>(&part[ty * 8 + i][tx * 4]) = make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
     cluster.sync();
-    // rank r finishes rows r, r + ranks, ... of the tile; shares in order
-    for (int e = tid; e < kTM / ranks * kTN; e += kTileThreads) {
-        const int m = e / kTN * ranks + rank, n = e % kTN;
-        if (m0 + m >= p.M || n0 + n >= p.N) continue;
-        float v = 0.0f;
-        for (int r = 0; r < ranks; r++) v += *cluster.map_shared_rank(&part[m][n], r);
-        finish(p, m0 + m, n0 + n, v);
+    // Rank r finishes rows r, r + ranks, ... of the tile: a thread every second
+    // of them in its column, eight at a time so that their residuals are on
+    // their way together.  Shares are added in order.
+    const int n = tid % kTN, mine = kTM / ranks;
+    if (n0 + n < p.N) {
+        const float bias = p.bias ? p.bias[n0 + n] : 0.0f;
+        for (int i0 = tid / kTN; i0 < mine; i0 += 16) {
+            float v[8], res[8];
+            int64_t at[8];
+            bool in[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int idx = i0 + 2 * i, m = idx * ranks + rank;
+                in[i] = idx < mine && m0 + m < p.M;
+                at[i] = (m0 + m) * p.N + n0 + n;
+                res[i] = p.residual && in[i] ? p.residual[at[i]] : 0.0f;
+                v[i] = 0.0f;
+                if (in[i])
+                    for (int r = 0; r < ranks; r++) v[i] += *cluster.map_shared_rank(&part[m][n], r);
+                if (p.bias) v[i] = __fadd_rn(v[i], bias);
+            }
+            if (p.z) {
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    if (in[i]) p.z[at[i]] = v[i];
+            }
+            act_values(p.act, v);
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (in[i]) p.y[at[i]] = p.residual ? __fadd_rn(v[i], res[i]) : v[i];
+        }
     }
     cluster.sync();
 }

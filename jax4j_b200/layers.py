@@ -9,6 +9,7 @@ jit, scan and checkpoint compose with it as with any other equation.
 """
 from __future__ import annotations
 
+import functools
 from typing import List, Optional
 
 import torch
@@ -31,10 +32,8 @@ def activation_code(name: Optional[str]) -> int:
 
 
 def _apply(meta: FfiMeta, inputs: List[NDArray], out_shape: Shape) -> NDArray:
-    """The layer on its arrays, or its equation under a trace."""
+    """The layer's equation under a trace."""
     tracer = Tracer.current()
-    if tracer is None:
-        return meta.forward(inputs, False)[0]
     in_vars = [to_var(x) for x in inputs]
     out = tracer.nextVar(out_shape, in_vars[0].dtype)
     tracer.addEquation(Equation(in_vars, [out], Primitive.FFI_CALL, meta))
@@ -44,8 +43,8 @@ def _apply(meta: FfiMeta, inputs: List[NDArray], out_shape: Shape) -> NDArray:
 def _device_of(inputs: List[ConcreteNDArray]):
     """The result's device, by the rules of elementwise operations
     (core/ConcreteNDArray.java:261-267)."""
-    dev = inputs[0].device()
-    for x in inputs[1:]:
+    dev = inputs[0]._device
+    for x in inputs:
         if x._device is not dev:
             first = ConcreteNDArray._wrap(inputs[0]._t, inputs[0]._shape, inputs[0]._dtype, dev)
             dev = first._check_devices(x)
@@ -53,10 +52,11 @@ def _device_of(inputs: List[ConcreteNDArray]):
 
 
 def _floating(what: str, first: NDArray, others) -> None:
-    if not first.dtype().is_floating():
-        raise IllegalArgumentException(f"{what} requires FLOAT32 or FLOAT64 operands, got {first.dtype()}")
+    dt = first.dtype()
+    if not dt.is_floating():
+        raise IllegalArgumentException(f"{what} requires FLOAT32 or FLOAT64 operands, got {dt}")
     for x in others:
-        if x is not None and x.dtype() != first.dtype():
+        if x is not None and x.dtype() is not dt:
             raise IllegalArgumentException(f"{what} requires operands of one floating dtype, got {first.dtype()} and "
                                            f"{x.dtype()} — use .astype() to convert.")
 
@@ -82,6 +82,8 @@ def group_norm(x: NDArray, groups: int, gamma: Optional[NDArray], beta: Optional
         raise IllegalArgumentException(f"groupNorm: eps is not negative, got {eps}")
     inputs = [x] + [p for p in (gamma, beta) if p is not None]
     meta = _GroupNorm(groups, gamma is not None, beta is not None, float(eps), act)
+    if Tracer.current() is None:
+        return meta.forward(inputs, False)[0]
     return _apply(meta, inputs, x.shape())
 
 
@@ -180,20 +182,27 @@ def _small(M: int, K: int, N: int) -> bool:
 
 def dense(x: NDArray, w: NDArray, bias: Optional[NDArray], activation: Optional[str],
           residual: Optional[NDArray]) -> NDArray:
-    xd, wd = x.shape().dimensions(), w.shape().dimensions()
+    xd, wd = x.shape()._d, w.shape()._d
     act = activation_code(activation)
     if len(xd) < 1 or len(wd) != 2:
         raise IllegalArgumentException(f"dense takes [..., K] and a weight [K, N], got {x.shape()} and {w.shape()}")
     if xd[-1] != wd[0]:
         raise IllegalArgumentException(f"dense: inner dimensions differ ({x.shape()} . {w.shape()})")
     _floating("dense", x, (w, bias, residual))
-    out = Shape(xd[:-1] + (wd[1],))
-    if bias is not None and bias.shape().dimensions() != (wd[1],):
-        raise IllegalArgumentException(f"dense: bias is {bias.shape()}, the outputs are [{wd[1]}]")
-    if residual is not None and residual.shape() != out:
-        raise IllegalArgumentException(f"dense: residual is {residual.shape()}, the output {out}")
-    inputs = [x, w] + [p for p in (bias, residual) if p is not None]
-    return _apply(_Dense(bias is not None, residual is not None, act), inputs, out)
+    out = xd[:-1] + wd[1:]
+    inputs = [x, w]
+    if bias is not None:
+        if bias.shape()._d != wd[1:]:
+            raise IllegalArgumentException(f"dense: bias is {bias.shape()}, the outputs are [{wd[1]}]")
+        inputs.append(bias)
+    if residual is not None:
+        if residual.shape()._d != out:
+            raise IllegalArgumentException(f"dense: residual is {residual.shape()}, the output {Shape(out)}")
+        inputs.append(residual)
+    meta = _dense_meta(bias is not None, residual is not None, act)
+    if Tracer.current() is None:
+        return meta.forward(inputs, False)[0]
+    return _apply(meta, inputs, Shape(out))
 
 
 def _product(a: ConcreteNDArray, b: ConcreteNDArray, trans_a: bool, trans_b: bool, dev) -> ConcreteNDArray:
@@ -316,3 +325,8 @@ class _Dense(FfiMeta):
         if not batched[0] or batched[1] or (self.has_bias and batched[2]) or (self.has_residual and not batched[-1]):
             raise UnsupportedOperationException("vmap of dense batches x, together with the residual")
         return self.forward(inputs, False)[0]
+
+
+@functools.lru_cache(maxsize=None)
+def _dense_meta(has_bias: bool, has_residual: bool, act: int) -> _Dense:
+    return _Dense(has_bias, has_residual, act)  # 24 of them, which hold nothing else
