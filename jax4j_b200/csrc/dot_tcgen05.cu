@@ -487,6 +487,7 @@ struct Epilogue {
     int bits_words;
     int act_kind;
     const float *residual;
+    int chunk_kb;  // with ACT: k-blocks of a promotion chunk
 };
 
 // The bits of |v| for finite v, else 0.
@@ -599,7 +600,8 @@ gemm_3xtf32_kernel(const __grid_constant__ CUtensorMap tAh, const __grid_constan
     constexpr int UMMA_K = Elt<F16>::UMMA_K;
     constexpr int NPAIR = PAIR ? 2 : 1;
     // end of chunk n of a unit that starts at k-block kb0 and ends at end
-    auto chunk_end = [](int kb0, int n, int end) { return min(end, kb0 + (n < 2 ? Q::CHUNK_KB : Q::CHUNK2_KB)); };
+    const int chunk1 = ACT ? ep.chunk_kb : Q::CHUNK_KB, chunk2 = ACT ? ep.chunk_kb : Q::CHUNK2_KB;
+    auto chunk_end = [chunk1, chunk2](int kb0, int n, int end) { return min(end, kb0 + (n < 2 ? chunk1 : chunk2)); };
     {
         // What the operands' splits say, the same for every thread: a split
         // must match its use (under 3xFP16 its lines are the rows of a
@@ -1575,8 +1577,7 @@ __global__ void __launch_bounds__(256) split16_kernel(const float *__restrict__ 
 // The row-line split alone, of an X whose maxima nobody has computed: WARPS
 // warps hold a row of up to 1024 WARPS columns in registers, so its maximum
 // and its split come from one read of X -- 8 B per element instead of the max
-// pass's 4 and the split's 8 ([8192, 4096]: 100 us for those two, see the
-// launch's figure).  The same bits as split16_kernel's.  hdr starts zeroed.
+// pass's 4 and the split's 8 ([8192, 4096]: 38 us, those two 100).  The same bits as split16_kernel's.  hdr starts zeroed.
 constexpr int kSplitRowCols = 8 * 1024;
 template <int WARPS>
 __global__ void __launch_bounds__(256) split16_rows_kernel(const float *__restrict__ src, int64_t rows, int64_t cols,
@@ -2153,7 +2154,7 @@ static int gemm_presplit_ws(const float *ah, const float *al, const float *bh, c
     J4C_REQUIRE(!act_bits || act, "dot: relu bits need the relu output");
     J4C_REQUIRE(!(mask_bits || act_bits) || batch == 1, "dot: mask bits of a batched product");
     const tc::Epilogue ep{bias,      mask,     act, out_lines, (int)M, out_lines ? out_lines + M + N : nullptr,
-                          mask_bits, act_bits, (int)ceil_div(N, 32), J4C_ACT_NONE, nullptr};
+                          mask_bits, act_bits, (int)ceil_div(N, 32), J4C_ACT_NONE, nullptr, 0};
     const bool ab = a_batched != 0, bb = b_batched != 0;
     // CTA pairs (256-row tiles, cta_group::2) for 3xFP16 products whose
     // stored rows (the kernel's M: N when C is stored transposed) fill them
@@ -2178,7 +2179,16 @@ int tc_gemm_act(const float *ah, const float *al, const float *bh, const float *
                 const float *bias, int act, const float *residual, float *z, float *y, cudaStream_t s) {
     J4C_REQUIRE(aligned16(ah) && aligned16(al) && aligned16(bh) && aligned16(bl),
                 "dot: split operands must be 16-byte aligned");
-    const tc::Epilogue ep{bias, nullptr, y, nullptr, (int)M, nullptr, nullptr, nullptr, 0, act, residual};
+    // Chunks of 128 K up to 2048, then 256 (a k-block holds 32 K under 3xFP16, 16
+    // under 3xTF32).  A chunk's truncation bias does not grow with K while the
+    // error of an FP32 sum does, so the longer chunk is held against the larger
+    // error: at K = 4096 the relative error is 9.3e-7, of a plain FP32 product
+    // 1.15e-6; at 2048 with chunks of 128 it is 4.8e-7 and 5.7 to 8.1e-7.
+    // Fewer chunks leave the epilogue's warps less to add: [8192,4096] .
+    // [4096,4096] gelu + residual 827 -> 806 us.
+    const int block = tc::split_fp16() ? 32 : 16;
+    const tc::Epilogue ep{bias, nullptr, y,   nullptr,  (int)M,
+                          nullptr, nullptr, nullptr, 0, act, residual, (K <= 2048 ? 128 : 256) / block};
     static const bool pair = [] {
         const char *v = getenv("J4C_GEMM_PAIR");
         return !(v && v[0] == '0');

@@ -166,10 +166,9 @@ class _GroupNorm(FfiMeta):
 # FLOAT32 products of at most this many multiply-adds run on the CUDA cores
 # straight from their arrays (j4c_dot_act); the tensor-core product first
 # splits both operands (five launches more), which larger ones win back: forward
-# and gradients of [1024,1024]x[1024,512] 161 against 188 us, of [1024,1024]x
-# [1024,1024] 260 against 204.
+# of [1024,1024]x[1024,512] 48 against 60 us, with gradients 163 against 169; of
+# [1024,1024]x[1024,1024] 89 against 60 and 264 against 168.
 SMALL_PRODUCT = 1 << 29
-
 
 # As many rows or fewer run there whatever the weight's size: they are bound by
 # reading it once, which the splits read, write and read again.
@@ -210,6 +209,15 @@ def _product(a: ConcreteNDArray, b: ConcreteNDArray, trans_a: bool, trans_b: boo
     if a._t.numel() and b._t.numel():
         return _dot_raw(a, b, trans_a, trans_b, dev)
     return ConcreteNDArray.full(Shape(a._shape[1 if trans_a else 0], b._shape[0 if trans_b else 1]), 0.0, a._dtype, dev)
+
+
+def _split_product(a, a_kind: str, b, b_kind: str, M: int, K: int, N: int, bias, act: int, residual, z, out: torch.Tensor,
+                   stream) -> None:
+    """out [M, N] = act(A . B^T + bias) + residual on the tensor cores, with A
+    [M, K] and B [N, K] the splits of a and b by rows of these kinds."""
+    (ah, al), (bh, bl) = _split_of(a, a_kind), _split_of(b, b_kind)
+    call("j4c_dot_split_act", ah.data_ptr(), al.data_ptr(), bh.data_ptr(), bl.data_ptr(), M, K, N, bias, act, residual, z,
+         out.data_ptr(), stream)
 
 
 class _Dense(FfiMeta):
@@ -253,11 +261,9 @@ class _Dense(FfiMeta):
             call("j4c_dot_act", t.data_ptr(), w._t.data_ptr(), M, K, N, 0, 0, bp, self.act, rp, zp, y.data_ptr(), stream)
         elif f32:
             if keep:  # with those that the gradient's products take, each operand's in one pass
-                _make_splits(x2, ["r", "t" if K < N else "c"])
+                _make_splits(x2, ["r", "t"])
                 _make_splits(w, ["t", "r"])
-            (xh, xl), (wh, wl) = _split_of(x2, "r"), _split_of(w, "t")
-            call("j4c_dot_split_act", xh.data_ptr(), xl.data_ptr(), wh.data_ptr(), wl.data_ptr(), M, K, N, bp, self.act,
-                 rp, zp, y.data_ptr(), stream)
+            _split_product(x2, "r", w, "t", M, K, N, bp, self.act, rp, zp, y, stream)
         else:
             c = _product(x2, w, False, False, dev)._t  # FLOAT64: the product, then the rest in place or beside it
             if keep_z:
@@ -309,11 +315,21 @@ class _Dense(FfiMeta):
             d = ConcreteNDArray._wrap(dz, Shape(M, N), dt, dev)
             if f32:
                 d._lines = lines
-                _make_splits(d, (["r"] if wanted[0] else []) + ([("c" if K < N else "t")] if wanted[1] else []))
-            if wanted[0]:
-                grads[0] = _product(d, w, False, True, dev).reshape(x._shape)
-            if wanted[1]:
-                grads[1] = _product(x2, d, True, False, dev)
+                _make_splits(d, (["r"] if wanted[0] else []) + (["t"] if wanted[1] else []))
+                # dx = dz . w^T and dw = x^T . dz, every operand read along its rows
+                if wanted[0]:
+                    dx = torch.empty(M * K, dtype=t.dtype, device=t.device)
+                    _split_product(d, "r", w, "r", M, N, K, None, 0, None, None, dx, stream)
+                    grads[0] = ConcreteNDArray._wrap(dx, x._shape, dt, dev)
+                if wanted[1]:
+                    dw = torch.empty(K * N, dtype=t.dtype, device=t.device)
+                    _split_product(x2, "t", d, "t", K, M, N, None, 0, None, None, dw, stream)
+                    grads[1] = ConcreteNDArray._wrap(dw, w._shape, dt, dev)
+            else:
+                if wanted[0]:
+                    grads[0] = _product(d, w, False, True, dev).reshape(x._shape)
+                if wanted[1]:
+                    grads[1] = _product(x2, d, True, False, dev)
         if self.has_bias:
             grads.append(ConcreteNDArray._wrap(dbias, inputs[2]._shape, dt, dev) if want_bias else None)
         if self.has_residual:
