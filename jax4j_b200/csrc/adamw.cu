@@ -13,10 +13,10 @@
 // Bound by HBM with moments in the tensors' type: 28 B per FLOAT32 element (w,
 // g, m, v read; w, m, v written), 41.9 M elements in 209 us = 5.6 TB/s.  With
 // moments in 8 bits 16.1 B, and bound by instructions (some 100 an element, a
-// third of them the IEEE root and quotient and the root's encoding): 190 us =
-// 3.6 TB/s; four elements a lane and an IEEE quotient took 207.  All tensors of a tree share one
-// launch: the table of pointers travels in the kernel's parameters (no copy to
-// the device, nothing a captured graph would have to keep alive), and a CTA
+// third of them the IEEE root and quotient and the root's encoding): 172 us =
+// 3.9 TB/s; without the copies a chunk ahead 188 us.  All tensors of a tree share
+// one launch: the table of pointers travels in the kernel's parameters (no copy
+// to the device, nothing a captured graph would have to keep alive), and a CTA
 // takes chunks of consecutive elements, finding a chunk's tensor by bisection.
 //
 // Moments in 8 bits.  A tensor is cut into blocks of 128 elements, half a
@@ -33,7 +33,6 @@
 #include <cuda_fp8.h>
 
 #include <algorithm>
-#include <cstring>
 
 #include "common.cuh"
 
@@ -42,6 +41,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kCtas = 4;                 // per SM: 64 registers a thread
+constexpr int kQCtas = 3;                // with 8-bit moments, 80 registers a thread (2: 199 us, 4: as fast, with spills)
 constexpr int kQBlock = 128;             // elements that share a step
 constexpr float kTopM = 448.0f;          // largest e4m3 value
 constexpr float kTopR = 480.0f;          // largest code of a root (0xFE; 0xFF is NaN)
@@ -280,14 +280,9 @@ __device__ __forceinline__ void store_codes(uint32_t *p, int64_t at, bool vec, u
     else p[at] = c.x, p[at + 1] = c.y;
 }
 // Eight values at p, those from `left` on behind the tensor.
-__device__ __forceinline__ void load8(const float *p, bool whole, int left, float (&x)[8]) {
-    if (whole) {
-        const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 4);
-        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-    } else {
+__device__ __forceinline__ void load8(const float *p, int left, float (&x)[8]) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) x[e] = e < left ? p[e] : 0.0f;
-    }
+    for (int e = 0; e < 8; e++) x[e] = e < left ? p[e] : 0.0f;
 }
 __device__ __forceinline__ void store8(float *p, bool whole, int left, const float (&x)[8]) {
     if (whole) {
@@ -300,30 +295,95 @@ __device__ __forceinline__ void store8(float *p, bool whole, int left, const flo
     }
 }
 
+// What a half warp does of a chunk: one block (a chunk has at most 16).
+struct Share {
+    int64_t b, i, at, nb;  // the block, its first element and word of the lane, the tensor's blocks
+    int left;              // of the lane's elements, those in the tensor
+    bool is, vec, whole;   // is there a block; 16-byte loads; of all eight elements
+};
 template <int N>
-__global__ void __launch_bounds__(kThreads, kCtas) adamw_q8_kernel(const __grid_constant__ Table<N> tab,
+__device__ __forceinline__ Share share_of(const Table<N> &tab, const Tensor &t, int chunk) {
+    const int lane = threadIdx.x % 16, half = threadIdx.x / 16, per = tab.chunk_elems / kQBlock;
+    Share p;
+    p.nb = (t.n + kQBlock - 1) / kQBlock;
+    p.b = (int64_t)(chunk - t.first) * per + half;
+    p.is = half < per && p.b < p.nb;
+    p.i = p.b * kQBlock + lane * 8;
+    p.at = p.b * 32 + lane * 2;
+    p.left = (int)max((int64_t)0, min((int64_t)8, t.n - p.i));
+    p.vec = t.vec;
+    p.whole = p.vec && p.left == 8;
+    return p;
+}
+template <int BYTES, typename V>
+__device__ __forceinline__ void copy_async(V *to, const void *from) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from),
+                 "n"(BYTES)
+                 : "memory");
+}
+
+// While a chunk is worked on the next one's values are on their way, to the
+// threads' own slots in shared memory (two sets take turns) and the steps to
+// registers.
+template <int N>
+__global__ void __launch_bounds__(kThreads, kQCtas) adamw_q8_kernel(const __grid_constant__ Table<N> tab,
                                                                    const __grid_constant__ Hyper h) {
+    __shared__ __align__(16) float4 slots[2][4][kThreads];  // w, g
+    __shared__ __align__(16) uint2 codes[2][2][kThreads];   // of m, of the roots
     const Coef<float> k(h);
-    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-    for (int chunk = blockIdx.x; chunk < tab.chunks; chunk += gridDim.x) {
+    const int tid = threadIdx.x;
+    float next_m = 0.0f, next_r = 0.0f;
+    auto fetch = [&](int64_t chunk, int to) {
+        if (chunk < tab.chunks) {
+            const Tensor &t = tensor_of(tab, (int)chunk);
+            const Share p = share_of(tab, t, (int)chunk);
+            if (p.is) {
+                const Packed q(t.m, p.nb);
+                next_m = q.steps_m[p.b], next_r = q.steps_r[p.b];
+                if (p.vec) {
+                    copy_async<8>(&codes[to][0][tid], q.m + p.at);
+                    copy_async<8>(&codes[to][1][tid], q.r + p.at);
+                }
+                if (p.whole) {
+                    const float *w = static_cast<const float *>(t.w) + p.i, *g = static_cast<const float *>(t.g) + p.i;
+                    copy_async<16>(&slots[to][0][tid], w);
+                    copy_async<16>(&slots[to][1][tid], w + 4);
+                    copy_async<16>(&slots[to][2][tid], g);
+                    copy_async<16>(&slots[to][3][tid], g + 4);
+                }
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    fetch(blockIdx.x, 0);
+    int turn = 0;
+    for (int chunk = blockIdx.x; chunk < tab.chunks; chunk += gridDim.x, turn ^= 1) {
         const Tensor &t = tensor_of(tab, chunk);
-        const int64_t n = t.n, nb = (n + kQBlock - 1) / kQBlock;
-        const bool vec = t.vec;
-        const int per = tab.chunk_elems / kQBlock;  // blocks of a chunk
-        const int64_t b0 = (int64_t)(chunk - t.first) * per, b1 = min(nb, b0 + per);
-        const float *w = static_cast<const float *>(t.w), *g = static_cast<const float *>(t.g);
+        const Share p = share_of(tab, t, chunk);
+        const int64_t b = p.b, i = p.i, at = p.at;
+        const int left = p.left;
+        const bool vec = p.vec, whole = p.whole;
+        const Packed q(t.m, p.nb), qo(t.m_out, p.nb);
         float *wo = static_cast<float *>(t.w_out);
-        const Packed q(t.m, nb), qo(t.m_out, nb);
         const float decay = k.decay(h, t.wd);
-        for (int64_t b = b0 + 2 * warp + lane / 16; b < b1; b += 2 * (kThreads / 32)) {  // a half warp's block
-            const int64_t i = b * kQBlock + (lane % 16) * 8, at = b * 32 + (lane % 16) * 2;
-            const int left = (int)max((int64_t)0, min((int64_t)8, n - i));  // of the lane's elements, those in the tensor
-            const bool whole = vec && left == 8;
+        const float sm = next_m, sr = next_r;
+        fetch(chunk + (int64_t)gridDim.x, turn ^ 1);
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        if (p.is) {
             float ww[8], gg[8], mm[8], rr[8];
-            load8(w + i, whole, left, ww);
-            load8(g + i, whole, left, gg);
-            const uint2 cm = load_codes(q.m, at, vec), cr = load_codes(q.r, at, vec);
-            const float sm = q.steps_m[b], sr = q.steps_r[b];
+            if (whole) {
+                const float4 x[4] = {slots[turn][0][tid], slots[turn][1][tid], slots[turn][2][tid], slots[turn][3][tid]};
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    ww[4 * e] = x[e].x, ww[4 * e + 1] = x[e].y, ww[4 * e + 2] = x[e].z, ww[4 * e + 3] = x[e].w;
+                    gg[4 * e] = x[2 + e].x, gg[4 * e + 1] = x[2 + e].y, gg[4 * e + 2] = x[2 + e].z, gg[4 * e + 3] = x[2 + e].w;
+                }
+            } else {
+                load8(static_cast<const float *>(t.w) + i, left, ww);
+                load8(static_cast<const float *>(t.g) + i, left, gg);
+            }
+            const uint2 cm = vec ? codes[turn][0][tid] : load_codes(q.m, at, false);
+            const uint2 cr = vec ? codes[turn][1][tid] : load_codes(q.r, at, false);
             decode_m(cm.x, sm, mm);
             decode_m(cm.y, sm, mm + 4);
             decode_r(cr.x, sr, rr);
@@ -380,7 +440,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) adamw_q8_kernel(const __grid_
             }
             store_codes(qo.m, at, vec, make_uint2(om[0], om[1]));
             store_codes(qo.r, at, vec, make_uint2(orr[0], orr[1]));
-            if (lane % 16 == 0) {
+            if (tid % 16 == 0) {
                 qo.steps_m[b] = step_m;
                 qo.steps_r[b] = step_r;
             }
@@ -425,10 +485,10 @@ bool aligned8(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0
 // Lays the tensors' chunks out and launches; chunks of 2048 elements (two
 // vectors of every thread), or of 1024 when that leaves SMs without one.
 template <int N, typename Launch>
-int launch_table(Table<N> &tab, int count, Launch launch) {
+int launch_table(Table<N> &tab, int count, int ctas, Launch launch) {
     int64_t total = 0;
     for (int i = 0; i < count; i++) total += tab.t[i].n;
-    const int64_t slots = (int64_t)sm_count() * kCtas;
+    const int64_t slots = (int64_t)sm_count() * ctas;
     tab.count = count;
     tab.chunk_elems = total >= 2048 * slots ? 2048 : 1024;
     int64_t chunks = 0;
@@ -443,7 +503,7 @@ int launch_table(Table<N> &tab, int count, Launch launch) {
 
 // fill(i, tensor) for every non-empty tensor i; launch(table, grid) per table.
 template <typename Fill, typename Launch>
-int for_tables(int ntensors, const int64_t *numel, Fill fill, Launch launch) {
+int for_tables(int ntensors, const int64_t *numel, int ctas, Fill fill, Launch launch) {
     int nonempty = 0;
     for (int i = 0; i < ntensors; i++) nonempty += numel[i] > 0;
     auto run = [&](auto &tab, int cap) {
@@ -458,7 +518,7 @@ int for_tables(int ntensors, const int64_t *numel, Fill fill, Launch launch) {
                 count++;
             }
             if (count == 0) return (int)J4C_OK;
-            if (int rc = launch_table(tab, count, [&](unsigned grid) { return launch(tab, grid); })) return rc;
+            if (int rc = launch_table(tab, count, ctas, [&](unsigned grid) { return launch(tab, grid); })) return rc;
         }
     };
     if (nonempty <= kSmallTable) {
@@ -524,7 +584,7 @@ int j4c_adamw_step(int dtype, int state_bits, int ntensors, const int64_t *numel
         h.steps_out = nullptr;  // one launch advances the counter
         return (int)J4C_OK;
     };
-    if (int rc = for_tables(ntensors, numel, fill, launch)) return rc;
+    if (int rc = for_tables(ntensors, numel, state_bits == 8 ? kQCtas : kCtas, fill, launch)) return rc;
     if (!any && steps_out) {  // nothing but empty tensors: the counter still advances
         advance_kernel<<<1, 1, 0, s>>>(h);
         J4C_LAUNCH_CHECK("advance_kernel");
@@ -552,7 +612,7 @@ int j4c_adamw_moments(int ntensors, const int64_t *numel, const void *const *sta
         J4C_LAUNCH_CHECK("adamw_moments_kernel");
         return (int)J4C_OK;
     };
-    return for_tables(ntensors, numel, fill, launch);
+    return for_tables(ntensors, numel, kCtas, fill, launch);
 }
 
 }  // extern "C"

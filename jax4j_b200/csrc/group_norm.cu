@@ -16,10 +16,10 @@
 // dy in, dx out backward (12 B).  Two forms:
 //  * Groups of at most 8192 values (rows of features are S = 1, G = 1: layer
 //    norm) are held in registers by 1 to 32 warps, sixteen values a thread where
-//    they come four at a time, else eight: every value is read once, and while a group is worked on the thread's
-//    values of the next one are on their way to shared memory (cp.async).
-//    Backward a warp set keeps its group and walks over samples, so dgamma and
-//    dbeta gather in registers too.
+//    they come four at a time, else eight: every value is read once, and while a
+//    group is worked on the thread's values of the next one are on their way to
+//    shared memory (cp.async).  Backward a warp set keeps its group and walks
+//    over samples, so dgamma and dbeta gather in registers too.
 //  * Larger groups are cut into tiles of rows.  Forward, one kernel leaves every
 //    tile's mean and squared differences per group -- of a thread's batch of
 //    values from registers, merged by Chan, Golub and LeVeque's pairwise update,
