@@ -703,20 +703,18 @@ J4C_API int j4c_group_norm_grad(int dtype, int64_t B, int64_t S, int64_t C, int6
                                 j4c_stream stream);
 
 /* A dense layer, y = act(x . w + bias) + residual (bias [N], residual [M, N]
- * and the pre-activation z [M, N] may each be NULL), FLOAT32:
- * from splits, x's by rows (j4c_split_f32) and w's transposed
+ * and the pre-activation z [M, N] may each be NULL):
+ * FLOAT32 from splits, x's by rows (j4c_split_f32) and w's transposed
  * (j4c_split_f32_transposed), on the tensor cores; */
 J4C_API int j4c_dot_split_act(const float *x_hi, const float *x_lo, const float *wt_hi, const float *wt_lo, int64_t M,
                               int64_t K, int64_t N, const float *bias, int act, const float *residual, float *z,
                               float *y, j4c_stream stream);
-/* and from the arrays themselves, op(A) . op(B) in FP32 FMAs in one launch, for
- * products too small for the splits to pay (K = 0: the sum is 0). */
-J4C_API int j4c_dot_act(const float *a, const float *b, int64_t M, int64_t K, int64_t N, int trans_a, int trans_b,
-                        const float *bias, int act, const float *residual, float *z, float *y, j4c_stream stream);
-/* The elementwise part alone: z += bias, y = act(z) + residual.  y may be z,
- * which then ends as y. */
-J4C_API int j4c_dense_finish(int dtype, void *z, int64_t M, int64_t N, const void *bias, int act, const void *residual,
-                             void *y, j4c_stream stream);
+/* and from the arrays themselves, op(A) . op(B) in FMAs of the dtype (FLOAT32 or
+ * FLOAT64) in one launch, for FLOAT64 and for products too small for the splits
+ * to pay (K = 0: the sum is 0). */
+J4C_API int j4c_dot_act(int dtype, const void *a, const void *b, int64_t M, int64_t K, int64_t N, int trans_a,
+                        int trans_b, const void *bias, int act, const void *residual, void *z, void *y,
+                        j4c_stream stream);
 /* The pass over a dense layer's output gradient dy [M, N]: dz = dy * act'(z)
  * with u = z, or with u = the layer's output before the residual (from_output;
  * none, relu, tanh or sigmoid); dbias [N] = the column sums of dz; lines = dz's
@@ -726,12 +724,11 @@ J4C_API int j4c_dense_finish(int dtype, void *z, int64_t M, int64_t N, const voi
 J4C_API size_t j4c_dense_grad_workspace(int dtype, int64_t M, int64_t N);
 J4C_API int j4c_dense_grad(int dtype, int64_t M, int64_t N, const void *dy, const void *u, int act, int from_output,
                            void *dz, void *dbias, uint32_t *lines, void *ws, size_t ws_bytes, j4c_stream stream);
-/* The whole gradient of a small FLOAT32 layer (see j4c_dot_act) in two
- * launches: j4c_dense_grad, then dx = dz . w^T [M, K] and dw = x^T . dz [K, N]
- * together.  dx or dw, and dbias, may be NULL: not wanted; dz is scratch [M, N]
- * (NULL where act is J4C_ACT_NONE). */
-J4C_API int j4c_dense_backward(const float *x, const float *w, int64_t M, int64_t K, int64_t N, const float *dy,
-                               const float *u, int act, int from_output, float *dz, float *dx, float *dw, float *dbias,
+/* The whole gradient of a layer that j4c_dot_act evaluates: j4c_dense_grad, then
+ * dx = dz . w^T [M, K] and dw = x^T . dz [K, N].  dx or dw, and dbias, may be
+ * NULL: not wanted; dz is scratch [M, N] (NULL where act is J4C_ACT_NONE). */
+J4C_API int j4c_dense_backward(int dtype, const void *x, const void *w, int64_t M, int64_t K, int64_t N, const void *dy,
+                               const void *u, int act, int from_output, void *dz, void *dx, void *dw, void *dbias,
                                void *ws, size_t ws_bytes, j4c_stream stream);
 
 #ifdef __cplusplus

@@ -231,18 +231,15 @@ public final class J4C {
         JAVA_INT, ADDRESS, ADDRESS, ADDRESS, ADDRESS, JAVA_LONG, JAVA_LONG, JAVA_LONG, ADDRESS, JAVA_INT, ADDRESS,
         ADDRESS, ADDRESS, ADDRESS));
     static final MethodHandle DOT_ACT = h("j4c_dot_act", FunctionDescriptor.of(
-        JAVA_INT, ADDRESS, ADDRESS, JAVA_LONG, JAVA_LONG, JAVA_LONG, JAVA_INT, JAVA_INT, ADDRESS, JAVA_INT, ADDRESS,
-        ADDRESS, ADDRESS, ADDRESS));
-    static final MethodHandle DENSE_FINISH = h("j4c_dense_finish", FunctionDescriptor.of(
-        JAVA_INT, JAVA_INT, ADDRESS, JAVA_LONG, JAVA_LONG, ADDRESS, JAVA_INT, ADDRESS, ADDRESS, ADDRESS));
+        JAVA_INT, JAVA_INT, ADDRESS, ADDRESS, JAVA_LONG, JAVA_LONG, JAVA_LONG, JAVA_INT, JAVA_INT, ADDRESS, JAVA_INT,
+        ADDRESS, ADDRESS, ADDRESS, ADDRESS));
     static final MethodHandle DENSE_GRAD_WORKSPACE = h("j4c_dense_grad_workspace", FunctionDescriptor.of(
         JAVA_LONG, JAVA_INT, JAVA_LONG, JAVA_LONG));
     static final MethodHandle DENSE_GRAD = h("j4c_dense_grad", FunctionDescriptor.of(
         JAVA_INT, JAVA_INT, JAVA_LONG, JAVA_LONG, ADDRESS, ADDRESS, JAVA_INT, JAVA_INT, ADDRESS, ADDRESS, ADDRESS,
         ADDRESS, JAVA_LONG, ADDRESS));
-
     static final MethodHandle DENSE_BACKWARD = h("j4c_dense_backward", FunctionDescriptor.of(
-        JAVA_INT, ADDRESS, ADDRESS, JAVA_LONG, JAVA_LONG, JAVA_LONG, ADDRESS, ADDRESS, JAVA_INT, JAVA_INT, ADDRESS,
+        JAVA_INT, JAVA_INT, ADDRESS, ADDRESS, JAVA_LONG, JAVA_LONG, JAVA_LONG, ADDRESS, ADDRESS, JAVA_INT, JAVA_INT, ADDRESS,
         ADDRESS, ADDRESS, ADDRESS, ADDRESS, JAVA_LONG, ADDRESS));
 
     // ---- group norm with an activation (group_norm.cu) ----

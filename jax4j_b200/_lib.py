@@ -131,11 +131,10 @@ SIGNATURES = {
                        C.c_double, P],
     "j4c_adamw_moments": [I32, P, P, P, P, P],
     "j4c_dot_split_act": [P, P, P, P, I64, I64, I64, P, I32, P, P, P, P],
-    "j4c_dot_act": [P, P, I64, I64, I64, I32, I32, P, I32, P, P, P, P],
-    "j4c_dense_finish": [I32, P, I64, I64, P, I32, P, P, P],
+    "j4c_dot_act": [I32, P, P, I64, I64, I64, I32, I32, P, I32, P, P, P, P],
     "j4c_dense_grad_workspace": [I32, I64, I64],
     "j4c_dense_grad": [I32, I64, I64, P, P, I32, I32, P, P, P, P, C.c_size_t, P],
-    "j4c_dense_backward": [P, P, I64, I64, I64, P, P, I32, I32, P, P, P, P, P, C.c_size_t, P],
+    "j4c_dense_backward": [I32, P, P, I64, I64, I64, P, P, I32, I32, P, P, P, P, P, C.c_size_t, P],
     "j4c_group_norm_workspace": [I32, I64, I64, I64, I64, I32],
     "j4c_group_norm": [I32, I64, I64, I64, I64, P, P, P, C.c_double, I32, P, P, P, P, C.c_size_t, P],
     "j4c_group_norm_grad": [I32, I64, I64, I64, I64, P, P, P, I32, P, P, P, P, P, P, P, C.c_size_t, P],

@@ -1,6 +1,6 @@
 // dense.cu -- what a dense layer needs beside the tensor-core product:
-// y = act(x . w + bias) + residual for small products, its elementwise part
-// for FLOAT64, and the pass over the output gradient.
+// y = act(x . w + bias) + residual for small products and for FLOAT64, and the
+// pass over the output gradient.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -20,84 +20,83 @@ bool tc_gemm_supported(int64_t M, int64_t K, int64_t N);
 
 namespace {
 
-// ---- small FLOAT32 products ----------------------------------------------------------
-// A product too small for the tensor-core kernel's splits to pay (each operand
-// is read and written twice before the first MMA, eight launches in all) runs
-// on the CUDA cores in one launch, in FP32 FMAs.  K is cut over a cluster of
-// CTAs so that few output tiles still fill the GPU; their partial sums meet
+// ---- products straight from the arrays --------------------------------------------------------
+// A FLOAT32 product too small for the tcgen05 kernel's splits to pay (each
+// operand is read and written twice before the first MMA, eight launches in
+// all) runs here in one launch of FP32 FMAs, and every FLOAT64 product with the
+// FP64 tensor instruction (tcgen05 has no FP64 kind).  K is cut over a cluster
+// of CTAs so that few output tiles still fill the GPU; their partial sums meet
 // through distributed shared memory and are added in rank order.
+template <typename T>
 struct Product {
-    const float *A, *B, *bias, *residual;
-    float *z, *y;  // z may be NULL
+    const T *A, *B, *bias, *residual;
+    T *z, *y;  // z may be NULL
     int64_t M, K, N;
     int act;
 };
 
+template <typename T, int V>
+struct alignas(sizeof(T) * V) Vec {
+    T e[V];
+};
+
 // acc -> y (and z) at row m, column n.
-__device__ __forceinline__ void finish(const Product &p, int64_t m, int64_t n, float v) {
+template <typename T>
+__device__ __forceinline__ void finish(const Product<T> &p, int64_t m, int64_t n, T v) {
     const int64_t at = m * p.N + n;
-    if (p.bias) v = __fadd_rn(v, p.bias[n]);
+    if (p.bias) v = r_add(v, p.bias[n]);
     if (p.z) p.z[at] = v;
-    float o[1] = {v};
+    T o[1] = {v};
     act_values(p.act, o);
-    p.y[at] = p.residual ? __fadd_rn(o[0], p.residual[at]) : o[0];
+    p.y[at] = p.residual ? r_add(o[0], p.residual[at]) : o[0];
 }
 
 // Up to 16 rows of x against a weight [K, N], bound by reading the weight: a
 // CTA holds 32 V columns, its eight warps take turns along K, a thread V
 // columns of MT rows; x comes from shared memory, one value for the warp.
 constexpr int kRowsThreads = 256, kRowsK = 256;  // rows of the weight whose x is staged together
-template <int MT, int V>
-__global__ void __launch_bounds__(kRowsThreads) rows_kernel(const Product p) {
+template <typename T, int MT, int V>
+__global__ void __launch_bounds__(kRowsThreads) rows_kernel(const Product<T> p) {
     constexpr int COLS = 32 * V;
-    extern __shared__ __align__(16) float smem[];
-    float *xs = smem;   // [kRowsK][MT]
-    float *sum = smem;  // [8 warps][MT][COLS], then [MT][COLS]: after the last use of xs
+    extern __shared__ __align__(16) unsigned char smem[];
+    T *xs = reinterpret_cast<T *>(smem);   // [kRowsK][MT]
+    T *sum = reinterpret_cast<T *>(smem);  // [8 warps][MT][COLS], then [MT][COLS]: after the last use of xs
     const cg::cluster_group cluster = cg::this_cluster();
     const int ranks = cluster.num_blocks(), rank = cluster.block_rank();
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     const int64_t n0 = (int64_t)(blockIdx.x / ranks) * COLS + lane * V, m0 = (int64_t)blockIdx.y * MT;
     const int64_t k0 = p.K * rank / ranks, k1 = p.K * (rank + 1) / ranks;
-    float acc[MT][V];
+    T acc[MT][V];
 #pragma unroll
     for (int m = 0; m < MT; m++)
 #pragma unroll
-        for (int v = 0; v < V; v++) acc[m][v] = 0.0f;
+        for (int v = 0; v < V; v++) acc[m][v] = T(0);
     for (int64_t kb = k0; kb < k1; kb += kRowsK) {
         const int len = (int)min((int64_t)kRowsK, k1 - kb);
         __syncthreads();
         for (int e = threadIdx.x; e < MT * len; e += kRowsThreads) {
             const int m = e / len, k = e - m * len;
-            xs[k * MT + m] = m0 + m < p.M ? p.A[(m0 + m) * p.K + kb + k] : 0.0f;
+            xs[k * MT + m] = m0 + m < p.M ? p.A[(m0 + m) * p.K + kb + k] : T(0);
         }
         __syncthreads();
         if (n0 < p.N) {  // V divides N
-            const float *w = p.B + kb * p.N + n0;
+            const T *w = p.B + kb * p.N + n0;
             constexpr int U = 8;  // loads of the weight in flight
             for (int k = warp; k < len; k += 8 * U) {
-                float b[U][V];
+                Vec<T, V> b[U];
 #pragma unroll
                 for (int u = 0; u < U; u++) {
-                    const float *at = w + (int64_t)(k + 8 * u) * p.N;
-                    const bool in = k + 8 * u < len;
-                    if constexpr (V == 4) {
-                        const float4 t = in ? __ldg(reinterpret_cast<const float4 *>(at)) : float4{0, 0, 0, 0};
-                        b[u][0] = t.x, b[u][1] = t.y, b[u][2] = t.z, b[u][3] = t.w;
-                    } else if constexpr (V == 2) {
-                        const float2 t = in ? __ldg(reinterpret_cast<const float2 *>(at)) : float2{0, 0};
-                        b[u][0] = t.x, b[u][1] = t.y;
-                    } else {
-                        b[u][0] = in ? __ldg(at) : 0.0f;
-                    }
+                    const T *at = w + (int64_t)(k + 8 * u) * p.N;
+                    if (k + 8 * u < len) b[u] = *reinterpret_cast<const Vec<T, V> *>(at);
                 }
 #pragma unroll
                 for (int u = 0; u < U; u++) {
                     if (k + 8 * u >= len) break;
-                    const float *x = xs + (k + 8 * u) * MT;
+                    const T *x = xs + (k + 8 * u) * MT;
 #pragma unroll
                     for (int m = 0; m < MT; m++)
 #pragma unroll
-                        for (int v = 0; v < V; v++) acc[m][v] = fmaf(x[m], b[u][v], acc[m][v]);
+                        for (int v = 0; v < V; v++) acc[m][v] = fma(x[m], b[u].e[v], acc[m][v]);
                 }
             }
         }
@@ -109,7 +108,7 @@ __global__ void __launch_bounds__(kRowsThreads) rows_kernel(const Product p) {
         for (int v = 0; v < V; v++) sum[(warp * MT + m) * COLS + lane * V + v] = acc[m][v];
     __syncthreads();
     for (int e = threadIdx.x; e < MT * COLS; e += kRowsThreads) {
-        float v = sum[e];
+        T v = sum[e];
 #pragma unroll
         for (int w = 1; w < 8; w++) v += sum[w * MT * COLS + e];
         sum[e] = v;
@@ -119,7 +118,7 @@ __global__ void __launch_bounds__(kRowsThreads) rows_kernel(const Product p) {
     for (int e = rank * kRowsThreads + threadIdx.x; e < MT * COLS; e += ranks * kRowsThreads) {
         const int m = e / COLS, c = e - m * COLS;
         if (m0 + m >= p.M || c0 + c >= p.N) continue;
-        float v = 0.0f;
+        T v = T(0);
         for (int r = 0; r < ranks; r++) v += *cluster.map_shared_rank(sum + e, r);
         finish(p, m0 + m, c0 + c, v);
     }
@@ -127,105 +126,148 @@ __global__ void __launch_bounds__(kRowsThreads) rows_kernel(const Product p) {
 }
 
 // The general form, op(A) [M, K] . op(B) [K, N] with either operand stored
-// transposed: 64 x 64 tiles of 128 threads (8 x 4 results each), K in steps of
-// 16 through a ring of three buffers filled by asynchronous copies, two steps
+// transposed: 64 x 64 tiles of 128 threads, K in steps of 16 (FLOAT64: 8) through
+// a ring of three buffers (four) filled by asynchronous copies, two steps (three)
 // ahead: a CTA's share of K is a few steps, each bound by the copies' latency.
-// Also measured, and no faster at [256,784]x[784,512] (13.4 us) to 1024^3 (81
-// us): rings of four and six buffers, 8 x 8 results a thread, and two or four
-// shares of K within a CTA.
-constexpr int kTM = 64, kTN = 64, kTK = 16, kPitch = 68;  // a row of a buffer: padded, 16-byte multiples
-constexpr int kRing = 3, kTileThreads = 128;
-struct TileStep {
-    float A[kTK][kPitch], B[kTK][kPitch];
+// FLOAT32: 8 x 4 results a thread.  FLOAT64: a warp has a quarter of the tile as
+// 4 x 4 tiles of m8n8k4 (A element: row lane / 4, k lane % 4; B: k lane % 4,
+// column lane / 4; results: row lane / 4, columns 2 (lane % 4) and the next).
+// FLOAT32 [256,784]x[784,512] takes 16 us, [1024,1024]x[1024,512] 45; FLOAT64 15
+// and, at 2048^3, 572 us (30 TFLOP/s).  Also measured, and no faster in FLOAT32:
+// rings of four and six buffers, 8 x 8 results a thread, and two or four shares
+// of K within a CTA; in FLOAT64 FMAs instead of the tensor instruction: 22 and
+// 1021 us.
+constexpr int kTM = 64, kTN = 64, kPitch = 68;  // kPitch: a row of a buffer, padded, 16-byte multiples
+constexpr int kTileThreads = 128;
+template <typename T>
+constexpr int kTK = sizeof(T) == 8 ? 8 : 16;
+template <typename T>
+constexpr int kRing = sizeof(T) == 8 ? 4 : 3;
+template <typename T>
+struct alignas(16) TileStep {
+    T A[kTK<T>][kPitch], B[kTK<T>][kPitch];
 };
-__device__ __forceinline__ void copy4_async(float *to, const float *from) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from)
+template <typename T>
+__device__ __forceinline__ void copy_async(T *to, const T *from) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from),
+                 "n"(sizeof(T))
                  : "memory");
 }
-template <bool TA, bool TB>
-__device__ __forceinline__ void tile_product(const Product &p, int64_t tile_m, int64_t tile_n, TileStep *ring) {
+__device__ __forceinline__ void mma_8x8x4(double &d0, double &d1, double a, double b) {
+    asm volatile("mma.sync.aligned.m8n8k4.row.col.f64.f64.f64.f64 {%0, %1}, {%2}, {%3}, {%0, %1};"
+                 : "+d"(d0), "+d"(d1)
+                 : "d"(a), "d"(b));
+}
+template <typename T, bool TA, bool TB>
+__device__ __forceinline__ void tile_product(const Product<T> &p, int64_t tile_m, int64_t tile_n, TileStep<T> *ring) {
+    constexpr int TK = kTK<T>, RING = kRing<T>;
+    constexpr int PER = kTM * TK / kTileThreads, ROWS = kTileThreads / TK;  // values a thread copies of an operand
     // the tile's sums take the ring's place once it has been read
-    float(*const part)[kTN] = reinterpret_cast<float(*)[kTN]>(ring);
-    static_assert(kRing * sizeof(TileStep) >= kTM * kTN * sizeof(float), "the tile's sums take the ring's place");
+    T(*const part)[kTN] = reinterpret_cast<T(*)[kTN]>(ring);
+    static_assert(RING * sizeof(TileStep<T>) >= kTM * kTN * sizeof(T), "the tile's sums take the ring's place");
     const cg::cluster_group cluster = cg::this_cluster();
     const int ranks = cluster.num_blocks(), rank = cluster.block_rank();
     const int tid = threadIdx.x, tx = tid % 16, ty = tid / 16;
     const int64_t n0 = tile_n * kTN, m0 = tile_m * kTM;
     const int64_t k0 = p.K * rank / ranks, k1 = p.K * (rank + 1) / ranks;
-    const int steps = (int)((k1 - k0 + kTK - 1) / kTK);
-    // This thread copies eight values of each operand a step: of one stored
-    // along K, one K of every eighth row; of one stored across, every second K
-    // of a row.  Bit i of the masks: its i-th row (or its row) is in the operand.
-    const int am = TA ? tid % kTM : tid / kTK, ak = TA ? tid / kTM : tid % kTK;
-    const int bn = TB ? tid / kTK : tid % kTN, bk = TB ? tid % kTK : tid / kTN;
-    const float *a = p.A + (TA ? (k0 + ak) * p.M + m0 + am : (m0 + am) * p.K + k0 + ak);
-    const float *b = p.B + (TB ? (n0 + bn) * p.K + k0 + bk : (k0 + bk) * p.N + n0 + bn);
-    const int64_t a_next = TA ? 2 * p.M : 8 * p.K, b_next = TB ? 8 * p.K : 2 * p.N;  // to the thread's next value
-    const int64_t a_step = TA ? kTK * p.M : kTK, b_step = TB ? kTK : kTK * p.N;      // to the next step
+    const int steps = (int)((k1 - k0 + TK - 1) / TK);
+    // This thread copies PER values of each operand a step: of one stored along
+    // K, one K of every ROWS-th row; of one stored across, every second K of a
+    // row.  Bit i of the masks: its i-th row (or its row) is in the operand.
+    const int am = TA ? tid % kTM : tid / TK, ak = TA ? tid / kTM : tid % TK;
+    const int bn = TB ? tid / TK : tid % kTN, bk = TB ? tid % TK : tid / kTN;
+    const T *a = p.A + (TA ? (k0 + ak) * p.M + m0 + am : (m0 + am) * p.K + k0 + ak);
+    const T *b = p.B + (TB ? (n0 + bn) * p.K + k0 + bk : (k0 + bk) * p.N + n0 + bn);
+    const int64_t a_next = TA ? 2 * p.M : ROWS * p.K, b_next = TB ? ROWS * p.K : 2 * p.N;  // to the thread's next value
+    const int64_t a_step = TA ? TK * p.M : TK, b_step = TB ? TK : TK * p.N;                // to the next step
     uint32_t a_in = 0, b_in = 0;
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        a_in |= (m0 + am + (TA ? 0 : 8 * i) < p.M ? 1u : 0u) << i;
-        b_in |= (n0 + bn + (TB ? 8 * i : 0) < p.N ? 1u : 0u) << i;
+    for (int i = 0; i < PER; i++) {
+        a_in |= (m0 + am + (TA ? 0 : ROWS * i) < p.M ? 1u : 0u) << i;
+        b_in |= (n0 + bn + (TB ? ROWS * i : 0) < p.N ? 1u : 0u) << i;
     }
     auto fetch = [&](int step) {
         if (step < steps) {
-            TileStep &to = ring[step % kRing];
-            const int left = (int)min((int64_t)kTK, k1 - k0 - (int64_t)step * kTK);  // Ks of this step
-            const float *pa = a, *pb = b;
+            TileStep<T> &to = ring[step % RING];
+            const int left = (int)min((int64_t)TK, k1 - k0 - (int64_t)step * TK);  // Ks of this step
+            const T *pa = a, *pb = b;
 #pragma unroll
-            for (int i = 0; i < 8; i++, pa += a_next) {
-                const int m = TA ? am : am + 8 * i, k = TA ? ak + 2 * i : ak;
-                if ((a_in >> i & 1u) && k < left) copy4_async(&to.A[k][m], pa);
-                else to.A[k][m] = 0.0f;
+            for (int i = 0; i < PER; i++, pa += a_next) {
+                const int m = TA ? am : am + ROWS * i, k = TA ? ak + 2 * i : ak;
+                if ((a_in >> i & 1u) && k < left) copy_async(&to.A[k][m], pa);
+                else to.A[k][m] = T(0);
             }
 #pragma unroll
-            for (int i = 0; i < 8; i++, pb += b_next) {
-                const int n = TB ? bn + 8 * i : bn, k = TB ? bk : bk + 2 * i;
-                if ((b_in >> i & 1u) && k < left) copy4_async(&to.B[k][n], pb);
-                else to.B[k][n] = 0.0f;
+            for (int i = 0; i < PER; i++, pb += b_next) {
+                const int n = TB ? bn + ROWS * i : bn, k = TB ? bk : bk + 2 * i;
+                if ((b_in >> i & 1u) && k < left) copy_async(&to.B[k][n], pb);
+                else to.B[k][n] = T(0);
             }
             a += a_step, b += b_step;
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    float acc[8][4];
+    constexpr bool MMA = sizeof(T) == 8;
+    T acc[8][4];  // with MMA: tile (i, j) of 8 x 8 is acc[2 i + j / 2][2 (j % 2) ..]
+    const int fr = tid % 32 / 4, fk = tid % 4, wm = tid / 64 * 32, wn = tid / 32 % 2 * 32;
 #pragma unroll
     for (int i = 0; i < 8; i++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) acc[i][j] = 0.0f;
+        for (int j = 0; j < 4; j++) acc[i][j] = T(0);
 #pragma unroll
-    for (int i = 0; i < kRing - 1; i++) fetch(i);
+    for (int i = 0; i < RING - 1; i++) fetch(i);
     for (int step = 0; step < steps; step++) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 2) : "memory");
+        asm volatile("cp.async.wait_group %0;" ::"n"(RING - 2) : "memory");
         __syncthreads();  // this step's copies are everyone's, and the buffer of the step before has been read
-        fetch(step + kRing - 1);
-        const TileStep &at = ring[step % kRing];
+        fetch(step + RING - 1);
+        const TileStep<T> &at = ring[step % RING];
+        if constexpr (MMA) {
 #pragma unroll
-        for (int k = 0; k < kTK; k++) {
-            const float4 a0 = *reinterpret_cast<const float4 *>(&at.A[k][ty * 8]);
-            const float4 a1 = *reinterpret_cast<const float4 *>(&at.A[k][ty * 8 + 4]);
-            const float4 b0 = *reinterpret_cast<const float4 *>(&at.B[k][tx * 4]);
-            const float av[8] = {a0.x, a0.y, a0.z, a0.w, a1.x, a1.y, a1.z, a1.w}, bv[4] = {b0.x, b0.y, b0.z, b0.w};
+            for (int k = 0; k < TK; k += 4) {
+                T av[4], bv[4];
 #pragma unroll
-            for (int i = 0; i < 8; i++)
+                for (int i = 0; i < 4; i++) av[i] = at.A[k + fk][wm + i * 8 + fr], bv[i] = at.B[k + fk][wn + i * 8 + fr];
 #pragma unroll
-                for (int j = 0; j < 4; j++) acc[i][j] = fmaf(av[i], bv[j], acc[i][j]);
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        mma_8x8x4(acc[2 * i + j / 2][j % 2 * 2], acc[2 * i + j / 2][j % 2 * 2 + 1], av[i], bv[j]);
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < TK; k++) {
+                Vec<T, 4> av[2];
+                av[0] = *reinterpret_cast<const Vec<T, 4> *>(&at.A[k][ty * 8]);
+                av[1] = *reinterpret_cast<const Vec<T, 4> *>(&at.A[k][ty * 8 + 4]);
+                const Vec<T, 4> bv = *reinterpret_cast<const Vec<T, 4> *>(&at.B[k][tx * 4]);
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) acc[i][j] = fma(av[i / 4].e[i % 4], bv.e[j], acc[i][j]);
+            }
         }
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 8; i++)
-        *reinterpret_cast<float4 *>(&part[ty * 8 + i][tx * 4]) = make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
+    for (int i = 0; i < 8; i++) {
+        if constexpr (MMA) {
+#pragma unroll
+            for (int j = 0; j < 4; j += 2)
+                *reinterpret_cast<Vec<T, 2> *>(&part[wm + i / 2 * 8 + fr][wn + (i % 2 * 2 + j / 2) * 8 + 2 * fk]) =
+                    Vec<T, 2>{acc[i][j], acc[i][j + 1]};
+        } else {
+            *reinterpret_cast<Vec<T, 4> *>(&part[ty * 8 + i][tx * 4]) = Vec<T, 4>{acc[i][0], acc[i][1], acc[i][2], acc[i][3]};
+        }
+    }
     cluster.sync();
     // Rank r finishes rows r, r + ranks, ... of the tile: a thread every second
     // of them in its column, eight at a time so that their residuals are on
     // their way together.  Shares are added in order.
     const int n = tid % kTN, mine = kTM / ranks;
     if (n0 + n < p.N) {
-        const float bias = p.bias ? p.bias[n0 + n] : 0.0f;
+        const T bias = p.bias ? p.bias[n0 + n] : T(0);
         for (int i0 = tid / kTN; i0 < mine; i0 += 16) {
-            float v[8], res[8];
+            T v[8], res[8];
             int64_t at[8];
             bool in[8];
 #pragma unroll
@@ -233,11 +275,11 @@ __device__ __forceinline__ void tile_product(const Product &p, int64_t tile_m, i
                 const int idx = i0 + 2 * i, m = idx * ranks + rank;
                 in[i] = idx < mine && m0 + m < p.M;
                 at[i] = (m0 + m) * p.N + n0 + n;
-                res[i] = p.residual && in[i] ? p.residual[at[i]] : 0.0f;
-                v[i] = 0.0f;
+                res[i] = p.residual && in[i] ? p.residual[at[i]] : T(0);
+                v[i] = T(0);
                 if (in[i])
                     for (int r = 0; r < ranks; r++) v[i] += *cluster.map_shared_rank(&part[m][n], r);
-                if (p.bias) v[i] = __fadd_rn(v[i], bias);
+                if (p.bias) v[i] = r_add(v[i], bias);
             }
             if (p.z) {
 #pragma unroll
@@ -247,34 +289,36 @@ __device__ __forceinline__ void tile_product(const Product &p, int64_t tile_m, i
             act_values(p.act, v);
 #pragma unroll
             for (int i = 0; i < 8; i++)
-                if (in[i]) p.y[at[i]] = p.residual ? __fadd_rn(v[i], res[i]) : v[i];
+                if (in[i]) p.y[at[i]] = p.residual ? r_add(v[i], res[i]) : v[i];
         }
     }
     cluster.sync();
 }
 
-template <bool TA, bool TB>
-__global__ void __launch_bounds__(kTileThreads) tile_kernel(const Product p) {
-    __shared__ __align__(16) TileStep ring[kRing];
+template <typename T, bool TA, bool TB>
+__global__ void __launch_bounds__(kTileThreads) tile_kernel(const Product<T> p) {
+    __shared__ TileStep<T> ring[kRing<T>];
     const int64_t tile = blockIdx.x / cg::this_cluster().num_blocks(), tiles_n = (p.N + kTN - 1) / kTN;
-    tile_product<TA, TB>(p, tile / tiles_n, tile % tiles_n, ring);
+    tile_product<T, TA, TB>(p, tile / tiles_n, tile % tiles_n, ring);
 }
 
 // Two products in one launch, x's gradient dz . w^T and w's x^T . dz: neither
 // fills the GPU, and together they cost one launch.
+template <typename T>
 struct TwoProducts {
-    Product dx, dw;
+    Product<T> dx, dw;
     int64_t dx_tiles;
 };
-__global__ void __launch_bounds__(kTileThreads) two_products_kernel(const TwoProducts p) {
-    __shared__ __align__(16) TileStep ring[kRing];
+template <typename T>
+__global__ void __launch_bounds__(kTileThreads) two_products_kernel(const TwoProducts<T> p) {
+    __shared__ TileStep<T> ring[kRing<T>];
     const int64_t tile = blockIdx.x / cg::this_cluster().num_blocks();
     if (tile < p.dx_tiles) {
         const int64_t tiles_n = (p.dx.N + kTN - 1) / kTN;
-        tile_product<false, true>(p.dx, tile / tiles_n, tile % tiles_n, ring);
+        tile_product<T, false, true>(p.dx, tile / tiles_n, tile % tiles_n, ring);
     } else {
         const int64_t tiles_n = (p.dw.N + kTN - 1) / kTN, t = tile - p.dx_tiles;
-        tile_product<true, false>(p.dw, t / tiles_n, t % tiles_n, ring);
+        tile_product<T, true, false>(p.dw, t / tiles_n, t % tiles_n, ring);
     }
 }
 
@@ -282,6 +326,7 @@ template <typename Kernel, typename Arg>
 int launch_cluster(Kernel kernel, dim3 grid, int threads, size_t smem, int ranks, const Arg &p, cudaStream_t s) {
     if (smem > 48 * 1024)
         J4C_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    if (ranks > 8) J4C_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid.x * ranks, grid.y);
     cfg.blockDim = dim3(threads);
@@ -298,64 +343,75 @@ int launch_cluster(Kernel kernel, dim3 grid, int threads, size_t smem, int ranks
     return J4C_OK;
 }
 
-// CTAs along K: two output tiles' worth of CTAs an SM where K has 64 for each.
-int ranks_for(int64_t tiles, int64_t K, int64_t most_k) {
+// CTAs along K: two output tiles' worth of CTAs an SM where K has 64 (FLOAT64:
+// 32) for each; clusters of 16 only where few of them are wanted (64 rows of
+// [4096,512] 41 -> 29 us, but [256,784]x[784,512] FLOAT64 15 -> 22 us).
+template <typename T>
+int ranks_for(int64_t tiles, int64_t K) {
     int ranks = 1;
-    while (ranks < 8 && tiles * ranks < 2 * sm_count() && K >= 2 * ranks * most_k) ranks *= 2;
+    while (ranks < 16 && tiles * ranks < (ranks < 8 ? 2 : 1) * sm_count() && K >= 2 * ranks * (256 / (int)sizeof(T))) ranks *= 2;
     return ranks;
 }
 
-template <int MT, int V>
-int launch_rows(const Product &p, cudaStream_t s) {
-    constexpr size_t smem = std::max<size_t>(8 * MT * 32 * V, kRowsK * MT) * sizeof(float);
+template <typename T, int MT, int V>
+int launch_rows(const Product<T> &p, cudaStream_t s) {
+    constexpr size_t smem = std::max<size_t>(8 * MT * 32 * V, kRowsK * MT) * sizeof(T);
     const dim3 grid((unsigned)ceil_div(p.N, 32 * V), (unsigned)ceil_div(p.M, MT));
-    return launch_cluster(rows_kernel<MT, V>, grid, kRowsThreads, smem, ranks_for((int64_t)grid.x * grid.y, p.K, 64), p, s);
+    return launch_cluster(rows_kernel<T, MT, V>, grid, kRowsThreads, smem, ranks_for<T>((int64_t)grid.x * grid.y, p.K), p, s);
 }
-template <int V>
-int launch_rows_m(const Product &p, cudaStream_t s) {
-    if (p.M == 1) return launch_rows<1, V>(p, s);
-    if (p.M == 2) return launch_rows<2, V>(p, s);
-    if (p.M <= 4) return launch_rows<4, V>(p, s);
-    if (p.M <= 8) return launch_rows<8, V>(p, s);
-    return launch_rows<16, V>(p, s);
+template <typename T, int V>
+int launch_rows_m(const Product<T> &p, cudaStream_t s) {
+    if (p.M == 1) return launch_rows<T, 1, V>(p, s);
+    if (p.M == 2) return launch_rows<T, 2, V>(p, s);
+    if (p.M <= 4) return launch_rows<T, 4, V>(p, s);
+    if (p.M <= 8) return launch_rows<T, 8, V>(p, s);
+    return launch_rows<T, 16, V>(p, s);
 }
 
-int64_t tiles_of(const Product &p) { return ceil_div(p.M, kTM) * ceil_div(p.N, kTN); }
+template <typename T>
+int64_t tiles_of(const Product<T> &p) {
+    return ceil_div(p.M, kTM) * ceil_div(p.N, kTN);
+}
 
 // ranks: CTAs along K of the tile form (0: by the product's own size).
-int small_product(const Product &p, int ta, int tb, int ranks, cudaStream_t s) {
+template <typename T>
+int small_product(const Product<T> &p, int ta, int tb, int ranks, cudaStream_t s) {
     if (p.M <= 16 && !ta && !tb) {
         // the widest loads that still give every SM a strip of columns
         auto fits = [&](int v) {
-            return p.N % v == 0 && reinterpret_cast<uintptr_t>(p.B) % (4 * v) == 0 && p.N / (32 * v) * 8 >= sm_count();
+            return p.N % v == 0 && reinterpret_cast<uintptr_t>(p.B) % (sizeof(T) * v) == 0 &&
+                   p.N / (32 * v) * 8 >= sm_count();
         };
-        return fits(4) ? launch_rows_m<4>(p, s) : fits(2) ? launch_rows_m<2>(p, s) : launch_rows_m<1>(p, s);
+        if constexpr (sizeof(T) == 4)
+            if (fits(4)) return launch_rows_m<T, 4>(p, s);
+        return fits(2) ? launch_rows_m<T, 2>(p, s) : launch_rows_m<T, 1>(p, s);
     }
     const int64_t tiles = tiles_of(p);
-    if (!ranks) ranks = ranks_for(tiles, p.K, 64);
+    if (!ranks) ranks = ranks_for<T>(tiles, p.K);
     auto launch = [&](auto kernel) {
         return launch_cluster(kernel, dim3((unsigned)tiles), kTileThreads, 0, ranks, p, s);
     };
-    if (ta) return tb ? launch(tile_kernel<true, true>) : launch(tile_kernel<true, false>);
-    return tb ? launch(tile_kernel<false, true>) : launch(tile_kernel<false, false>);
+    if (ta) return tb ? launch(tile_kernel<T, true, true>) : launch(tile_kernel<T, true, false>);
+    return tb ? launch(tile_kernel<T, false, true>) : launch(tile_kernel<T, false, false>);
 }
 
-// ---- the elementwise part alone (FLOAT64, whose product is the DMMA kernel's) ---------
-// y = act(z) + residual with z += bias first; z is written back unless y is z.
+// x's and w's gradients, in one launch (a cut of K for both) unless that left
+// one of them more than 256 K a CTA that its own cut would not: the gradients of
+// [1839,2090]x[2090,6], dw with 1839 K, 191 us in one launch, 46 in two.  How K is
+// cut depends on the layer's sizes alone, not on which of the two are wanted: the
+// same bits.
 template <typename T>
-__global__ void __launch_bounds__(256) finish_kernel(T *z, int64_t M, int64_t N, const T *__restrict__ bias, int act,
-                                                     const T *__restrict__ residual, T *y) {
-    const int64_t all = M * N;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
-        T v = z[i];
-        if (bias) {
-            v += bias[i % N];
-            if (y != z) z[i] = v;
-        }
-        T o[1] = {v};
-        act_values(act, o);
-        y[i] = residual ? o[0] + residual[i] : o[0];
-    }
+int gradients(const Product<T> &dx, const Product<T> &dw, bool dx_too, bool dw_too, cudaStream_t s) {
+    const int64_t tx = tiles_of(dx), tw = tiles_of(dw);
+    const int both = ranks_for<T>(tx + tw, std::max(dx.K, dw.K));
+    const int rx = ranks_for<T>(tx, dx.K), rw = ranks_for<T>(tw, dw.K);
+    const bool together = std::max(dx.K, dw.K) <= both * 256ll || (rx <= both && rw <= both);
+    if (together && dx_too && dw_too)
+        return launch_cluster(two_products_kernel<T>, dim3((unsigned)(tx + tw)), kTileThreads, 0, both,
+                              TwoProducts<T>{dx, dw, tx}, s);
+    if (dx_too)
+        if (int rc = small_product(dx, 0, 1, together ? both : rx, s)) return rc;
+    return dw_too ? small_product(dw, 1, 0, together ? both : rw, s) : (int)J4C_OK;
 }
 
 // ---- the pass over the output gradient ------------------------------------------------
@@ -392,11 +448,6 @@ struct GradArgs {
     uint32_t *lines;  // FLOAT32: rows, columns, flag (zeroed), or NULL
     int64_t M, N, groups;
     int act, from_output;
-};
-
-template <typename T, int V>
-struct alignas(sizeof(T) * V) Vec {
-    T e[V];
 };
 
 // CLUSTER: the groups of rows of a strip are one cluster, which adds its column
@@ -550,22 +601,30 @@ int dense_grad(int64_t M, int64_t N, const T *dy, const T *u, int act, int from_
 
 using namespace j4c;
 
-// More tiles (eight CTAs each) than a grid takes.
+// More tiles than a grid takes.
 static bool too_many(int64_t M, int64_t N) {
     return M >= (1ll << 40) || N >= (1ll << 33) || ceil_div(M, kTM) * ceil_div(N, 32) >= (1ll << 27);
 }
 
 extern "C" {
 
-int j4c_dot_act(const float *a, const float *b, int64_t M, int64_t K, int64_t N, int trans_a, int trans_b,
-                const float *bias, int act, const float *residual, float *z, float *y, j4c_stream stream) {
+int j4c_dot_act(int dtype, const void *a, const void *b, int64_t M, int64_t K, int64_t N, int trans_a, int trans_b,
+                const void *bias, int act, const void *residual, void *z, void *y, j4c_stream stream) {
+    J4C_REQUIRE(dtype == J4C_FLOAT32 || dtype == J4C_FLOAT64, "j4c_dot_act requires FLOAT32 or FLOAT64 arrays, got %s",
+                dtype_name(dtype));
     J4C_REQUIRE(M >= 0 && K >= 0 && N >= 0, "j4c_dot_act: negative dimension");
     J4C_REQUIRE(act_known(act), "j4c_dot_act: unknown activation %d", act);
     if (M == 0 || N == 0) return J4C_OK;
     J4C_REQUIRE(y && (K == 0 || (a && b)), "j4c_dot_act: NULL pointer");
     if (too_many(M, N))
         return set_error(J4C_E_UNSUPPORTED, "j4c_dot_act: %lld x %lld results are too many", (long long)M, (long long)N);
-    return small_product(Product{a, b, bias, residual, z, y, M, K, N, act}, trans_a, trans_b, 0, as_stream(stream));
+    auto run = [&](auto t) {
+        using T = decltype(t);
+        return small_product(Product<T>{(const T *)a, (const T *)b, (const T *)bias, (const T *)residual, (T *)z, (T *)y, M,
+                                        K, N, act},
+                             trans_a, trans_b, 0, as_stream(stream));
+    };
+    return dtype == J4C_FLOAT64 ? run(0.0) : run(0.0f);
 }
 
 int j4c_dot_split_act(const float *a_hi, const float *a_lo, const float *bt_hi, const float *bt_lo, int64_t M, int64_t K,
@@ -580,24 +639,6 @@ int j4c_dot_split_act(const float *a_hi, const float *a_lo, const float *bt_hi, 
         return set_error(J4C_E_UNSUPPORTED, "j4c_dot_split_act: shape %lld x %lld x %lld is too large", (long long)M,
                          (long long)K, (long long)N);
     return tc_gemm_act(a_hi, a_lo, bt_hi, bt_lo, M, K, N, bias, act, residual, z, y, as_stream(stream));
-}
-
-int j4c_dense_finish(int dtype, void *z, int64_t M, int64_t N, const void *bias, int act, const void *residual, void *y,
-                     j4c_stream stream) {
-    J4C_REQUIRE(dtype == J4C_FLOAT32 || dtype == J4C_FLOAT64, "j4c_dense_finish requires FLOAT32 or FLOAT64 arrays, got %s",
-                dtype_name(dtype));
-    J4C_REQUIRE(M >= 0 && N >= 0, "j4c_dense_finish: negative dimension");
-    J4C_REQUIRE(act_known(act), "j4c_dense_finish: unknown activation %d", act);
-    if (M == 0 || N == 0) return J4C_OK;
-    J4C_REQUIRE(z && y, "j4c_dense_finish: NULL pointer");
-    auto run = [&](auto t) {
-        using T = decltype(t);
-        finish_kernel<T><<<grid_for(M * N, 256), 256, 0, as_stream(stream)>>>((T *)z, M, N, (const T *)bias, act,
-                                                                              (const T *)residual, (T *)y);
-        J4C_LAUNCH_CHECK("finish_kernel");
-        return (int)J4C_OK;
-    };
-    return dtype == J4C_FLOAT64 ? run(0.0) : run(0.0f);
 }
 
 size_t j4c_dense_grad_workspace(int dtype, int64_t M, int64_t N) {
@@ -632,34 +673,31 @@ int j4c_dense_grad(int dtype, int64_t M, int64_t N, const void *dy, const void *
     return dtype == J4C_FLOAT64 ? run(0.0) : run(0.0f);
 }
 
-int j4c_dense_backward(const float *x, const float *w, int64_t M, int64_t K, int64_t N, const float *dy, const float *u,
-                       int act, int from_output, float *dz, float *dx, float *dw, float *dbias, void *ws, size_t ws_bytes,
-                       j4c_stream stream) {
+int j4c_dense_backward(int dtype, const void *x, const void *w, int64_t M, int64_t K, int64_t N, const void *dy,
+                       const void *u, int act, int from_output, void *dz, void *dx, void *dw, void *dbias, void *ws,
+                       size_t ws_bytes, j4c_stream stream) {
+    J4C_REQUIRE(dtype == J4C_FLOAT32 || dtype == J4C_FLOAT64, "j4c_dense_backward requires FLOAT32 or FLOAT64 arrays, got %s",
+                dtype_name(dtype));
     J4C_REQUIRE(M >= 0 && K >= 0 && N >= 0, "j4c_dense_backward: negative dimension");
     J4C_REQUIRE(dx || dw || K == 0 || (M == 0 && N == 0),
                 "j4c_dense_backward: neither product is wanted (j4c_dense_grad gives dbias alone)");
-    const float *d = dy;
+    const void *d = dy;
     if (dbias || act != J4C_ACT_NONE) {
-        if (int rc = j4c_dense_grad(J4C_FLOAT32, M, N, dy, u, act, from_output, dz, dbias, nullptr, ws, ws_bytes, stream))
-            return rc;
+        if (int rc = j4c_dense_grad(dtype, M, N, dy, u, act, from_output, dz, dbias, nullptr, ws, ws_bytes, stream)) return rc;
         if (act != J4C_ACT_NONE) d = dz;
     }
     const bool dx_too = dx && M && K, dw_too = dw && K && N;
     J4C_REQUIRE((!dx_too || N == 0 || (d && w)) && (!dw_too || M == 0 || (d && x)), "j4c_dense_backward: NULL pointer");
-    const Product px{d, w, nullptr, nullptr, nullptr, dx, M, N, K, J4C_ACT_NONE};
-    const Product pw{x, d, nullptr, nullptr, nullptr, dw, K, M, N, J4C_ACT_NONE};
     if ((dx_too && too_many(M, K)) || (dw_too && too_many(K, N)))
         return set_error(J4C_E_UNSUPPORTED, "j4c_dense_backward: %lld x %lld x %lld is too large", (long long)M,
                          (long long)K, (long long)N);
-    cudaStream_t s = as_stream(stream);
-    // the same cut of K whether one product is wanted or both: the same bits
-    const int64_t tx = tiles_of(px), tw = tiles_of(pw);
-    const int ranks = ranks_for(tx + tw, std::max(M, N), 64);
-    if (dx_too && dw_too)
-        return launch_cluster(two_products_kernel, dim3((unsigned)(tx + tw)), kTileThreads, 0, ranks,
-                              TwoProducts{px, pw, tx}, s);
-    if (dx_too) return small_product(px, 0, 1, ranks, s);
-    return dw_too ? small_product(pw, 1, 0, ranks, s) : (int)J4C_OK;
+    auto run = [&](auto t) {
+        using T = decltype(t);
+        const Product<T> px{(const T *)d, (const T *)w, nullptr, nullptr, nullptr, (T *)dx, M, N, K, J4C_ACT_NONE};
+        const Product<T> pw{(const T *)x, (const T *)d, nullptr, nullptr, nullptr, (T *)dw, K, M, N, J4C_ACT_NONE};
+        return gradients(px, pw, dx_too, dw_too, as_stream(stream));
+    };
+    return dtype == J4C_FLOAT64 ? run(0.0) : run(0.0f);
 }
 
 }  // extern "C"

@@ -17,7 +17,7 @@ import torch
 from . import _lib
 from ._lib import call
 from .core import (ConcreteNDArray, DType, IllegalArgumentException, NDArray, Primitive, Shape,
-                   UnsupportedOperationException, _dot_raw, _make_splits, _split_of)
+                   UnsupportedOperationException, _make_splits, _split_of)
 from .tracing import Equation, FfiMeta, TracedNDArray, Tracer, to_var
 
 # J4C_ACT_* (include/jax4j_cuda.h)
@@ -163,8 +163,8 @@ class _GroupNorm(FfiMeta):
 # ---------------------------------------------------------------------------
 # dense layer
 # ---------------------------------------------------------------------------
-# FLOAT32 products of at most this many multiply-adds run on the CUDA cores
-# straight from their arrays (j4c_dot_act); the tensor-core product first
+# FLOAT64 products, and FLOAT32 ones of at most this many multiply-adds, run on
+# the CUDA cores straight from their arrays (j4c_dot_act); the FLOAT32 tensor-core product first
 # splits both operands (five launches more), which larger ones win back: forward
 # of [1024,1024]x[1024,512] 48 against 60 us, with gradients 163 against 169; of
 # [1024,1024]x[1024,1024] 89 against 60 and 264 against 168.
@@ -202,13 +202,6 @@ def dense(x: NDArray, w: NDArray, bias: Optional[NDArray], activation: Optional[
     if Tracer.current() is None:
         return meta.forward(inputs, False)[0]
     return _apply(meta, inputs, Shape(out))
-
-
-def _product(a: ConcreteNDArray, b: ConcreteNDArray, trans_a: bool, trans_b: bool, dev) -> ConcreteNDArray:
-    """op(a) . op(b), which is zeros (of no extent, perhaps) where an extent is 0."""
-    if a._t.numel() and b._t.numel():
-        return _dot_raw(a, b, trans_a, trans_b, dev)
-    return ConcreteNDArray.full(Shape(a._shape[1 if trans_a else 0], b._shape[0 if trans_b else 1]), 0.0, a._dtype, dev)
 
 
 def _split_product(a, a_kind: str, b, b_kind: str, M: int, K: int, N: int, bias, act: int, residual, z, out: torch.Tensor,
@@ -251,26 +244,20 @@ class _Dense(FfiMeta):
         stream = x._stream()
         x2 = x if x._shape.rank() == 2 else x.reshape(Shape(M, K))
         out_shape = Shape(x._shape._d[:-1] + (N,))
-        f32, keep_z = dt == DType.FLOAT32, keep and self.act and not self._from_output()
-        y = torch.empty(M * N, dtype=t.dtype, device=t.device) if f32 or keep_z else None
-        z = torch.empty(M * N, dtype=t.dtype, device=t.device) if f32 and keep_z else None
+        keep_z = keep and self.act and not self._from_output()
+        y = torch.empty(M * N, dtype=t.dtype, device=t.device)
+        z = torch.empty(M * N, dtype=t.dtype, device=t.device) if keep_z else None
         bp = bias._t.data_ptr() if bias is not None else None
         rp = residual._t.data_ptr() if residual is not None else None
         zp = z.data_ptr() if z is not None else None
-        if f32 and (M <= FEW_ROWS or _small(M, K, N)):
-            call("j4c_dot_act", t.data_ptr(), w._t.data_ptr(), M, K, N, 0, 0, bp, self.act, rp, zp, y.data_ptr(), stream)
-        elif f32:
+        if dt != DType.FLOAT32 or M <= FEW_ROWS or _small(M, K, N):
+            call("j4c_dot_act", dt.ordinal, t.data_ptr(), w._t.data_ptr(), M, K, N, 0, 0, bp, self.act, rp, zp, y.data_ptr(),
+                 stream)
+        else:
             if keep:  # with those that the gradient's products take, each operand's in one pass
                 _make_splits(x2, ["r", "t"])
                 _make_splits(w, ["t", "r"])
             _split_product(x2, "r", w, "t", M, K, N, bp, self.act, rp, zp, y, stream)
-        else:
-            c = _product(x2, w, False, False, dev)._t  # FLOAT64: the product, then the rest in place or beside it
-            if keep_z:
-                z = c
-            else:
-                y = c
-            call("j4c_dense_finish", dt.ordinal, c.data_ptr(), M, N, bp, self.act, rp, y.data_ptr(), stream)
         return ConcreteNDArray._wrap(y, out_shape, dt, dev), ((x2, z) if keep else None)
 
     def vjp(self, inputs, out, saved, g, wanted):
@@ -281,14 +268,12 @@ class _Dense(FfiMeta):
         stream = g._stream()
         want_bias = self.has_bias and wanted[2]
         products = wanted[0] or wanted[1]
-        f32 = dt == DType.FLOAT32
-        small = f32 and _small(M, K, N)
+        small = dt != DType.FLOAT32 or _small(M, K, N)
         dz, dbias, lines = t, None, None
         grads: List[Optional[ConcreteNDArray]] = [None, None]
         if want_bias or products:
-            # the pass over g, and for small products all of the gradient
+            # the pass over g, and for products on the CUDA cores all of the gradient
             dev_t = t.device
-            pass_over = want_bias or self.act or (f32 and not small)
             need = _lib.lib().j4c_dense_grad_workspace(dt.ordinal, M, N) if want_bias else 0
             ws = torch.empty(need, dtype=torch.uint8, device=dev_t) if need else None
             wp = ws.data_ptr() if need else None
@@ -301,35 +286,29 @@ class _Dense(FfiMeta):
             if small and products:
                 dx = torch.empty(M * K, dtype=t.dtype, device=dev_t) if wanted[0] else None
                 dw = torch.empty(K * N, dtype=t.dtype, device=dev_t) if wanted[1] else None
-                call("j4c_dense_backward", x2._t.data_ptr(), w._t.data_ptr(), M, K, N, t.data_ptr(), up, self.act,
+                call("j4c_dense_backward", dt.ordinal, x2._t.data_ptr(), w._t.data_ptr(), M, K, N, t.data_ptr(), up, self.act,
                      int(z is None), zp, dx.data_ptr() if wanted[0] else None, dw.data_ptr() if wanted[1] else None, bp,
                      wp, need, stream)
                 grads = [ConcreteNDArray._wrap(dx, x._shape, dt, dev) if wanted[0] else None,
                          ConcreteNDArray._wrap(dw, w._shape, dt, dev) if wanted[1] else None]
-            elif pass_over:
-                if f32 and products:
+            else:
+                if products:
                     lines = torch.empty(M + N + 1, dtype=torch.int32, device=dev_t)
                 call("j4c_dense_grad", dt.ordinal, M, N, t.data_ptr(), up, self.act, int(z is None), zp, bp,
                      lines.data_ptr() if lines is not None else None, wp, need, stream)
         if products and not small:
             d = ConcreteNDArray._wrap(dz, Shape(M, N), dt, dev)
-            if f32:
-                d._lines = lines
-                _make_splits(d, (["r"] if wanted[0] else []) + (["t"] if wanted[1] else []))
-                # dx = dz . w^T and dw = x^T . dz, every operand read along its rows
-                if wanted[0]:
-                    dx = torch.empty(M * K, dtype=t.dtype, device=t.device)
-                    _split_product(d, "r", w, "r", M, N, K, None, 0, None, None, dx, stream)
-                    grads[0] = ConcreteNDArray._wrap(dx, x._shape, dt, dev)
-                if wanted[1]:
-                    dw = torch.empty(K * N, dtype=t.dtype, device=t.device)
-                    _split_product(x2, "t", d, "t", K, M, N, None, 0, None, None, dw, stream)
-                    grads[1] = ConcreteNDArray._wrap(dw, w._shape, dt, dev)
-            else:
-                if wanted[0]:
-                    grads[0] = _product(d, w, False, True, dev).reshape(x._shape)
-                if wanted[1]:
-                    grads[1] = _product(x2, d, True, False, dev)
+            d._lines = lines
+            _make_splits(d, (["r"] if wanted[0] else []) + (["t"] if wanted[1] else []))
+            # dx = dz . w^T and dw = x^T . dz, every operand read along its rows
+            if wanted[0]:
+                dx = torch.empty(M * K, dtype=t.dtype, device=t.device)
+                _split_product(d, "r", w, "r", M, N, K, None, 0, None, None, dx, stream)
+                grads[0] = ConcreteNDArray._wrap(dx, x._shape, dt, dev)
+            if wanted[1]:
+                dw = torch.empty(K * N, dtype=t.dtype, device=t.device)
+                _split_product(x2, "t", d, "t", K, M, N, None, 0, None, None, dw, stream)
+                grads[1] = ConcreteNDArray._wrap(dw, w._shape, dt, dev)
         if self.has_bias:
             grads.append(ConcreteNDArray._wrap(dbias, inputs[2]._shape, dt, dev) if want_bias else None)
         if self.has_residual:

@@ -1,5 +1,5 @@
-"""Nn.dense and its gradients against their formulas in 64 bits: the CUDA-core
-products, the tensor-core products and FLOAT64."""
+"""Nn.dense and its gradients against their formulas in 64 bits: the products
+straight from the arrays (FLOAT32 and FLOAT64) and those from splits."""
 import numpy as np
 import pytest
 
@@ -111,6 +111,28 @@ def test_small_products(J, shape, N, f64):
     x, w, b, res, dy = make(sum(shape) + N, shape, N, np.float64 if f64 else np.float32, bias=N % 2 == 0,
                             residual=sum(shape) % 2 == 0)
     check(run(J, x, w, b, name, res, dy), reference(x, w, b, name, res, dy, 2.0 ** -53 if f64 else U, False))
+
+
+# Few tiles and a long sum, whose K goes over 16 CTAs, and gradients of which one
+# has a long sum and the other many tiles: a launch each.
+LONG = [((40, 4100), 70), ((5000, 24), 30), ((1200, 1500), 5), ((1100, 5), 900), ((2500, 700), 33)]
+
+
+@pytest.mark.parametrize("shape,N", LONG, ids=[f"{'x'.join(map(str, s))}x{n}" for s, n in LONG])
+@pytest.mark.parametrize("f64", [False, True], ids=["f32", "f64"])
+def test_long_sums(J, shape, N, f64):
+    x, w, b, res, dy = make(sum(shape) + N, shape, N, np.float64 if f64 else np.float32)
+    check(run(J, x, w, b, "silu", res, dy), reference(x, w, b, "silu", res, dy, 2.0 ** -53 if f64 else U, False))
+
+
+def test_only_one_gradient_of_long_sums(J):
+    x, w, _, _, dy = make(9, (1200, 1500), 5, bias=False, residual=False)
+    X, W, DY = arr(J, x), arr(J, w), arr(J, dy)
+    both = J.JAX.vjp(lambda a, b: J.Nn.dense(a, b), X, W)[1](DY)
+    dx = J.JAX.vjp(lambda a: J.Nn.dense(a, W), X)[1](DY)
+    dw = J.JAX.vjp(lambda b: J.Nn.dense(X, b), W)[1](DY)
+    np.testing.assert_array_equal(both[0].numpy(), dx[0].numpy())
+    np.testing.assert_array_equal(both[1].numpy(), dw[0].numpy())
 
 
 LARGE = [((17, 5), 3), ((128, 64), 256), ((130, 64), 260), ((257, 1000), 513), ((300, 513), 1000), ((3, 100, 48), 77),

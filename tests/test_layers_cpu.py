@@ -67,22 +67,22 @@ def test_dense_c_entries_refuse_bad_arguments():
     def told(rc, text, code=_lib.E_INVALID):
         assert rc == code and text in L.j4c_last_error().decode(), (rc, L.j4c_last_error())
 
-    told(L.j4c_dot_act(fake, fake, -1, 2, 3, 0, 0, None, 0, None, None, fake, None), "negative")
-    told(L.j4c_dot_act(fake, fake, 1, 2, 3, 0, 0, None, 6, None, None, fake, None), "activation")
-    told(L.j4c_dot_act(fake, None, 1, 2, 3, 0, 0, None, 0, None, None, fake, None), "NULL")
-    told(L.j4c_dot_act(fake, fake, 1, 2, 3, 0, 0, None, 0, None, None, None, None), "NULL")
-    told(L.j4c_dot_act(fake, fake, 1 << 33, 2, 3, 0, 0, None, 0, None, None, fake, None), "too many", _lib.E_UNSUPPORTED)
+    told(L.j4c_dot_act(0, fake, fake, -1, 2, 3, 0, 0, None, 0, None, None, fake, None), "negative")
+    told(L.j4c_dot_act(0, fake, fake, 1, 2, 3, 0, 0, None, 6, None, None, fake, None), "activation")
+    told(L.j4c_dot_act(0, fake, None, 1, 2, 3, 0, 0, None, 0, None, None, fake, None), "NULL")
+    told(L.j4c_dot_act(0, fake, fake, 1, 2, 3, 0, 0, None, 0, None, None, None, None), "NULL")
+    told(L.j4c_dot_act(0, fake, fake, 1 << 33, 2, 3, 0, 0, None, 0, None, None, fake, None), "too many", _lib.E_UNSUPPORTED)
     told(L.j4c_dot_split_act(fake, fake, fake, fake, 2, 0, 3, None, 0, None, None, fake, None), "K = 0")
     told(L.j4c_dot_split_act(fake, None, fake, fake, 2, 4, 3, None, 0, None, None, fake, None), "NULL")
     told(L.j4c_dot_split_act(fake, fake, fake, fake, 2, 4, 3, None, -1, None, None, fake, None), "activation")
-    told(L.j4c_dense_finish(2, fake, 2, 3, None, 0, None, fake, None), "FLOAT32 or FLOAT64")
-    told(L.j4c_dense_finish(1, fake, 2, 3, None, 0, None, None, None), "NULL")
+    told(L.j4c_dot_act(2, fake, fake, 1, 2, 3, 0, 0, None, 0, None, None, fake, None), "FLOAT32 or FLOAT64")
+    told(L.j4c_dense_backward(2, fake, fake, 2, 3, 4, fake, None, 0, 0, None, fake, fake, None, None, 0, None), "FLOAT32 or FLOAT64")
     told(L.j4c_dense_grad(0, 2, 3, fake, None, 3, 0, fake, None, None, None, 0, None), "NULL")
     told(L.j4c_dense_grad(0, 2, 3, fake, fake, 5, 1, fake, None, None, None, 0, None), "does not tell")
     told(L.j4c_dense_grad(1, 2, 3, fake, fake, 2, 1, fake, None, fake, None, 0, None), "line words")
-    told(L.j4c_dense_backward(fake, fake, 2, 3, 4, fake, None, 0, 0, None, None, None, fake, None, 0, None), "neither product")
-    told(L.j4c_dense_backward(fake, fake, 2, 3, 4, fake, fake, 5, 0, None, fake, fake, None, None, 0, None), "NULL")
-    told(L.j4c_dense_backward(fake, None, 2, 3, 4, fake, None, 0, 0, None, fake, fake, None, None, 0, None), "NULL")
+    told(L.j4c_dense_backward(0, fake, fake, 2, 3, 4, fake, None, 0, 0, None, None, None, fake, None, 0, None), "neither product")
+    told(L.j4c_dense_backward(0, fake, fake, 2, 3, 4, fake, fake, 5, 0, None, fake, fake, None, None, 0, None), "NULL")
+    told(L.j4c_dense_backward(0, fake, None, 2, 3, 4, fake, None, 0, 0, None, fake, fake, None, None, 0, None), "NULL")
     told(L.j4c_dense_grad(0, 2000, 3, fake, fake, 2, 1, fake, fake, None, None, 0, None), "workspace")
 
 
