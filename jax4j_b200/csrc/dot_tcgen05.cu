@@ -1840,6 +1840,23 @@ size_t tail_scratch_bound(int64_t m, int64_t n, int64_t batch) {
     return most;
 }
 
+// The microseconds that telling tiles of 256 x 256 from 256 x 128 takes: a CTA
+// pair goes through 1000 K in 19.5 and 14.7 (a tile of half the width reads its A
+// as often), and joining the parts of a split tile takes 4.25 a part of 256
+// columns.  Narrow tiles win where wide ones are split for want of tiles
+// ([1024,1024]x[1024,1024] with gelu, residual and pre-activation 37 -> 29 us) or
+// end in a wave of few (153 of them at [4099,1000]x[1000,2050]: 131 -> 114 us),
+// and lose elsewhere (4096^3: 287 -> 421 us).
+template <int BN, int STAGES>
+static double act_us(int64_t M, int64_t K, int64_t N) {
+    using Q = Cfg<BN, STAGES, 16, true, true>;
+    const int64_t tiles = ceil_div(M, Q::TM) * ceil_div(N, BN), slots = sm_count() / 2;
+    const TailPlan tp = tail_plan(tiles, ceil_div(K, Q::BKE), Q::CHUNK_KB, slots);
+    const double waves = (double)(tp.full_tiles / slots) + (tp.full_tiles % slots != 0) +
+                         (tp.full_tiles < tiles ? 1.0 / tp.splits : 0.0);
+    return waves * (double)K * (BN == 256 ? 0.0195 : 0.0147) + (tp.splits > 1 ? 4.25 * tp.splits * BN / 256 : 0.0);
+}
+
 template <int BN, int STAGES, int BK, bool A_MN, bool B_MN, bool F16, bool PAIR, bool ACT = false>
 static int launch_gemm(const float *ah, const float *al, const float *bh, const float *bl, float *c,
                        int64_t M, int64_t N, int64_t K, bool store_t, const Epilogue &ep, int64_t batch,
@@ -2193,10 +2210,15 @@ int tc_gemm_act(const float *ah, const float *al, const float *bh, const float *
         const char *v = getenv("J4C_GEMM_PAIR");
         return !(v && v[0] == '0');
     }();
-    // the variants of gemm_presplit_ws, with a stage less for the epilogue's areas
-    if (tc::split_fp16() && pair && M >= 2 * tc::BM)
+    // the variants of gemm_presplit_ws, with a stage less for the epilogue's areas,
+    // and for pairs tiles half as wide where they are the faster ones
+    if (tc::split_fp16() && pair && M >= 2 * tc::BM) {
+        if (tc::act_us<128, 6>(M, K, N) < tc::act_us<256, 5>(M, K, N))
+            return tc::launch_gemm<128, 6, 16, false, false, true, true, true>(ah, al, bh, bl, z, M, N, K, false, ep, 1,
+                                                                               false, false, nullptr, s);
         return tc::launch_gemm<256, 5, 16, false, false, true, true, true>(ah, al, bh, bl, z, M, N, K, false, ep, 1, false,
                                                                            false, nullptr, s);
+    }
     if (tc::split_fp16())
         return tc::launch_gemm<256, 3, 16, false, false, true, false, true>(ah, al, bh, bl, z, M, N, K, false, ep, 1, false,
                                                                             false, nullptr, s);

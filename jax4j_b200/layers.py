@@ -166,8 +166,8 @@ class _GroupNorm(FfiMeta):
 # FLOAT64 products, and FLOAT32 ones of at most this many multiply-adds, run on
 # the CUDA cores straight from their arrays (j4c_dot_act); the FLOAT32 tensor-core product first
 # splits both operands (five launches more), which larger ones win back: forward
-# of [1024,1024]x[1024,512] 48 against 60 us, with gradients 163 against 169; of
-# [1024,1024]x[1024,1024] 89 against 60 and 264 against 168.
+# of [1024,1024]x[1024,512] 48 against 62 us, with gradients 152 against 170; of
+# [1024,1024]x[1024,1024] 89 against 60 and 270 against 169.
 SMALL_PRODUCT = 1 << 29
 
 # As many rows or fewer run there whatever the weight's size: they are bound by

@@ -149,6 +149,16 @@ def test_tensor_core_products(J, monkeypatch, shape, N, name, extras):
     check(run(J, x, w, b, name, res, dy), reference(x, w, b, name, res, dy, U, True))
 
 
+# Wide tiles of a CTA pair, one wave of them and a wave and a half whose last
+# tiles are split along K (the shapes above mostly take narrow ones).
+@pytest.mark.parametrize("shape,N", [((2048, 40), 2048), ((3840, 704), 1790)], ids=["2048x40x2048", "3840x704x1790"])
+def test_wide_tiles(J, monkeypatch, shape, N):
+    from jax4j_b200 import layers
+    monkeypatch.setattr(layers, "SMALL_PRODUCT", 0)
+    x, w, b, res, dy = make(N, shape, N)
+    check(run(J, x, w, b, "silu", res, dy), reference(x, w, b, "silu", res, dy, U, True))
+
+
 @pytest.mark.parametrize("name", ACTS)
 @pytest.mark.parametrize("extras", ["both", "bias", "residual", "none"])
 @pytest.mark.parametrize("small", [True, False])
