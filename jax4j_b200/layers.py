@@ -163,11 +163,11 @@ class _GroupNorm(FfiMeta):
 # ---------------------------------------------------------------------------
 # dense layer
 # ---------------------------------------------------------------------------
-# FLOAT64 products, and FLOAT32 ones of at most this many multiply-adds, run on
-# the CUDA cores straight from their arrays (j4c_dot_act); the FLOAT32 tensor-core product first
-# splits both operands (five launches more), which larger ones win back: forward
-# of [1024,1024]x[1024,512] 48 against 62 us, with gradients 152 against 170; of
-# [1024,1024]x[1024,1024] 89 against 60 and 270 against 169.
+# FLOAT64 products, and FLOAT32 ones of at most this many multiply-adds, run
+# straight from their arrays (j4c_dot_act); the FLOAT32 product on the tcgen05
+# tensor cores first splits both operands (five launches more), which larger ones
+# win back: forward of [1024,1024]x[1024,512] 48 against 62 us, with gradients 152
+# against 170; of [1024,1024]x[1024,1024] 89 against 60 and 270 against 169.
 SMALL_PRODUCT = 1 << 29
 
 # As many rows or fewer run there whatever the weight's size: they are bound by
@@ -272,7 +272,7 @@ class _Dense(FfiMeta):
         dz, dbias, lines = t, None, None
         grads: List[Optional[ConcreteNDArray]] = [None, None]
         if want_bias or products:
-            # the pass over g, and for products on the CUDA cores all of the gradient
+            # the pass over g, and without splits all of the gradient
             dev_t = t.device
             need = _lib.lib().j4c_dense_grad_workspace(dt.ordinal, M, N) if want_bias else 0
             ws = torch.empty(need, dtype=torch.uint8, device=dev_t) if need else None
