@@ -453,7 +453,7 @@ struct GradArgs {
 // CLUSTER: the groups of rows of a strip are one cluster, which adds its column
 // sums through distributed shared memory: a.sums is the bias's gradient itself.
 template <typename T, int V, bool CLUSTER>
-__global__ void __launch_bounds__(256) dense_grad_kernel(const GradArgs<T> a) {
+__global__ void __launch_bounds__(256, 4) dense_grad_kernel(const GradArgs<T> a) {
     __shared__ T sums[8][256];
     __shared__ uint32_t tops[8][256];
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
@@ -466,54 +466,46 @@ __global__ void __launch_bounds__(256) dense_grad_kernel(const GradArgs<T> a) {
     bool bad = false;
 #pragma unroll
     for (int i = 0; i < 8; i++) sum[i] = T(0), top[i] = 0;
-    constexpr int U = 2;  // rows in flight
-    for (int64_t r = r0 + warp; r < r1; r += 8 * U) {
-        T d[U][8], u[U][8];
+    for (int64_t r = r0 + warp; r < r1; r += 8) {
+        T d[8], u[8];
 #pragma unroll
-        for (int k = 0; k < U; k++) {
+        for (int i = 0; i < 8; i += V) {
+            Vec<T, V> x{}, z{};
+            if (c0 + col(i) < a.N) {  // V divides N
+                const int64_t at = r * a.N + c0 + col(i);
+                x = *reinterpret_cast<const Vec<T, V> *>(a.dy + at);
+                if (a.u) z = *reinterpret_cast<const Vec<T, V> *>(a.u + at);
+            }
 #pragma unroll
-            for (int i = 0; i < 8; i += V) {
-                Vec<T, V> x{}, z{};
-                if (r + 8 * k < r1 && c0 + col(i) < a.N) {  // V divides N
-                    const int64_t at = (r + 8 * k) * a.N + c0 + col(i);
-                    x = *reinterpret_cast<const Vec<T, V> *>(a.dy + at);
-                    if (a.u) z = *reinterpret_cast<const Vec<T, V> *>(a.u + at);
-                }
+            for (int e = 0; e < V; e++) d[i + e] = x.e[e], u[i + e] = z.e[e];
+        }
+        if (a.from_output) slopes_of_output(a.act, u, d);
+        else act_slopes(a.act, u, d);
+        uint32_t rtop = 0;
 #pragma unroll
-                for (int e = 0; e < V; e++) d[k][i + e] = x.e[e], u[k][i + e] = z.e[e];
+        for (int i = 0; i < 8; i++) {
+            sum[i] += d[i];
+            if constexpr (sizeof(T) == 4) {
+                const uint32_t b = __float_as_uint((float)d[i]) & 0x7FFFFFFFu;
+                const bool fin = b < 0x7F800000u;
+                bad |= !fin && c0 + col(i) < a.N;
+                top[i] = max(top[i], fin ? b : 0u);
+                rtop = max(rtop, fin ? b : 0u);
             }
         }
+        if (a.dz) {
 #pragma unroll
-        for (int k = 0; k < U; k++) {
-            if (r + 8 * k >= r1) break;  // the whole warp
-            if (a.from_output) slopes_of_output(a.act, u[k], d[k]);
-            else act_slopes(a.act, u[k], d[k]);
-            uint32_t rtop = 0;
+            for (int i = 0; i < 8; i += V)
+                if (c0 + col(i) < a.N) {
+                    Vec<T, V> x;
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                sum[i] += d[k][i];
-                if constexpr (sizeof(T) == 4) {
-                    const uint32_t b = __float_as_uint((float)d[k][i]) & 0x7FFFFFFFu;
-                    const bool fin = b < 0x7F800000u;
-                    bad |= !fin && c0 + col(i) < a.N;
-                    top[i] = max(top[i], fin ? b : 0u);
-                    rtop = max(rtop, fin ? b : 0u);
+                    for (int e = 0; e < V; e++) x.e[e] = d[i + e];
+                    *reinterpret_cast<Vec<T, V> *>(a.dz + r * a.N + c0 + col(i)) = x;
                 }
-            }
-            if (a.dz) {
-#pragma unroll
-                for (int i = 0; i < 8; i += V)
-                    if (c0 + col(i) < a.N) {
-                        Vec<T, V> x;
-#pragma unroll
-                        for (int e = 0; e < V; e++) x.e[e] = d[k][i + e];
-                        *reinterpret_cast<Vec<T, V> *>(a.dz + (r + 8 * k) * a.N + c0 + col(i)) = x;
-                    }
-            }
-            if (sizeof(T) == 4 && a.lines) {
-                rtop = __reduce_max_sync(0xffffffffu, rtop);
-                if (lane == 0 && rtop) atomicMax(a.lines + r + 8 * k, rtop);
-            }
+        }
+        if (sizeof(T) == 4 && a.lines) {
+            rtop = __reduce_max_sync(0xffffffffu, rtop);
+            if (lane == 0 && rtop) atomicMax(a.lines + r, rtop);
         }
     }
 #pragma unroll
@@ -547,11 +539,13 @@ __global__ void __launch_bounds__(256) dense_grad_kernel(const GradArgs<T> a) {
     if (a.lines && __any_sync(0xffffffffu, bad) && lane == 0) atomicOr(a.lines + a.M + a.N, 1u);
 }
 
-// Groups of rows: four CTAs an SM, at least 32 rows each; where eight are
-// enough for that, or for 512 rows, they are a cluster and need no second launch.
+// Groups of rows: four CTAs an SM (64 registers a thread, one row of a warp in
+// flight: [8192,4096] gelu 68 us, 5.9 TB/s; two rows in flight and two CTAs an SM
+// 75) and no more, at least 32 rows each; where eight are enough for that, or for
+// 512 rows, they are a cluster and need no second launch.
 int64_t grad_groups(int64_t M, int64_t N) {
     const int64_t groups = std::max<int64_t>(
-        1, std::min(ceil_div(M, 32), ceil_div((int64_t)sm_count() * 4, ceil_div(N, 256))));
+        1, std::min(ceil_div(M, 32), (int64_t)sm_count() * 4 / ceil_div(N, 256)));
     return M <= 512 ? std::min<int64_t>(groups, 8) : groups;
 }
 
