@@ -1234,8 +1234,10 @@ __device__ __forceinline__ void flag_nonfinite(bool bad, SplitHeader *h0, SplitH
 // non-negative floats order like their bits as unsigned integers).  Work
 // unit (s, g): the 512-column strip s of the rows [g R / G, (g + 1) R / G);
 // lane l reads the four columns 4l.. of each 128-column quarter of the strip
-// (16-byte loads when X allows), warp w every 8th row from w, four rows per
-// step (16 independent loads in flight per thread).  A row's max over the
+// (16-byte loads when X allows), warp w every 8th row from w, one row at a time
+// and four CTAs an SM, one wave of them ([4096,4096]: 14.7 us, with the SGD
+// update 40; four rows at a time took 146 registers and one CTA an SM: 25 and
+// 90; two and two 19 and 54).  A row's max over the
 // strip is reduced over the warp (redux.sync) and added with one atomic; a
 // column's over the unit's rows is kept in registers, reduced over the 8
 // warps in shared memory and added with one atomic per unit.
@@ -1243,12 +1245,12 @@ __device__ __forceinline__ void flag_nonfinite(bool bad, SplitHeader *h0, SplitH
 // w - ((gsrc * scale) * lr), written to out; the maxima are those of the result
 // (the SGD update of a weight leaving the line words its next splits take).
 template <bool ROWS, bool COLS, bool SGD = false>
-__global__ void __launch_bounds__(256) lines_max_kernel(const float *__restrict__ src, int64_t R, int64_t C, int vec,
+__global__ void __launch_bounds__(256, 4) lines_max_kernel(const float *__restrict__ src, int64_t R, int64_t C, int vec,
                                                         int64_t groups, uint32_t *__restrict__ rowmax,
                                                         uint32_t *__restrict__ colmax, uint32_t *__restrict__ flag,
                                                         const float *__restrict__ gsrc = nullptr, float scale = 0.0f,
                                                         float lr = 0.0f, float *__restrict__ out = nullptr) {
-    constexpr int TC = 512, RW = 4;
+    constexpr int TC = 512;
     __shared__ uint32_t cm[COLS ? 8 : 1][COLS ? TC : 1];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t strips = (C + TC - 1) / TC;
@@ -1259,62 +1261,53 @@ __global__ void __launch_bounds__(256) lines_max_kernel(const float *__restrict_
         uint32_t cmx[16];
 #pragma unroll
         for (int k = 0; k < 16; k++) cmx[k] = 0;
-        for (int64_t rb = r_begin + warp; rb < r_end; rb += 8 * RW) {
-            uint32_t b[RW][16];
+        for (int64_t r = r_begin + warp; r < r_end; r += 8) {
+            const float *p = src + r * C;
+            uint32_t b[16];
 #pragma unroll
-            for (int i = 0; i < RW; i++) {
-                const int64_t r = rb + 8 * i;
-                const float *p = src + r * C;
-#pragma unroll
-                for (int qq = 0; qq < 4; qq++) {
-                    const int64_t c = c0 + qq * 128 + 4 * lane;
-                    if (r < r_end && vec && c + 4 <= C) {
-                        const uint4 u = __ldg(reinterpret_cast<const uint4 *>(p + c));
-                        b[i][4 * qq] = u.x; b[i][4 * qq + 1] = u.y; b[i][4 * qq + 2] = u.z; b[i][4 * qq + 3] = u.w;
-                        if constexpr (SGD) {
-                            const float4 gv = __ldg(reinterpret_cast<const float4 *>(gsrc + r * C + c));
-                            const float gg[4] = {gv.x, gv.y, gv.z, gv.w};
-                            float o[4];
-#pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                o[e] = __fsub_rn(__uint_as_float(b[i][4 * qq + e]),
-                                                 __fmul_rn(__fmul_rn(gg[e], scale), lr));
-                                b[i][4 * qq + e] = __float_as_uint(o[e]);
-                            }
-                            *reinterpret_cast<float4 *>(out + r * C + c) = make_float4(o[0], o[1], o[2], o[3]);
-                        }
-                    } else {
+            for (int qq = 0; qq < 4; qq++) {
+                const int64_t c = c0 + qq * 128 + 4 * lane;
+                if (vec && c + 4 <= C) {
+                    const uint4 u = __ldg(reinterpret_cast<const uint4 *>(p + c));
+                    b[4 * qq] = u.x; b[4 * qq + 1] = u.y; b[4 * qq + 2] = u.z; b[4 * qq + 3] = u.w;
+                    if constexpr (SGD) {
+                        const float4 gv = __ldg(reinterpret_cast<const float4 *>(gsrc + r * C + c));
+                        const float gg[4] = {gv.x, gv.y, gv.z, gv.w};
+                        float o[4];
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
-                            const bool in = r < r_end && c + e < C;
-                            b[i][4 * qq + e] = in ? __float_as_uint(p[c + e]) : 0u;
-                            if constexpr (SGD) {
-                                if (in) {
-                                    const float o = __fsub_rn(__uint_as_float(b[i][4 * qq + e]),
-                                                              __fmul_rn(__fmul_rn(gsrc[r * C + c + e], scale), lr));
-                                    out[r * C + c + e] = o;
-                                    b[i][4 * qq + e] = __float_as_uint(o);
-                                }
+                            o[e] = __fsub_rn(__uint_as_float(b[4 * qq + e]), __fmul_rn(__fmul_rn(gg[e], scale), lr));
+                            b[4 * qq + e] = __float_as_uint(o[e]);
+                        }
+                        *reinterpret_cast<float4 *>(out + r * C + c) = make_float4(o[0], o[1], o[2], o[3]);
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const bool in = c + e < C;
+                        b[4 * qq + e] = in ? __float_as_uint(p[c + e]) : 0u;
+                        if constexpr (SGD) {
+                            if (in) {
+                                const float o = __fsub_rn(__uint_as_float(b[4 * qq + e]),
+                                                          __fmul_rn(__fmul_rn(gsrc[r * C + c + e], scale), lr));
+                                out[r * C + c + e] = o;
+                                b[4 * qq + e] = __float_as_uint(o);
                             }
                         }
                     }
                 }
             }
+            uint32_t rmx = 0;
 #pragma unroll
-            for (int i = 0; i < RW; i++) {
-                uint32_t rmx = 0;
-#pragma unroll
-                for (int k = 0; k < 16; k++) {
-                    bad |= (b[i][k] & 0x7F800000u) == 0x7F800000u;
-                    const uint32_t m = finite_bits(__uint_as_float(b[i][k]));
-                    rmx = max(rmx, m);
-                    cmx[k] = max(cmx[k], m);
-                }
-                if (ROWS) {
-                    rmx = __reduce_max_sync(0xffffffffu, rmx);
-                    const int64_t r = rb + 8 * i;
-                    if (lane == 0 && r < r_end && rmx) atomicMax(rowmax + r, rmx);
-                }
+            for (int k = 0; k < 16; k++) {
+                bad |= (b[k] & 0x7F800000u) == 0x7F800000u;
+                const uint32_t m = finite_bits(__uint_as_float(b[k]));
+                rmx = max(rmx, m);
+                cmx[k] = max(cmx[k], m);
+            }
+            if (ROWS) {
+                rmx = __reduce_max_sync(0xffffffffu, rmx);
+                if (lane == 0 && rmx) atomicMax(rowmax + r, rmx);
             }
         }
         if (COLS) {
@@ -1331,6 +1324,11 @@ __global__ void __launch_bounds__(256) lines_max_kernel(const float *__restrict_
         }
     }
     if (flag && __any_sync(0xffffffffu, bad) && lane == 0) atomicOr(flag, 1u);
+}
+
+// Row groups of a max pass: one wave of units, at least 32 rows each.
+inline int64_t lines_groups(int64_t rows, int64_t strips) {
+    return std::max<int64_t>(1, std::min<int64_t>(ceil_div(rows, 32), (int64_t)sm_count() * 4 / strips));
 }
 
 // The scale 2^e of a line from its max word.
@@ -1974,8 +1972,7 @@ static int lines_max(const float *src, int64_t rows, int64_t cols, uint32_t *row
     // units: 512-column strips times row groups of at least 32 rows, about
     // four per SM
     const int64_t strips = ceil_div(cols, 512);
-    const int64_t groups = std::max<int64_t>(1, std::min<int64_t>(ceil_div(rows, 32),
-                                                                  ceil_div((int64_t)sm_count() * 4, strips)));
+    const int64_t groups = lines_groups(rows, strips);
     const unsigned grid = (unsigned)std::min<int64_t>(strips * groups, (int64_t)sm_count() * 8);
     if (rowmax && colmax)
         lines_max_kernel<true, true><<<grid, 256, 0, s>>>(src, rows, cols, vec, groups, rowmax, colmax, flag);
@@ -1997,8 +1994,7 @@ int sgd_update_lines(const float *w, const float *g, int64_t rows, int64_t cols,
     J4C_CUDA(cudaMemsetAsync(lines, 0, (size_t)(rows + cols + 1) * sizeof(uint32_t), s));
     const int vec = (cols % 4 == 0) && aligned16(w) && aligned16(g) && aligned16(out);
     const int64_t strips = ceil_div(cols, 512);
-    const int64_t groups = std::max<int64_t>(1, std::min<int64_t>(ceil_div(rows, 32),
-                                                                  ceil_div((int64_t)sm_count() * 4, strips)));
+    const int64_t groups = lines_groups(rows, strips);
     const unsigned grid = (unsigned)std::min<int64_t>(strips * groups, (int64_t)sm_count() * 8);
     lines_max_kernel<true, true, true><<<grid, 256, 0, s>>>(w, rows, cols, vec, groups, lines, lines + rows,
                                                             lines + rows + cols, g, scale, lr, out);
