@@ -518,9 +518,15 @@ def _relu_fed_dots(jaxpr: Jaxpr, need) -> Dict[int, object]:
     return found
 
 
+_current_pmap = None  # PmapContext.current, imported at its first use (pmap imports this module)
+
+
 def _pmap_context():
-    from .pmap import PmapContext
-    return PmapContext.current()
+    global _current_pmap
+    if _current_pmap is None:
+        from .pmap import PmapContext
+        _current_pmap = PmapContext.current
+    return _current_pmap()
 
 
 def do_backward(jaxpr: Jaxpr, values: Dict[int, NDArray], seeds: List[NDArray]) -> List[NDArray]:

@@ -273,19 +273,18 @@ class _Dense(FfiMeta):
         grads: List[Optional[ConcreteNDArray]] = [None, None]
         if want_bias or products:
             # the pass over g, and without splits all of the gradient
-            dev_t = t.device
             need = _lib.lib().j4c_dense_grad_workspace(dt.ordinal, M, N) if want_bias else 0
-            ws = torch.empty(need, dtype=torch.uint8, device=dev_t) if need else None
+            ws = torch.empty(need, dtype=torch.uint8, device=t.device) if need else None
             wp = ws.data_ptr() if need else None
             if self.act:
-                dz = torch.empty(M * N, dtype=t.dtype, device=dev_t)
+                dz = torch.empty_like(t)
             if want_bias:
-                dbias = torch.empty(N, dtype=t.dtype, device=dev_t)
+                dbias = torch.empty_like(inputs[2]._t)
             up = (z if z is not None else out._t).data_ptr() if self.act else None
             zp, bp = dz.data_ptr() if self.act else None, dbias.data_ptr() if want_bias else None
             if small and products:
-                dx = torch.empty(M * K, dtype=t.dtype, device=dev_t) if wanted[0] else None
-                dw = torch.empty(K * N, dtype=t.dtype, device=dev_t) if wanted[1] else None
+                dx = torch.empty_like(x2._t) if wanted[0] else None
+                dw = torch.empty_like(w._t) if wanted[1] else None
                 call("j4c_dense_backward", dt.ordinal, x2._t.data_ptr(), w._t.data_ptr(), M, K, N, t.data_ptr(), up, self.act,
                      int(z is None), zp, dx.data_ptr() if wanted[0] else None, dw.data_ptr() if wanted[1] else None, bp,
                      wp, need, stream)
@@ -293,7 +292,7 @@ class _Dense(FfiMeta):
                          ConcreteNDArray._wrap(dw, w._shape, dt, dev) if wanted[1] else None]
             else:
                 if products:
-                    lines = torch.empty(M + N + 1, dtype=torch.int32, device=dev_t)
+                    lines = torch.empty(M + N + 1, dtype=torch.int32, device=t.device)
                 call("j4c_dense_grad", dt.ordinal, M, N, t.data_ptr(), up, self.act, int(z is None), zp, bp,
                      lines.data_ptr() if lines is not None else None, wp, need, stream)
         if products and not small:
@@ -302,11 +301,11 @@ class _Dense(FfiMeta):
             _make_splits(d, (["r"] if wanted[0] else []) + (["t"] if wanted[1] else []))
             # dx = dz . w^T and dw = x^T . dz, every operand read along its rows
             if wanted[0]:
-                dx = torch.empty(M * K, dtype=t.dtype, device=t.device)
+                dx = torch.empty_like(x2._t)
                 _split_product(d, "r", w, "r", M, N, K, None, 0, None, None, dx, stream)
                 grads[0] = ConcreteNDArray._wrap(dx, x._shape, dt, dev)
             if wanted[1]:
-                dw = torch.empty(K * N, dtype=t.dtype, device=t.device)
+                dw = torch.empty_like(w._t)
                 _split_product(x2, "t", d, "t", K, M, N, None, 0, None, None, dw, stream)
                 grads[1] = ConcreteNDArray._wrap(dw, w._shape, dt, dev)
         if self.has_bias:
