@@ -343,13 +343,15 @@ def test_only_the_wanted_gradients(J, monkeypatch, small):
         np.testing.assert_array_equal(J.JAX.vjp(f, arg)[1](DY)[0].numpy(), full[n])
 
 
-@pytest.mark.parametrize("shape,N,small", [((64, 200), 100, True), ((512, 1024), 600, False)])
-def test_recorded_and_on_another_stream(J, monkeypatch, shape, N, small):
+@pytest.mark.parametrize("shape,N,small,dt", [((64, 200), 100, True, np.float32), ((512, 1024), 600, False, np.float32),
+                                              ((40, 4100), 70, True, np.float64), ((1200, 1500), 5, True, np.float32),
+                                              ((3840, 704), 1790, False, np.float32)])
+def test_recorded_and_on_another_stream(J, monkeypatch, shape, N, small, dt):
     import torch
     from jax4j_b200 import layers
     monkeypatch.setattr(layers, "SMALL_PRODUCT", layers.SMALL_PRODUCT if small else 0)
     from jax4j_b200.graphs import CapturedStep
-    x, w, b, res, dy = make(12, shape, N)
+    x, w, b, res, dy = make(12, shape, N, dt)
     r = np.random.default_rng(13)
 
     def step(*a):
@@ -360,7 +362,7 @@ def test_recorded_and_on_another_stream(J, monkeypatch, shape, N, small):
     y, pull = J.JAX.vjp(lambda p, q: J.Nn.dense(p, q, args[2], "gelu"), args[0], args[1])
     graphs = [CapturedStep(step, [J.ConcreteNDArray(a.tensor().clone(), a.shape()) for a in args]) for _ in range(2)]
     for _ in range(2):
-        args = [arr(J, r.standard_normal(a.shape().dimensions()).astype(np.float32)) for a in args]
+        args = [arr(J, r.standard_normal(a.shape().dimensions()).astype(dt)) for a in args]
         want = [a.numpy() for a in step(*args)]
         for gr in graphs:
             for i, a in enumerate(args):
