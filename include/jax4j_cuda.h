@@ -711,7 +711,8 @@ J4C_API int j4c_dot_split_act(const float *x_hi, const float *x_lo, const float 
                               float *y, j4c_stream stream);
 /* and from the arrays themselves, op(A) . op(B) in FMAs of the dtype (FLOAT32 or
  * FLOAT64) in one launch, for FLOAT64 and for products too small for the splits
- * to pay (K = 0: the sum is 0). */
+ * to pay (K = 0: the sum is 0).  Sums too long for a cluster of CTAs come in
+ * parts, through stream-ordered scratch and a second launch. */
 J4C_API int j4c_dot_act(int dtype, const void *a, const void *b, int64_t M, int64_t K, int64_t N, int trans_a,
                         int trans_b, const void *bias, int act, const void *residual, void *z, void *y,
                         j4c_stream stream);

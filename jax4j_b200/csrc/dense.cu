@@ -26,7 +26,10 @@ namespace {
 // all) runs here in one launch of FP32 FMAs, and every FLOAT64 product with the
 // FP64 tensor instruction (tcgen05 has no FP64 kind).  K is cut over a cluster
 // of CTAs so that few output tiles still fill the GPU; their partial sums meet
-// through distributed shared memory and are added in rank order.
+// through distributed shared memory and are added in rank order.  A sum too long
+// for one cluster is cut into parts first (gridDim.z, parts_for): each part's
+// results go to its own [M, N] of y, and join_kernel adds the parts in order and
+// applies the rest.
 template <typename T>
 struct Product {
     const T *A, *B, *bias, *residual;
@@ -42,13 +45,34 @@ struct alignas(sizeof(T) * V) Vec {
 
 // acc -> y (and z) at row m, column n.
 template <typename T>
-__device__ __forceinline__ void finish(const Product<T> &p, int64_t m, int64_t n, T v) {
+__device__ __forceinline__ void finish(const Product<T> &p, T *y, int64_t m, int64_t n, T v) {
     const int64_t at = m * p.N + n;
     if (p.bias) v = r_add(v, p.bias[n]);
     if (p.z) p.z[at] = v;
     T o[1] = {v};
     act_values(p.act, o);
-    p.y[at] = p.residual ? r_add(o[0], p.residual[at]) : o[0];
+    y[at] = p.residual ? r_add(o[0], p.residual[at]) : o[0];
+}
+
+// The sums over K of the calling CTA: [from, to) of its part and its rank in the
+// cluster; and its part's results.
+template <typename T>
+struct Share {
+    int64_t from, to;
+    T *y;
+    __device__ __forceinline__ Share(const Product<T> &p, int rank, int ranks) {
+        const int64_t at = (int64_t)blockIdx.z * ranks + rank, all = (int64_t)gridDim.z * ranks;
+        from = p.K * at / all;
+        to = p.K * (at + 1) / all;
+        y = p.y + blockIdx.z * p.M * p.N;
+    }
+};
+
+template <typename T>
+__global__ void __launch_bounds__(1024) join_kernel(const Product<T> p, const T *__restrict__ sums, int64_t parts) {
+    const T v = column_sum(sums, parts, p.M * p.N);
+    const int64_t e = (int64_t)blockIdx.x * 32 + threadIdx.x / 32;
+    if (threadIdx.x % 32 == 0 && e < p.M * p.N) finish(p, p.y, e / p.N, e % p.N, v);
 }
 
 // Up to 16 rows of x against a weight [K, N], bound by reading the weight: a
@@ -65,7 +89,8 @@ __global__ void __launch_bounds__(kRowsThreads) rows_kernel(const Product<T> p) 
     const int ranks = cluster.num_blocks(), rank = cluster.block_rank();
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     const int64_t n0 = (int64_t)(blockIdx.x / ranks) * COLS + lane * V, m0 = (int64_t)blockIdx.y * MT;
-    const int64_t k0 = p.K * rank / ranks, k1 = p.K * (rank + 1) / ranks;
+    const Share<T> share(p, rank, ranks);
+    const int64_t k0 = share.from, k1 = share.to;
     T acc[MT][V];
 #pragma unroll
     for (int m = 0; m < MT; m++)
@@ -120,7 +145,7 @@ __global__ void __launch_bounds__(kRowsThreads) rows_kernel(const Product<T> p) 
         if (m0 + m >= p.M || c0 + c >= p.N) continue;
         T v = T(0);
         for (int r = 0; r < ranks; r++) v += *cluster.map_shared_rank(sum + e, r);
-        finish(p, m0 + m, c0 + c, v);
+        finish(p, share.y, m0 + m, c0 + c, v);
     }
     cluster.sync();  // no rank leaves while its sums are read
 }
@@ -169,7 +194,8 @@ __device__ __forceinline__ void tile_product(const Product<T> &p, int64_t tile_m
     const int ranks = cluster.num_blocks(), rank = cluster.block_rank();
     const int tid = threadIdx.x, tx = tid % 16, ty = tid / 16;
     const int64_t n0 = tile_n * kTN, m0 = tile_m * kTM;
-    const int64_t k0 = p.K * rank / ranks, k1 = p.K * (rank + 1) / ranks;
+    const Share<T> share(p, rank, ranks);
+    const int64_t k0 = share.from, k1 = share.to;
     const int steps = (int)((k1 - k0 + TK - 1) / TK);
     // This thread copies PER values of each operand a step: of one stored along
     // K, one K of every ROWS-th row; of one stored across, every second K of a
@@ -289,7 +315,7 @@ __device__ __forceinline__ void tile_product(const Product<T> &p, int64_t tile_m
             act_values(p.act, v);
 #pragma unroll
             for (int i = 0; i < 8; i++)
-                if (in[i]) p.y[at[i]] = p.residual ? r_add(v[i], res[i]) : v[i];
+                if (in[i]) share.y[at[i]] = p.residual ? r_add(v[i], res[i]) : v[i];
         }
     }
     cluster.sync();
@@ -328,7 +354,7 @@ int launch_cluster(Kernel kernel, dim3 grid, int threads, size_t smem, int ranks
         J4C_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     if (ranks > 8) J4C_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid.x * ranks, grid.y);
+    cfg.gridDim = dim3(grid.x * ranks, grid.y, grid.z);
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
@@ -353,11 +379,48 @@ int ranks_for(int64_t tiles, int64_t K) {
     return ranks;
 }
 
+// Parts of a sum of K terms whose `ctas` CTAs have `adders` threads after one
+// another along K: so many that no thread adds more than kMaxTerms of them in a
+// row.  Each addition in FP32 loses up to half a step of the running sum, so the
+// error grows with the row: the weight's gradient of [4000000,8]x[8,8], values of
+// one sign, came out 1.4e-5 off from the 16 CTAs of one cluster (250000 terms a
+// thread) and 8e-8 in parts, and forward and gradients take 3.1 ms instead of
+// 13.6.  FLOAT64 has the digits to spare; there parts only fill idle SMs.
+constexpr int64_t kMaxTerms = 1024;
+template <typename T>
+int64_t parts_for(int64_t ctas, int64_t adders, int64_t K) {
+    int64_t parts = std::min<int64_t>(ceil_div(K, adders * kMaxTerms), 65535);
+    if (sizeof(T) == 8) parts = std::min(parts, 2 * sm_count() / std::max<int64_t>(ctas, 1));
+    return std::max<int64_t>(parts, 1);
+}
+
+template <typename T, typename Kernel>
+int launch_parts(Kernel kernel, dim3 grid, int threads, size_t smem, int ranks, int64_t parts, const Product<T> &p,
+                 cudaStream_t s) {
+    if (parts == 1) return launch_cluster(kernel, grid, threads, smem, ranks, p, s);
+    void *sums = nullptr;
+    if (int rc = scratch_alloc((size_t)(parts * p.M * p.N) * sizeof(T), &sums, s)) return rc;
+    grid.z = (unsigned)parts;
+    int rc = launch_cluster(kernel, grid, threads, smem, ranks,
+                            Product<T>{p.A, p.B, nullptr, nullptr, nullptr, (T *)sums, p.M, p.K, p.N, J4C_ACT_NONE}, s);
+    if (rc == J4C_OK) {
+        join_kernel<T><<<(unsigned)ceil_div(p.M * p.N, 32), 1024, 0, s>>>(p, (const T *)sums, parts);
+        count_launch();
+        const cudaError_t e = cudaGetLastError();
+        if (e != cudaSuccess) rc = cuda_status(e, "join_kernel");
+    }
+    const int freed = scratch_free(sums, s);
+    return rc ? rc : freed;
+}
+
 template <typename T, int MT, int V>
 int launch_rows(const Product<T> &p, cudaStream_t s) {
     constexpr size_t smem = std::max<size_t>(8 * MT * 32 * V, kRowsK * MT) * sizeof(T);
     const dim3 grid((unsigned)ceil_div(p.N, 32 * V), (unsigned)ceil_div(p.M, MT));
-    return launch_cluster(rows_kernel<T, MT, V>, grid, kRowsThreads, smem, ranks_for<T>((int64_t)grid.x * grid.y, p.K), p, s);
+    const int64_t strips = (int64_t)grid.x * grid.y;
+    const int ranks = ranks_for<T>(strips, p.K);
+    return launch_parts(rows_kernel<T, MT, V>, grid, kRowsThreads, smem, ranks,
+                        parts_for<T>(strips * ranks, ranks * (kRowsThreads / 32), p.K), p, s);
 }
 template <typename T, int V>
 int launch_rows_m(const Product<T> &p, cudaStream_t s) {
@@ -388,16 +451,18 @@ int small_product(const Product<T> &p, int ta, int tb, int ranks, cudaStream_t s
     }
     const int64_t tiles = tiles_of(p);
     if (!ranks) ranks = ranks_for<T>(tiles, p.K);
+    const int64_t parts = parts_for<T>(tiles * ranks, ranks, p.K);
     auto launch = [&](auto kernel) {
-        return launch_cluster(kernel, dim3((unsigned)tiles), kTileThreads, 0, ranks, p, s);
+        return launch_parts(kernel, dim3((unsigned)tiles), kTileThreads, 0, ranks, parts, p, s);
     };
     if (ta) return tb ? launch(tile_kernel<T, true, true>) : launch(tile_kernel<T, true, false>);
     return tb ? launch(tile_kernel<T, false, true>) : launch(tile_kernel<T, false, false>);
 }
 
 // x's and w's gradients, in one launch (a cut of K for both) unless that left
-// one of them more than 256 K a CTA that its own cut would not: the gradients of
-// [1839,2090]x[2090,6], dw with 1839 K, 191 us in one launch, 46 in two.  How K is
+// one of them more than 256 K a CTA that its own cut would not, or one comes in
+// parts: the gradients of [1839,2090]x[2090,6], dw with 1839 K, 191 us in one
+// launch, 46 in two.  How K is
 // cut depends on the layer's sizes alone, not on which of the two are wanted: the
 // same bits.
 template <typename T>
@@ -405,7 +470,8 @@ int gradients(const Product<T> &dx, const Product<T> &dw, bool dx_too, bool dw_t
     const int64_t tx = tiles_of(dx), tw = tiles_of(dw);
     const int both = ranks_for<T>(tx + tw, std::max(dx.K, dw.K));
     const int rx = ranks_for<T>(tx, dx.K), rw = ranks_for<T>(tw, dw.K);
-    const bool together = std::max(dx.K, dw.K) <= both * 256ll || (rx <= both && rw <= both);
+    const bool parts = parts_for<T>(tx * both, both, dx.K) > 1 || parts_for<T>(tw * both, both, dw.K) > 1;
+    const bool together = !parts && (std::max(dx.K, dw.K) <= both * 256ll || (rx <= both && rw <= both));
     if (together && dx_too && dw_too)
         return launch_cluster(two_products_kernel<T>, dim3((unsigned)(tx + tw)), kTileThreads, 0, both,
                               TwoProducts<T>{dx, dw, tx}, s);

@@ -13,18 +13,14 @@ __device__ __forceinline__ T warp_sum(T v) {
     return v;
 }
 
-// out[j] = sum over r of in[r, j], r < rows, for two [rows, cols] arrays back
-// to back (blockIdx.y; one array: a grid of one row): 32 columns and 32 lanes
-// of rows a CTA; either output may be NULL.
+// The sums over the rows r < rows of an array [rows, cols], 32 columns a CTA and
+// 32 lanes of rows (1024 threads): lane 0 of warp w gets that of column
+// 32 blockIdx.x + w.  Every thread of the CTA comes along.
 template <typename T>
-__global__ void __launch_bounds__(1024) sum_rows_kernel(const T *__restrict__ in, int64_t rows, int64_t cols, T *out0,
-                                                        T *out1) {
+__device__ __forceinline__ T column_sum(const T *__restrict__ in, int64_t rows, int64_t cols) {
     __shared__ T part[32][33];
     const int lane = threadIdx.x % 32, rl = threadIdx.x / 32;
     const int64_t c = (int64_t)blockIdx.x * 32 + lane;
-    T *out = blockIdx.y ? out1 : out0;
-    if (!out) return;
-    in += blockIdx.y * rows * cols;
     T v = T(0);
     if (c < cols) {
         int64_t r = rl;
@@ -39,9 +35,19 @@ __global__ void __launch_bounds__(1024) sum_rows_kernel(const T *__restrict__ in
     part[rl][lane] = v;
     __syncthreads();
     // the warp of a column adds the column's 32 lanes
-    v = warp_sum(part[lane][rl]);
-    const int64_t mine = (int64_t)blockIdx.x * 32 + rl;
-    if (lane == 0 && mine < cols) out[mine] = v;
+    return warp_sum(part[lane][rl]);
+}
+
+// out[j] = sum over r of in[r, j], r < rows, for two [rows, cols] arrays back
+// to back (blockIdx.y; one array: a grid of one row); either output may be NULL.
+template <typename T>
+__global__ void __launch_bounds__(1024) sum_rows_kernel(const T *__restrict__ in, int64_t rows, int64_t cols, T *out0,
+                                                        T *out1) {
+    T *out = blockIdx.y ? out1 : out0;
+    if (!out) return;
+    const T v = column_sum(in + blockIdx.y * rows * cols, rows, cols);
+    const int64_t mine = (int64_t)blockIdx.x * 32 + threadIdx.x / 32;
+    if (threadIdx.x % 32 == 0 && mine < cols) out[mine] = v;
 }
 
 }  // namespace
