@@ -2192,16 +2192,19 @@ int tc_gemm_act(const float *ah, const float *al, const float *bh, const float *
                 const float *bias, int act, const float *residual, float *z, float *y, cudaStream_t s) {
     J4C_REQUIRE(aligned16(ah) && aligned16(al) && aligned16(bh) && aligned16(bl),
                 "dot: split operands must be 16-byte aligned");
-    // Chunks of 128 K up to 2048, then 256 (a k-block holds 32 K under 3xFP16, 16
-    // under 3xTF32).  A chunk's truncation bias does not grow with K while the
+    // Chunks of 128 K up to 2048, then 256 under 3xFP16 (a k-block holds 32 K there,
+    // 16 under 3xTF32).  A chunk's truncation bias does not grow with K while the
     // error of an FP32 sum does, so the longer chunk is held against the larger
     // error: at K = 4096 the relative error is 9.3e-7, of a plain FP32 product
     // 1.15e-6; at 2048 with chunks of 128 it is 4.8e-7 and 5.7 to 8.1e-7.
     // Fewer chunks leave the epilogue's warps less to add: [8192,4096] .
-    // [4096,4096] gelu + residual 827 -> 806 us.
-    const int block = tc::split_fp16() ? 32 : 16;
+    // [4096,4096] gelu + residual 827 -> 806 us.  3xTF32 issues twice the MMAs for
+    // a K and has twice the bias (positive operands -2.4e-6 with 256, -1.1e-6 with
+    // 128 at every K; the plain product -1.4e-6 at 8192): it keeps 128.
+    const bool f16 = tc::split_fp16();
+    const int chunk_kb = f16 ? (K <= 2048 ? 128 : 256) / 32 : 128 / 16;
     const tc::Epilogue ep{bias, nullptr, y,   nullptr,  (int)M,
-                          nullptr, nullptr, nullptr, 0, act, residual, (K <= 2048 ? 128 : 256) / block};
+                          nullptr, nullptr, nullptr, 0, act, residual, chunk_kb};
     static const bool pair = [] {
         const char *v = getenv("J4C_GEMM_PAIR");
         return !(v && v[0] == '0');

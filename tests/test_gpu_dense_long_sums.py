@@ -84,3 +84,30 @@ def test_recorded_and_on_another_stream(J, shape, N):
             np.testing.assert_array_equal(a.numpy(), v)
     for gr in graphs:
         gr.release()
+
+
+@pytest.mark.parametrize("K", [1024, 4096, 8192])
+def test_product_bias(J, K):
+    """Positive operands, where the tensor cores' truncation cannot cancel: it is
+    a chunk's (the adds of chunks round to nearest), and a layer's chunks are no
+    longer than the plain product's, so its mean error is no larger either (5 % for
+    the mean's own noise)."""
+    import torch
+    g = torch.Generator(device="cuda")
+    g.manual_seed(K)
+    x, w = (torch.rand(*s, generator=g, device="cuda") for s in ((1024, K), (K, 1024)))
+    want = x.double() @ w.double()
+    arrays = [J.ConcreteNDArray(t, J.Shape(tuple(t.shape))) for t in (x, w)]
+    bias = lambda y: abs(((y.tensor().view(1024, 1024).double() - want) / want).mean().item())  # noqa: E731
+    assert bias(J.Nn.dense(*arrays)) <= 1.05 * bias(arrays[0].dot(arrays[1]))
+
+
+def test_product_bias_under_3xtf32():
+    import os
+    import subprocess
+    import sys
+    r = subprocess.run([sys.executable, "-m", "pytest", "-q", "-x", "tests/test_gpu_dense_long_sums.py", "-k",
+                        "test_product_bias and not tf32"], env={**os.environ, "J4C_GEMM_SPLIT": "tf32"},
+                       capture_output=True, text=True, timeout=600,
+                       cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert r.returncode == 0, r.stdout[-3000:] + r.stderr[-2000:]
