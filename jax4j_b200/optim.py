@@ -30,10 +30,10 @@ from .tracing import Tracer
 class _Leaf:
     """What a state remembers of a parameter: no reference to its values."""
 
-    __slots__ = ("shape", "dtype", "device", "size")
+    __slots__ = ("shape", "dtype", "size")
 
     def __init__(self, a: NDArray):
-        self.shape, self.dtype, self.device, self.size = a.shape(), a.dtype(), a.device(), a.shape().size()
+        self.shape, self.dtype, self.size = a.shape(), a.dtype(), a.shape().size()
 
 
 def _q8_words(n: int) -> int:
@@ -119,8 +119,9 @@ class AdamWState:
         call("j4c_adamw_moments", n, (C.c_int64 * n)(*[l.size for l in ls]), _pointers(self._arrays),
              (C.c_void_p * n)(*[t.data_ptr() for t in out[:n]]), (C.c_void_p * n)(*[t.data_ptr() for t in out[n:]]),
              stream)
-        trees = [PyTrees.unflatten(self._tree, [ConcreteNDArray._wrap(t, l.shape, DType.FLOAT32, l.device)
-                                                for t, l in zip(part, ls)]) for part in (out[:n], out[n:])]
+        trees = [PyTrees.unflatten(self._tree, [ConcreteNDArray._wrap(t, l.shape, DType.FLOAT32, a._device)
+                                                for t, l, a in zip(part, ls, self._arrays)])
+                 for part in (out[:n], out[n:])]
         return trees[0], trees[1]
 
 

@@ -119,3 +119,45 @@ def test_c_entries_refuse_bad_arguments():
         assert rc == _lib.E_INVALID and text in msg, (kw, rc, msg)
     rc = L.j4c_adamw_moments(1, n, one, null, one, None)
     assert rc == _lib.E_INVALID and "NULL pointer" in L.j4c_last_error().decode()
+
+
+class GpuTensor:
+    """Stands in for a tensor on GPU `gpu` where no kernel runs."""
+
+    def __init__(self, gpu):
+        self.device = torch.device("cuda", gpu)
+
+    def get_device(self):
+        return self.device.index
+
+    def data_ptr(self):
+        return 0x1000
+
+    def to(self, device):
+        return GpuTensor(device.index)
+
+
+def on_gpu(gpu, n, dtype=J.DType.FLOAT32):
+    return J.ConcreteNDArray._wrap(GpuTensor(gpu), J.Shape(n), dtype, J.Device.cuda(gpu))
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_moments_lie_where_the_state_does(monkeypatch, bits):
+    """The moments of a state whose arrays were moved carry the arrays' device, not
+    that of the parameters the state was made for."""
+    from jax4j_b200 import optim
+    monkeypatch.setattr(optim, "call", lambda *a: None)
+    monkeypatch.setattr(optim, "stream_of", lambda ordinal: 0)
+    monkeypatch.setattr(optim, "_carve", lambda sizes, dtype, device: [GpuTensor(device.index) for _ in sizes])
+    p = tree(on_gpu(0, 5), on_gpu(0, 200))
+
+    def arrays(gpu):
+        moments = ([on_gpu(gpu, 66, J.DType.INT32), on_gpu(gpu, 132, J.DType.INT32)] if bits == 8 else
+                   [on_gpu(gpu, n) for n in (5, 5, 200, 200)])
+        return [on_gpu(gpu, 3, J.DType.FLOAT64)] + moments
+
+    first = arrays(0)
+    moved = J.AdamWState(p, bits, first[0], first[1:]).withArrays(arrays(1))
+    for part in moved.moments():
+        for a in J.PyTrees.flatten(part):
+            assert a.device() is J.Device.cuda(1) and a.tensor().device.index == 1
