@@ -422,11 +422,22 @@ class Lax:
         all-reduce: Optim.adamW of psumTree(grads), with scale = 1/D for the
         mean gradient; `hyper` are Optim.adamW's other arguments.  Every shard
         holds the same summed gradients, so every shard computes the same new
-        parameters and state.  Returns (new parameters, new state)."""
+        parameters and state.  Returns (new parameters, new state).
+
+        The shards of a pmap may share one `state` (and one `lr` array): on a
+        shard whose parameters lie on another GPU it is copied there first
+        (AdamWState.to), at every step that is given it.  A program that hands each shard its own last new
+        state makes no copy."""
         from .optim import Optim
         pl, gl = PyTrees.flatten(params), PyTrees.flatten(grads)
         if len(pl) != len(gl):
             raise IllegalArgumentException(f"psumAdamWTree: {len(pl)} parameters but {len(gl)} gradients")
+        if pl and isinstance(pl[0], ConcreteNDArray):
+            gpu = pl[0].tensor().get_device()
+            if any(a.tensor().get_device() != gpu for a in state.arrays()):
+                state = state.to(pl[0].device())
+            if isinstance(lr, ConcreteNDArray) and lr.tensor().get_device() != gpu:
+                lr = lr.to(pl[0].device())
         return Optim.adamW(params, Lax.psumTree(grads), state, lr, scale=scale, **hyper)
 
 

@@ -103,6 +103,11 @@ class AdamWState:
             raise IllegalArgumentException("AdamW: the arrays do not match those of the state")
         return AdamWState.__new__(AdamWState)._set(self._tree, self._leaves, self._bits, arrays[0], arrays[1:])
 
+    def to(self, device: Device) -> "AdamWState":
+        """This state on `device` (ConcreteNDArray.to for every array: copied
+        only if the device is another GPU)."""
+        return self.withArrays([a.to(device) for a in self.arrays()])
+
     def moments(self) -> Tuple[PyTree, PyTree]:
         """(m, v) as trees of the parameters' shapes; for 8-bit moments the
         FLOAT32 values that the codes stand for, one launch for all leaves."""

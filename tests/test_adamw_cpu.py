@@ -161,3 +161,26 @@ def test_moments_lie_where_the_state_does(monkeypatch, bits):
     for part in moved.moments():
         for a in J.PyTrees.flatten(part):
             assert a.device() is J.Device.cuda(1) and a.tensor().device.index == 1
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_shared_state_goes_where_the_shard_is(monkeypatch, bits):
+    """Lax.psumAdamWTree on a shard of another GPU than the state's takes the step
+    with the state beside the shard's parameters; on the state's own GPU with the
+    state itself."""
+    seen, lrs = [], []
+    monkeypatch.setattr(J.Optim, "adamW", lambda params, grads, state, lr, **k: seen.append(state) or lrs.append(lr))
+    monkeypatch.setattr(J.Lax, "psumTree", lambda grads: grads)
+    p = tree(on_gpu(0, 5))
+    moments = [on_gpu(0, 66, J.DType.INT32)] if bits == 8 else [on_gpu(0, 5), on_gpu(0, 5)]
+    state = J.AdamWState(p, bits, on_gpu(0, 3, J.DType.FLOAT64), moments)
+    lr = on_gpu(0, 1)
+    J.Lax.psumAdamWTree(p, p, state, lr)
+    other = tree(on_gpu(1, 5))
+    J.Lax.psumAdamWTree(other, other, state, lr)
+    assert seen[0] is state and lrs[0] is lr and lrs[1].tensor().device.index == 1
+    for a in seen[1].arrays():
+        assert a.device() is J.Device.cuda(1) and a.tensor().device.index == 1
+    assert seen[1].stateBits() == bits and [a.dtype() for a in seen[1].arrays()] == [a.dtype() for a in state.arrays()]
+    back = seen[1].to(J.Device.cuda(0))
+    assert all(a.device() is J.Device.cuda(0) and a.tensor().device.index == 0 for a in back.arrays())

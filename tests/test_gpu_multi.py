@@ -128,3 +128,39 @@ def test_psum_sgd_wait_runs_out_with_a_status(tmp_path):
     r = _torchrun("psum_sgd_timeout", out, {"NCCL_NVLS_ENABLE": "0"})
     assert r.returncode == 0, r.stderr[-2000:]
     assert int(open(out).read()) == 0x7C05
+
+
+@needs2
+@pytest.mark.parametrize("bits", [8, 32])
+def test_in_process_data_parallel_adamw(bits):
+    """Shards on two GPUs that share one AdamW state: each ends, on its own GPU,
+    with the step of the summed gradients, twice in a row."""
+    import jax4j_b200 as J
+    devices = [J.Device.cuda(0), J.Device.cuda(1)]
+    r = np.random.default_rng(3)
+    w = r.standard_normal((33, 20)).astype(np.float32)
+    x = r.standard_normal((2, 8, 33)).astype(np.float32)
+    params = J.PyTree.dictOf({"w": J.ConcreteNDArray.of(w)})
+    state = J.Optim.adamWInit(params, bits)
+    new = {}
+
+    def loss(p, xs):
+        return xs.dot(p.children["w"].value).tanh().sum()
+
+    def body(xs):
+        xs = xs.to(xs.device())
+        p, s = new.get(xs.device()) or (J.PyTrees.map(lambda a: a.to(xs.device()), params), state)
+        v, grads = J.JAX.valueAndGradTree(lambda q: loss(q, xs))(p)
+        new[xs.device()] = J.Lax.psumAdamWTree(p, grads, s, 1e-2, scale=0.5)
+        return v
+
+    p, s = params, state
+    for _ in range(2):
+        J.JAX.pmap(body, devices)(J.ConcreteNDArray.of(x))
+        gs = [J.JAX.gradTree(lambda q, i=i: loss(q, J.ConcreteNDArray.of(x[i])))(p) for i in range(2)]
+        p, s = J.Optim.adamW(p, J.PyTrees.map2(lambda a, b: a.add(b), *gs), s, 1e-2, scale=0.5)
+        for d in devices:
+            got, st = new[d]
+            for a, b in zip([*J.PyTrees.flatten(got), *st.arrays()], [*J.PyTrees.flatten(p), *s.arrays()]):
+                assert a.device() is d and a.tensor().device.index == d.ordinal()
+                np.testing.assert_array_equal(a.numpy(), b.numpy())
