@@ -739,7 +739,8 @@ int j4c_dense_backward(int dtype, const void *x, const void *w, int64_t M, int64
     J4C_REQUIRE(dtype == J4C_FLOAT32 || dtype == J4C_FLOAT64, "j4c_dense_backward requires FLOAT32 or FLOAT64 arrays, got %s",
                 dtype_name(dtype));
     J4C_REQUIRE(M >= 0 && K >= 0 && N >= 0, "j4c_dense_backward: negative dimension");
-    J4C_REQUIRE(dx || dw || K == 0 || (M == 0 && N == 0),
+    // (an empty gradient's pointer is NULL too)
+    J4C_REQUIRE(dx || dw || M == 0 || K == 0 || N == 0,
                 "j4c_dense_backward: neither product is wanted (j4c_dense_grad gives dbias alone)");
     const void *d = dy;
     if (dbias || act != J4C_ACT_NONE) {

@@ -116,3 +116,12 @@ def test_c_entries_refuse_bad_arguments():
     assert rc == _lib.E_INVALID and "workspace" in L.j4c_last_error().decode()
     rc = L.j4c_group_norm_grad(0, 2, 3, 8, 2, fake, None, None, 0, fake, None, fake, fake, None, None, fake, 1 << 20, None)
     assert rc == _lib.E_INVALID and "NULL" in L.j4c_last_error().decode()
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("M,K,N", [(0, 3, 4), (2, 0, 4), (2, 3, 0), (0, 0, 4), (0, 3, 0)])
+def test_empty_gradients_are_no_refusal(dtype, M, K, N):
+    """The pointer of an empty array is NULL, as that of a gradient that is not wanted."""
+    fake = C.c_void_p(0x1000)
+    rc = _lib.lib().j4c_dense_backward(dtype, fake, fake, M, K, N, fake, None, 0, 0, None, None, None, None, None, 0, None)
+    assert rc == _lib.OK, _lib.lib().j4c_last_error()
