@@ -263,7 +263,7 @@ def _run_equation(eq, values: Dict[int, NDArray], keep_for_vjp: bool = False) ->
     inputs = [values[v.id] for v in eq.inputs]
     if eq.primitive == Primitive.FFI_CALL:
         out = eq.outputs[0].id
-        values[out], saved = eq.metadata.forward(inputs, keep_for_vjp)
+        values[out], saved = eq.metadata.run(inputs, keep_for_vjp)
         if saved is not None:
             values[~out] = saved  # for its VJP, under an id no Var has
         return
@@ -545,8 +545,8 @@ def _layer_backward(jaxpr: Jaxpr, values: Dict[int, NDArray], seed: NDArray) -> 
     """do_backward of a Jaxpr that is one FFI_CALL and its output."""
     eq = jaxpr.equations[0]
     ids = [v.id for v in jaxpr.inVars]
-    g_ins = eq.metadata.vjp([values[v.id] for v in eq.inputs], values[eq.outputs[0].id], values.get(~eq.outputs[0].id),
-                            materialize(seed), [v.id in ids for v in eq.inputs])
+    g_ins = eq.metadata.pull([values[v.id] for v in eq.inputs], values[eq.outputs[0].id], values.get(~eq.outputs[0].id),
+                             materialize(seed), [v.id in ids for v in eq.inputs])
     grads: Dict[int, NDArray] = {}
     for v, g in zip(eq.inputs, g_ins):
         if g is not None:
@@ -626,7 +626,7 @@ def _process_backward_eq(eq, values, grads, need, fused_relu) -> None:
     inputs = [values.get(v.id) for v in eq.inputs]
     out_value = values.get(eq.outputs[0].id)
     if eq.primitive == Primitive.FFI_CALL:
-        g_ins = eq.metadata.vjp(inputs, out_value, values.get(~eq.outputs[0].id), materialize(g_out), wanted)
+        g_ins = eq.metadata.pull(inputs, out_value, values.get(~eq.outputs[0].id), materialize(g_out), wanted)
     else:
         g_ins = compute_vjps(eq.primitive, eq, g_out, inputs, out_value, wanted)
     for v, w, g in zip(eq.inputs, wanted, g_ins):
@@ -694,7 +694,7 @@ def execute_primitive(p: Primitive, eq, inputs: List[NDArray]) -> NDArray:
         m: CheckpointMeta = eq.metadata
         return forward_interpret(m.subJaxpr, [inputs[0]])[0]
     if p == Primitive.FFI_CALL:
-        return eq.metadata.forward(inputs, False)[0]
+        return eq.metadata.run(inputs, False)[0]
     raise UnsupportedOperationException(str(p))
 
 

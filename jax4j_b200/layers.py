@@ -10,15 +10,16 @@ jit, scan and checkpoint compose with it as with any other equation.
 from __future__ import annotations
 
 import functools
+import math
 from typing import List, Optional
 
 import torch
 
 from . import _lib
 from ._lib import call
-from .core import (ConcreteNDArray, DType, IllegalArgumentException, NDArray, Primitive, Shape,
-                   UnsupportedOperationException, _make_splits, _split_of)
-from .tracing import Equation, FfiMeta, TracedNDArray, Tracer, to_var
+from .core import (ConcreteNDArray, DType, IllegalArgumentException, NDArray, Shape, UnsupportedOperationException,
+                   _make_splits, _split_of)
+from .tracing import FfiMeta
 
 # J4C_ACT_* (include/jax4j_cuda.h)
 ACTIVATIONS = {"none": 0, "relu": 1, "tanh": 2, "sigmoid": 3, "silu": 4, "gelu": 5}
@@ -29,15 +30,6 @@ def activation_code(name: Optional[str]) -> int:
     if code is None:
         raise IllegalArgumentException(f"unknown activation {name!r}: one of {', '.join(ACTIVATIONS)}")
     return code
-
-
-def _apply(meta: FfiMeta, inputs: List[NDArray], out_shape: Shape) -> NDArray:
-    """The layer's equation under a trace."""
-    tracer = Tracer.current()
-    in_vars = [to_var(x) for x in inputs]
-    out = tracer.nextVar(out_shape, in_vars[0].dtype)
-    tracer.addEquation(Equation(in_vars, [out], Primitive.FFI_CALL, meta))
-    return TracedNDArray(out)
 
 
 def _device_of(inputs: List[ConcreteNDArray]):
@@ -81,30 +73,27 @@ def group_norm(x: NDArray, groups: int, gamma: Optional[NDArray], beta: Optional
     if not eps >= 0.0:
         raise IllegalArgumentException(f"groupNorm: eps is not negative, got {eps}")
     inputs = [x] + [p for p in (gamma, beta) if p is not None]
-    meta = _GroupNorm(groups, gamma is not None, beta is not None, float(eps), act)
-    if Tracer.current() is None:
-        return meta.forward(inputs, False)[0]
-    return _apply(meta, inputs, x.shape())
+    return _GroupNorm(groups, gamma is not None, beta is not None, float(eps), act).run(inputs, False)[0]
 
 
 class _GroupNorm(FfiMeta):
     name = "group_norm"
 
-    def __init__(self, groups: int, has_gamma: bool, has_beta: bool, eps: float, act: int):
+    def __init__(self, groups: int, has_gamma: bool, has_beta: bool, eps: float, act: int, sample_axes: int = 1):
         self.groups, self.has_gamma, self.has_beta, self.eps, self.act = groups, has_gamma, has_beta, eps, act
+        self.sample_axes = sample_axes  # leading axes that count samples: 1 and those that vmap adds
+
+    def outShape(self, inputs):
+        return inputs[0].shape()
 
     def _params(self, inputs):
         gamma = inputs[1] if self.has_gamma else None
         beta = inputs[-1] if self.has_beta else None
         return gamma, beta
 
-    @staticmethod
-    def _extents(shape: Shape):
-        d = shape.dimensions()
-        S = 1
-        for n in d[1:-1]:
-            S *= n
-        return d[0], S, d[-1]
+    def _extents(self, shape: Shape):
+        d, lead = shape.dimensions(), self.sample_axes
+        return math.prod(d[:lead]), math.prod(d[lead:-1]), d[-1]
 
     def forward(self, inputs, keep):
         x = inputs[0]
@@ -154,10 +143,8 @@ class _GroupNorm(FfiMeta):
         if not batched[0] or any(batched[1:]):
             raise UnsupportedOperationException("vmap of groupNorm batches x alone")
         # examples are samples side by side
-        x = inputs[0]
-        d = x.shape().dimensions()
-        y = self.forward([x.reshape(Shape((d[0] * d[1],) + d[2:]))] + list(inputs[1:]), False)[0]
-        return y.reshape(x.shape())
+        return _GroupNorm(self.groups, self.has_gamma, self.has_beta, self.eps, self.act,
+                          self.sample_axes + 1).run(inputs, False)[0]
 
 
 # ---------------------------------------------------------------------------
@@ -198,10 +185,7 @@ def dense(x: NDArray, w: NDArray, bias: Optional[NDArray], activation: Optional[
         if residual.shape()._d != out:
             raise IllegalArgumentException(f"dense: residual is {residual.shape()}, the output {Shape(out)}")
         inputs.append(residual)
-    meta = _dense_meta(bias is not None, residual is not None, act)
-    if Tracer.current() is None:
-        return meta.forward(inputs, False)[0]
-    return _apply(meta, inputs, Shape(out))
+    return _dense_meta(bias is not None, residual is not None, act).run(inputs, False)[0]
 
 
 def _split_product(a, a_kind: str, b, b_kind: str, M: int, K: int, N: int, bias, act: int, residual, z, out: torch.Tensor,
@@ -218,6 +202,9 @@ class _Dense(FfiMeta):
 
     def __init__(self, has_bias: bool, has_residual: bool, act: int):
         self.has_bias, self.has_residual, self.act = has_bias, has_residual, act
+
+    def outShape(self, inputs):
+        return Shape(inputs[0].shape()._d[:-1] + inputs[1].shape()._d[1:])
 
     def _params(self, inputs):
         return inputs[2] if self.has_bias else None, inputs[-1] if self.has_residual else None
@@ -318,7 +305,7 @@ class _Dense(FfiMeta):
         # x alone, or x and the residual: examples are rows side by side
         if not batched[0] or batched[1] or (self.has_bias and batched[2]) or (self.has_residual and not batched[-1]):
             raise UnsupportedOperationException("vmap of dense batches x, together with the residual")
-        return self.forward(inputs, False)[0]
+        return self.run(inputs, False)[0]
 
 
 @functools.lru_cache(maxsize=None)

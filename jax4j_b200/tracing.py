@@ -71,14 +71,38 @@ class FfiMeta:
     """An FFI_CALL's function and its VJP (the pair api/FFI.java:17-31
     registers by name).  Instances hold parameters, never arrays.
 
+    outShape(inputs): the output's shape (its dtype is the first input's).
     forward(inputs, keep) -> (output, saved): saved is what vjp needs beside
     the inputs and the output, made only where keep is true.
     vjp(inputs, output, saved, g, wanted) -> one cotangent per input (None
     where wanted is false).
     batch(inputs, batched, batch): the function over a leading axis of the
-    batched inputs (JAX.vmap)."""
+    batched inputs (JAX.vmap).
+
+    A transformation calls run and pull, which under a trace record the call
+    (as any other operation's interpretation there records it) and refuse."""
 
     name = "?"
+
+    def run(self, inputs, keep):
+        if Tracer.current() is not None:
+            return self.record(inputs), None
+        return self.forward(inputs, keep)
+
+    def record(self, inputs) -> "TracedNDArray":
+        tracer = Tracer.current()
+        in_vars = [to_var(x) for x in inputs]
+        out = tracer.nextVar(self.outShape(inputs), in_vars[0].dtype)
+        tracer.addEquation(Equation(in_vars, [out], Primitive.FFI_CALL, self))
+        return TracedNDArray(out)
+
+    def pull(self, inputs, out, saved, g, wanted):
+        if Tracer.current() is not None:
+            raise UnsupportedOperationException(f"the gradient of {self.name} cannot be taken inside a trace")
+        return self.vjp(inputs, out, saved, g, wanted)
+
+    def outShape(self, inputs) -> Shape:
+        raise NotImplementedError
 
     def forward(self, inputs, keep):
         raise NotImplementedError

@@ -151,7 +151,7 @@ def _rule(eq, inputs: List[NDArray], batched: List[bool], batch: int) -> NDArray
         from .grad import take_eager
         return take_eager(inputs[0], inputs[1])
     if p == P.FFI_CALL:
-        return m.batch(inputs, batched, batch) if any(batched) else m.forward(inputs, False)[0]
+        return m.batch(inputs, batched, batch) if any(batched) else m.run(inputs, False)[0]
     if p == P.CHECKPOINT:
         # the rematerialisation hint is a no-op under vmap: batch the body inline
         return run(m.subJaxpr, [inputs[0]], [batched[0]], batch)

@@ -125,3 +125,38 @@ def test_empty_gradients_are_no_refusal(dtype, M, K, N):
     fake = C.c_void_p(0x1000)
     rc = _lib.lib().j4c_dense_backward(dtype, fake, fake, M, K, N, fake, None, 0, 0, None, None, None, None, None, 0, None)
     assert rc == _lib.OK, _lib.lib().j4c_last_error()
+
+
+def _layers():
+    w, b = leaf(8, 5), leaf(5)
+    return {"dense": (lambda a: J.Nn.dense(a, w, b, "silu"), (8,), (5,)),
+            "residual": (lambda a: J.Nn.dense(a, leaf(8, 8), None, "gelu", a), (2, 8), (2, 8)),
+            "group norm": (lambda a: J.Nn.groupNorm(a, 2, leaf(8), activation="tanh"), (2, 3, 8), (2, 3, 8))}
+
+
+@pytest.mark.parametrize("name", ["dense", "residual", "group norm"])
+def test_vmap_inside_a_trace_is_recorded(name):
+    """As vmap of elementwise operations is: jit and grad of a mapped layer, and vmap of vmap."""
+    f, shape, out = _layers()[name]
+    for maps in (1, 2):
+        g = f
+        for _ in range(maps):
+            g = J.JAX.vmap(g)
+        lead = (4, 6)[:maps]
+        jaxpr = J.JAX.make_jaxpr(lambda a: g(a).tanh(), leaf(*lead, *shape))
+        assert [e.primitive for e in jaxpr.equations] == [J.Primitive.FFI_CALL, J.Primitive.TANH]
+        assert jaxpr.outVars[0].shape == J.Shape(*lead, *out)
+        if name == "group norm":  # every example's samples keep their own groups
+            assert jaxpr.equations[0].metadata._extents(J.Shape(*lead, *shape)) == (2 * 4 * (6 if maps == 2 else 1), 3, 8)
+
+
+@pytest.mark.parametrize("name", ["dense", "residual", "group norm"])
+def test_interpretation_inside_a_trace_is_recorded_and_gradients_refused(monkeypatch, name):
+    from jax4j_b200 import grad
+    f, shape, out = _layers()[name]
+    inner = J.JAX.make_jaxpr(f, leaf(*shape))
+    outer = J.JAX.make_jaxpr(lambda a: grad.forward_interpret(inner, [a])[0], leaf(*shape))
+    assert [e.primitive for e in outer.equations] == [J.Primitive.FFI_CALL] and outer.outVars[0].shape == J.Shape(*out)
+    monkeypatch.setattr(grad, "ones", lambda s, dtype, device=None: leaf(*s.dimensions()))
+    with pytest.raises(J.UnsupportedOperationException, match="inside a trace"):
+        J.JAX.make_jaxpr(lambda a: J.JAX.grad(f)(a), leaf(*shape))
