@@ -46,3 +46,66 @@ def test_mapped_layers_under_jit_grad_and_vmap(J, monkeypatch, name, small):
         np.testing.assert_array_equal(two(X5).numpy().reshape(12, 4, 32), halves.numpy())
         np.testing.assert_array_equal(J.JAX.grad(loss(two))(X5).numpy().reshape(12, 4, 32),
                                       J.JAX.grad(loss(f))(arr(J, x.reshape(12, 4, 32))).numpy())
+
+
+@pytest.mark.parametrize("small", [True, False])
+@pytest.mark.parametrize("name", ["dense", "group norm"])
+def test_scan_and_its_gradients(J, monkeypatch, name, small):
+    """A carry through five steps of a layer: eager, traced and recorded scans, and
+    both gradients, are those of the steps written out."""
+    from jax4j_b200 import layers as L
+    monkeypatch.setattr(L, "SMALL_PRODUCT", L.SMALL_PRODUCT if small else 0)
+    f = layers(J)[name]
+    r = np.random.default_rng(7)
+    x, c = r.standard_normal((5, 20, 32)).astype(np.float32), r.standard_normal((20, 32)).astype(np.float32)
+    X, C = arr(J, x), arr(J, c)
+    X1 = arr(J, x, 1)  # its slices lie off every 16-byte boundary
+
+    def step(carry, xt):
+        h = f(carry.add(xt))
+        return h, h.tanh()
+
+    def steps(carry, xs):
+        ys = []
+        for t in range(5):
+            carry, y = step(carry, arr(J, xs.numpy()[t]))
+            ys.append(y.numpy())
+        return carry.numpy(), np.stack(ys)
+
+    carry, ys = steps(C, X)
+    for xs in (X, X1):
+        out = J.Lax.scan(step, C, xs)
+        np.testing.assert_array_equal(out.carry().numpy(), carry)
+        np.testing.assert_array_equal(out.ys().numpy(), ys)
+        traced = J.JAX.jit(lambda a: J.Lax.scan(step, C, a).ys())
+        np.testing.assert_array_equal(traced(xs).numpy(), ys)
+    loss = lambda cc, xx: J.Lax.scan(step, cc, xx).ys().sum()  # noqa: E731
+    gc, gx = J.JAX.gradBoth(loss)(C, X)
+    parts = [arr(J, x[t]) for t in range(5)]
+
+    def written_out(*a):
+        carry, total = a[0], None
+        for t in range(5):
+            carry, y = step(carry, a[1 + t])
+            total = y.sum() if total is None else total.add(y.sum())
+        return total
+
+    _, pull = J.JAX.vjp(written_out, C, *parts)
+    grads = pull(J.ConcreteNDArray.scalar(1.0))
+    # the same products; a carry's two cotangents are added in either order
+    np.testing.assert_allclose(gc.numpy(), grads[0].numpy(), rtol=1e-5, atol=1e-6)
+    np.testing.assert_allclose(gx.numpy(), np.stack([g.numpy() for g in grads[1:]]), rtol=1e-5, atol=1e-6)
+
+
+@pytest.mark.parametrize("name", ["dense", "group norm"])
+def test_cond_takes_the_branch_and_its_gradient(J, name):
+    f = layers(J)[name]
+    x = arr(J, np.random.default_rng(8).standard_normal((3, 4, 32)).astype(np.float32))
+    other = lambda a: a.mul(a)  # noqa: E731
+    for yes in (1.0, 0.0):
+        pred = J.ConcreteNDArray.scalar(yes)
+        branch = f if yes else other
+        net = lambda a: J.Lax.cond(pred, f, other, a)  # noqa: E731,B023
+        np.testing.assert_array_equal(J.JAX.jit(net)(x).numpy(), branch(x).numpy())
+        np.testing.assert_array_equal(J.JAX.grad(lambda a: net(a).tanh().sum())(x).numpy(),  # noqa: B023
+                                      J.JAX.grad(lambda a: branch(a).tanh().sum())(x).numpy())  # noqa: B023
