@@ -598,7 +598,7 @@ struct Column {
             bt[e] = a.beta ? a.beta[c + e] : T(0);
         }
     }
-    // x <- xhat, d <- du, for a batch of x and dy (rows behind the tile: d is 0)
+    // x <- xhat, d <- du, for a batch of x and dy
     __device__ __forceinline__ void du(int act, T (&x)[8], T (&d)[8]) const {
 #pragma unroll
         for (int i = 0; i < 8; i++) x[i] = (x[i] - mean) * rstd;
@@ -635,13 +635,14 @@ __global__ void __launch_bounds__(kTileThreads, 2) tile_sums_kernel(const Args<T
                 const int64_t at = base + r * q.C + j * V;
                 T x[N], d[N];
                 load_rows<WHOLE, T, V>(x, a.x + at, pitch, rows);
-                load_rows<WHOLE, T, V>(d, a.dy + at, pitch, rows);  // zeros behind the tile
+                load_rows<WHOLE, T, V>(d, a.dy + at, pitch, rows);
                 k.du(a.act, x, d);
 #pragma unroll
-                for (int i = 0; i < N; i++) {
-                    s1[i % V] += d[i];
-                    s2[i % V] += WHOLE || i / V < rows ? d[i] * x[i] : T(0);
-                }
+                for (int i = 0; i < N; i++)
+                    if (WHOLE || i / V < rows) {  // behind the tile x is 0, which may lie at infinity from the mean
+                        s1[i % V] += d[i];
+                        s2[i % V] += d[i] * x[i];
+                    }
             });
 #pragma unroll
             for (int e = 0; e < V; e++) {
