@@ -661,7 +661,7 @@ J4C_API int j4c_psum_sgd(const float *const *grads, const float *const *upd, uin
  * each, a value being its code times its step; first all codes of m, then of
  * sqrt(v), then the steps of m, then of sqrt(v).  A moment that is not finite
  * is held as NaN; the update uses the moments before they are rounded (its
- * quotient within 2 ulp).
+ * quotient within 2 ulp; eps is 0 or from 2^-126 to 2^125).
  * Outputs may be the inputs of the same index (an update in place), else must
  * not overlap them.  Tensors of no elements may have NULL pointers. */
 J4C_API int64_t j4c_adamw_q8_words(int64_t n);

@@ -88,8 +88,9 @@ __device__ __forceinline__ double r_sqrt(double x) { return __dsqrt_rn(x); }
 // r_div without its shortcut for zero dividends, which are rare here
 __device__ __forceinline__ float q_div(float a, float b) { return __fdiv_rn(a, b); }
 __device__ __forceinline__ double q_div(double a, double b) { return __ddiv_rn(a, b); }
-// Within 2 ulp for divisors below 2^126 and 0 above (the divisor is a root, at
-// most 2^64, times b, plus eps): no branch, so eight of them overlap.
+// Within 2 ulp for divisors of 2^-126 to 2^126, and x / 0 as it should be: the
+// divisor is a root, 0 or from 2^-75 to 2^64, times b (1 to 2^27), plus eps, which
+// the call checks.  No branch, so eight of them overlap.
 __device__ __forceinline__ float fast_div(float a, float b) { return __fdividef(a, b); }
 
 // What a step needs beside the elements, in the elements' type.
@@ -553,6 +554,8 @@ int j4c_adamw_step(int dtype, int state_bits, int ntensors, const int64_t *numel
     J4C_REQUIRE(steps && steps != steps_out, "j4c_adamw_step: steps is NULL or steps_out");
     J4C_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, "j4c_adamw_step: betas lie in [0, 1)");
     J4C_REQUIRE(eps >= 0.0, "j4c_adamw_step: negative eps");
+    J4C_REQUIRE(state_bits == 32 || eps == 0.0 || (eps >= 0x1p-126 && eps <= 0x1p125),
+                "j4c_adamw_step: with 8-bit moments eps is 0 or from 2^-126 to 2^125, got %g", eps);
     const int per = state_bits == 8 ? 1 : 2;
     for (int i = 0; i < ntensors; i++) {
         J4C_REQUIRE(numel[i] >= 0, "j4c_adamw_step: tensor %d has a negative size", i);

@@ -204,6 +204,8 @@ class Optim:
             raise IllegalArgumentException(f"adamW: betas lie in [0, 1), got {beta1} and {beta2}")
         if not eps >= 0.0:
             raise IllegalArgumentException(f"adamW: eps is not negative, got {eps}")
+        if state._bits == 8 and eps and not 2.0 ** -126 <= eps <= 2.0 ** 125:
+            raise IllegalArgumentException(f"adamW: with 8-bit moments eps is 0 or from 2^-126 to 2^125, got {eps}")
         wd = [float(x) for x in weightDecay] if isinstance(weightDecay, (list, tuple)) else [float(weightDecay)] * n
         if len(wd) != n:
             raise IllegalArgumentException(f"adamW: {len(wd)} weight decays for {n} parameters")

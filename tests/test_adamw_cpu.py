@@ -184,3 +184,19 @@ def test_a_shared_state_goes_where_the_shard_is(monkeypatch, bits):
     assert seen[1].stateBits() == bits and [a.dtype() for a in seen[1].arrays()] == [a.dtype() for a in state.arrays()]
     back = seen[1].to(J.Device.cuda(0))
     assert all(a.device() is J.Device.cuda(0) and a.tensor().device.index == 0 for a in back.arrays())
+
+
+def test_eps_that_the_8_bit_quotient_does_not_take():
+    """It is off beyond 2^-126 and 2^126, where a divisor may be eps alone."""
+    p = tree(leaf(6))
+    L = _lib.lib()
+    fake, n, wd = C.c_void_p(0x1000), (C.c_int64 * 1)(0), (C.c_double * 1)(0.0)
+    one = (C.c_void_p * 1)(None)
+    for eps in (2.0 ** -127, 1e-40, 5e-324, 2.0 ** 126, float("inf")):
+        with pytest.raises(J.IllegalArgumentException, match="8-bit moments eps"):
+            J.Optim.adamW(p, p, state(p, 8), 0.1, eps=eps)
+        rc = L.j4c_adamw_step(0, 8, 1, n, one, one, one, one, one, wd, fake, None, None, 0.1, 1.0, 0.9, 0.999, eps, None)
+        assert rc == _lib.E_INVALID and "eps" in L.j4c_last_error().decode()
+    for eps in (0.0, 2.0 ** -126, 1e-8, 2.0 ** 125):  # an empty tensor: nothing is launched
+        rc = L.j4c_adamw_step(0, 8, 1, n, one, one, one, one, one, wd, fake, None, None, 0.1, 1.0, 0.9, 0.999, eps, None)
+        assert rc == _lib.OK, L.j4c_last_error()
