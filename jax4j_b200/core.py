@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import enum
 import functools
+import math
 import threading
 from typing import Optional, Sequence
 
@@ -156,10 +157,7 @@ class Shape:
         return len(self._d)
 
     def size(self) -> int:
-        s = 1
-        for d in self._d:
-            s *= d
-        return s
+        return math.prod(self._d)
 
     @staticmethod
     def broadcast(a: "Shape", b: "Shape") -> "Shape":
@@ -395,15 +393,13 @@ class ConcreteNDArray(NDArray):
         if device is None:
             device = Device._default or Device.defaultDevice()
         if isinstance(data, torch.Tensor):
-            t = data
+            t, kind = data, data.dtype
             if dtype is None:
-                dtype = _OF_TORCH.get(t.dtype) or _from_torch(t.dtype)
-            if t.dtype is not dtype.torch or t.get_device() != device.ordinal():  # -1: not on a GPU
+                dtype = _OF_TORCH.get(kind) or _from_torch(kind)
+            if kind is not dtype.torch or t.get_device() != device.ordinal():  # -1: not on a GPU
                 t = t.to(device=device.torch_device(), dtype=dtype.torch)
-            if t.dim() != 1:
-                t = t.reshape(-1)
-            if not t.is_contiguous():
-                t = t.contiguous()
+            if t.dim() != 1 or not t.is_contiguous():
+                t = t.ravel()  # flat and contiguous: a view where it can be
         else:
             arr = np.asarray(data)
             if dtype is None:
@@ -418,7 +414,7 @@ class ConcreteNDArray(NDArray):
             shape = Shape(t.numel())
         elif not isinstance(shape, Shape):
             shape = Shape(shape)
-        if t.numel() != shape.size():
+        if t.numel() != math.prod(shape._d):
             raise IllegalArgumentException(f"data has {t.numel()} elements but shape {shape} needs {shape.size()}")
         self._t = t
         self._shape = shape
@@ -473,7 +469,7 @@ class ConcreteNDArray(NDArray):
         return torch.empty(shape.size(), dtype=dtype.torch, device=self._t.device)
 
     def _stream(self) -> int:
-        return stream_of(self._t.device.index)
+        return stream_of(self._t.get_device())
 
     # ---- accessors ----
     def shape(self) -> Shape:

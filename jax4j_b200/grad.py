@@ -41,7 +41,7 @@ from .tracing import (AxisMeta, CheckpointMeta, CondMeta, Jaxpr, PmapMeta, ScanM
 # constants (Grad.java:841-903)
 # ---------------------------------------------------------------------------
 def _float_or_default(dtype: DType) -> DType:
-    return dtype if dtype.is_floating() else DType.FLOAT32
+    return dtype if dtype._floating else DType.FLOAT32
 
 
 _CONSTS: Dict[tuple, ConcreteNDArray] = {}
@@ -235,7 +235,7 @@ def _evaluate(jaxpr: Jaxpr, args: List[NDArray], keep_for_vjp: bool) -> Dict[int
         raise IllegalArgumentException(f"expected {len(jaxpr.inVars)} arguments, got {len(args)}")
     for v, a in zip(jaxpr.inVars, args):
         values[v.id] = a
-    if len(jaxpr.equations) == 1 and jaxpr.equations[0].primitive == Primitive.FFI_CALL:
+    if len(jaxpr.equations) == 1 and jaxpr.equations[0].primitive is Primitive.FFI_CALL:
         _run_equation(jaxpr.equations[0], values, keep_for_vjp)  # one layer: nothing to plan
         return values
     if FUSION and all(isinstance(a, ConcreteNDArray) for a in values.values()):
@@ -261,7 +261,7 @@ def _evaluate(jaxpr: Jaxpr, args: List[NDArray], keep_for_vjp: bool) -> Dict[int
 
 def _run_equation(eq, values: Dict[int, NDArray], keep_for_vjp: bool = False) -> None:
     inputs = [values[v.id] for v in eq.inputs]
-    if eq.primitive == Primitive.FFI_CALL:
+    if eq.primitive is Primitive.FFI_CALL:
         out = eq.outputs[0].id
         values[out], saved = eq.metadata.run(inputs, keep_for_vjp)
         if saved is not None:
@@ -531,8 +531,9 @@ def _pmap_context():
 
 def do_backward(jaxpr: Jaxpr, values: Dict[int, NDArray], seeds: List[NDArray]) -> List[NDArray]:
     """Grad.doBackward (Grad.java:154-189)."""
-    if (len(jaxpr.equations) == 1 and jaxpr.equations[0].primitive == Primitive.FFI_CALL and len(seeds) == 1
-            and jaxpr.outVars[0].id == jaxpr.equations[0].outputs[0].id and _pmap_context() is None):
+    eqs = jaxpr.equations
+    if (len(eqs) == 1 and eqs[0].primitive is Primitive.FFI_CALL and len(seeds) == 1
+            and jaxpr.outVars[0].id == eqs[0].outputs[0].id and _pmap_context() is None):
         return _layer_backward(jaxpr, values, seeds[0])  # one layer: nothing to walk
     _lazy_scope.depth = getattr(_lazy_scope, "depth", 0) + 1
     try:
@@ -544,9 +545,11 @@ def do_backward(jaxpr: Jaxpr, values: Dict[int, NDArray], seeds: List[NDArray]) 
 def _layer_backward(jaxpr: Jaxpr, values: Dict[int, NDArray], seed: NDArray) -> List[NDArray]:
     """do_backward of a Jaxpr that is one FFI_CALL and its output."""
     eq = jaxpr.equations[0]
-    ids = [v.id for v in jaxpr.inVars]
-    g_ins = eq.metadata.pull([values[v.id] for v in eq.inputs], values[eq.outputs[0].id], values.get(~eq.outputs[0].id),
-                             materialize(seed), [v.id in ids for v in eq.inputs])
+    ids, eq_ids, out = [v.id for v in jaxpr.inVars], [v.id for v in eq.inputs], eq.outputs[0].id
+    g_ins = eq.metadata.pull([values[i] for i in eq_ids], values[out], values.get(~out), materialize(seed),
+                             [i in ids for i in eq_ids])
+    if ids == eq_ids and len(set(ids)) == len(ids):
+        return g_ins  # every argument once, in order: all of them wanted
     grads: Dict[int, NDArray] = {}
     for v, g in zip(eq.inputs, g_ins):
         if g is not None:
@@ -888,7 +891,7 @@ def vjp(fn: Callable, *args: NDArray):
         if len(seeds) != len(outs):
             raise IllegalArgumentException(f"pullback: {len(outs)} outputs take as many cotangents, got {len(seeds)}")
         for s, v in zip(seeds, jaxpr.outVars):
-            if s.shape() != v.shape or s.dtype() != _float_or_default(v.dtype):
+            if s.shape()._d != v.shape._d or s.dtype() is not _float_or_default(v.dtype):
                 raise IllegalArgumentException(f"pullback: cotangent {s.shape()} {s.dtype()} of an output {v.shape} "
                                                f"{v.dtype}")
         return do_backward(jaxpr, values, list(seeds))

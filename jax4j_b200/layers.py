@@ -18,7 +18,7 @@ import torch
 from . import _lib
 from ._lib import call
 from .core import (ConcreteNDArray, DType, IllegalArgumentException, NDArray, Shape, UnsupportedOperationException,
-                   _make_splits, _split_of)
+                   _make_splits, _split_of, stream_of)
 from .tracing import FfiMeta
 
 # J4C_ACT_* (include/jax4j_cuda.h)
@@ -168,22 +168,25 @@ def _small(M: int, K: int, N: int) -> bool:
 
 def dense(x: NDArray, w: NDArray, bias: Optional[NDArray], activation: Optional[str],
           residual: Optional[NDArray]) -> NDArray:
-    xd, wd = x.shape()._d, w.shape()._d
-    act = activation_code(activation)
+    xd, wd, dt = x.shape()._d, w.shape()._d, x.dtype()
+    act = ACTIVATIONS.get(activation)
+    if act is None:
+        act = activation_code(activation)
     if len(xd) < 1 or len(wd) != 2:
         raise IllegalArgumentException(f"dense takes [..., K] and a weight [K, N], got {x.shape()} and {w.shape()}")
     if xd[-1] != wd[0]:
         raise IllegalArgumentException(f"dense: inner dimensions differ ({x.shape()} . {w.shape()})")
-    _floating("dense", x, (w, bias, residual))
-    out = xd[:-1] + wd[1:]
+    if (not dt._floating or w.dtype() is not dt or bias is not None and bias.dtype() is not dt
+            or residual is not None and residual.dtype() is not dt):
+        _floating("dense", x, (w, bias, residual))
     inputs = [x, w]
     if bias is not None:
         if bias.shape()._d != wd[1:]:
             raise IllegalArgumentException(f"dense: bias is {bias.shape()}, the outputs are [{wd[1]}]")
         inputs.append(bias)
     if residual is not None:
-        if residual.shape()._d != out:
-            raise IllegalArgumentException(f"dense: residual is {residual.shape()}, the output {Shape(out)}")
+        if residual.shape()._d != xd[:-1] + wd[1:]:
+            raise IllegalArgumentException(f"dense: residual is {residual.shape()}, the output {Shape(xd[:-1] + wd[1:])}")
         inputs.append(residual)
     return _dense_meta(bias is not None, residual is not None, act).run(inputs, False)[0]
 
@@ -195,6 +198,12 @@ def _split_product(a, a_kind: str, b, b_kind: str, M: int, K: int, N: int, bias,
     (ah, al), (bh, bl) = _split_of(a, a_kind), _split_of(b, b_kind)
     call("j4c_dot_split_act", ah.data_ptr(), al.data_ptr(), bh.data_ptr(), bl.data_ptr(), M, K, N, bias, act, residual, z,
          out.data_ptr(), stream)
+
+
+@functools.lru_cache(maxsize=4096)
+def _grad_workspace(gpu: int, dtype: int, M: int, N: int) -> int:
+    """j4c_dense_grad_workspace on this GPU (the current one)."""
+    return int(_lib.lib().j4c_dense_grad_workspace(dtype, M, N))
 
 
 class _Dense(FfiMeta):
@@ -212,10 +221,7 @@ class _Dense(FfiMeta):
     @staticmethod
     def _extents(inputs):
         K, N = inputs[1]._shape._d
-        M = 1
-        for n in inputs[0]._shape._d[:-1]:
-            M *= n
-        return M, K, N
+        return math.prod(inputs[0]._shape._d[:-1]), K, N
 
     # The output tells the slope (and is kept anyway) unless a residual was
     # added to it or the activation is not monotone.
@@ -229,15 +235,15 @@ class _Dense(FfiMeta):
         M, K, N = self._extents(inputs)
         dt, t = x._dtype, x._t
         stream = x._stream()
-        x2 = x if x._shape.rank() == 2 else x.reshape(Shape(M, K))
+        x2 = x if len(x._shape._d) == 2 else x.reshape(Shape(M, K))
         out_shape = Shape(x._shape._d[:-1] + (N,))
         keep_z = keep and self.act and not self._from_output()
-        y = torch.empty(M * N, dtype=t.dtype, device=t.device)
-        z = torch.empty(M * N, dtype=t.dtype, device=t.device) if keep_z else None
+        y = t.new_empty(M * N)
+        z = t.new_empty(M * N) if keep_z else None
         bp = bias._t.data_ptr() if bias is not None else None
         rp = residual._t.data_ptr() if residual is not None else None
         zp = z.data_ptr() if z is not None else None
-        if dt != DType.FLOAT32 or M <= FEW_ROWS or _small(M, K, N):
+        if dt is not DType.FLOAT32 or M <= FEW_ROWS or _small(M, K, N):
             call("j4c_dot_act", dt.ordinal, t.data_ptr(), w._t.data_ptr(), M, K, N, 0, 0, bp, self.act, rp, zp, y.data_ptr(),
                  stream)
         else:
@@ -250,17 +256,18 @@ class _Dense(FfiMeta):
     def vjp(self, inputs, out, saved, g, wanted):
         x, w = inputs[0], inputs[1]
         x2, z = saved
-        M, K, N = self._extents(inputs)
+        (M, K), N = x2._shape._d, w._shape._d[1]
         dt, t, dev = x._dtype, g._t, g._device
-        stream = g._stream()
+        gpu = t.get_device()
+        stream = stream_of(gpu)
         want_bias = self.has_bias and wanted[2]
         products = wanted[0] or wanted[1]
-        small = dt != DType.FLOAT32 or _small(M, K, N)
+        small = dt is not DType.FLOAT32 or _small(M, K, N)
         dz, dbias, lines = t, None, None
         grads: List[Optional[ConcreteNDArray]] = [None, None]
         if want_bias or products:
             # the pass over g, and without splits all of the gradient
-            need = _lib.lib().j4c_dense_grad_workspace(dt.ordinal, M, N) if want_bias else 0
+            need = _grad_workspace(gpu, dt.ordinal, M, N) if want_bias else 0
             ws = torch.empty(need, dtype=torch.uint8, device=t.device) if need else None
             wp = ws.data_ptr() if need else None
             if self.act:

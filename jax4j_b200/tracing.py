@@ -91,9 +91,9 @@ class FfiMeta:
 
     def record(self, inputs) -> "TracedNDArray":
         tracer = Tracer.current()
-        in_vars = [to_var(x) for x in inputs]
+        in_vars = [x._var if type(x) is TracedNDArray else to_var(x) for x in inputs]
         out = tracer.nextVar(self.outShape(inputs), in_vars[0].dtype)
-        tracer.addEquation(Equation(in_vars, [out], Primitive.FFI_CALL, self))
+        tracer.equations.append(Equation(in_vars, [out], Primitive.FFI_CALL, self))
         return TracedNDArray(out)
 
     def pull(self, inputs, out, saved, g, wanted):
@@ -150,6 +150,9 @@ class Jaxpr:
 # ---------------------------------------------------------------------------
 # Tracer (tracing/Tracer.java)
 # ---------------------------------------------------------------------------
+_new_var = tuple.__new__  # Var(...) without the named tuple's own __new__
+
+
 class _Stack(threading.local):
     def __init__(self):
         self.stack: List["Tracer"] = []
@@ -184,7 +187,7 @@ class Tracer:
         _stack.stack.pop()
 
     def nextVar(self, shape: Shape, dtype: DType) -> Var:
-        return Var(next(self._counter), shape, dtype)
+        return _new_var(Var, (next(self._counter), shape, dtype))
 
     def nextConstant(self, value: NDArray) -> Var:
         v = self.nextVar(value.shape(), value.dtype())
