@@ -152,10 +152,20 @@ class _GroupNorm(FfiMeta):
 # ---------------------------------------------------------------------------
 # FLOAT64 products, and FLOAT32 ones of at most this many multiply-adds, run
 # straight from their arrays (j4c_dot_act); the FLOAT32 product on the tcgen05
-# tensor cores first splits both operands (five launches more), which larger ones
-# win back: forward of [1024,1024]x[1024,512] 48 against 62 us, with gradients 152
-# against 170; of [1024,1024]x[1024,1024] 89 against 60 and 270 against 169.
+# tensor cores first splits both operands (three launches more forward), which
+# larger ones win back: forward of [1024,1024]x[1024,512] 48 against 60 us, with
+# gradients 153 against 167; of [1024,1024]x[1024,1024] 89 against 60 and 270
+# against 169.
 SMALL_PRODUCT = 1 << 29
+
+# The CUDA cores' tiles have 64 columns whether they hold outputs or not, so these
+# count: [8192,4096]x[4096,10] takes 162 us there and 107 on the tensor cores, with
+# gradients 474 and 333.  Not where a sum is longer than this, which the tensor
+# cores cut into four parts at most: [512,65536]x[65536,10] 200 against 365 us
+# ([16384,2048]x[2048,10] 165 against 114, [1024,32768]x[32768,10] 201 against 241
+# and with gradients 552 against 425).
+TILE_COLUMNS = 64
+LONG_SUM = 1 << 15
 
 # As many rows or fewer run there whatever the weight's size: they are bound by
 # reading it once, which the splits read, write and read again.
@@ -163,7 +173,9 @@ FEW_ROWS = 16
 
 
 def _small(M: int, K: int, N: int) -> bool:
-    return M * K * N <= SMALL_PRODUCT or not (M and N and K)
+    if M * K * (-(-N // TILE_COLUMNS) * TILE_COLUMNS) <= SMALL_PRODUCT:
+        return True
+    return not (M and N and K) or M * K * N <= SMALL_PRODUCT and max(M, K, N) > LONG_SUM
 
 
 def dense(x: NDArray, w: NDArray, bias: Optional[NDArray], activation: Optional[str],

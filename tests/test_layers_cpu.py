@@ -160,3 +160,14 @@ def test_interpretation_inside_a_trace_is_recorded_and_gradients_refused(monkeyp
     monkeypatch.setattr(grad, "ones", lambda s, dtype, device=None: leaf(*s.dimensions()))
     with pytest.raises(J.UnsupportedOperationException, match="inside a trace"):
         J.JAX.make_jaxpr(lambda a: J.JAX.grad(f)(a), leaf(*shape))
+
+
+def test_which_products_run_straight_from_their_arrays():
+    """Whole tiles of 64 columns count, except where a sum is long."""
+    from jax4j_b200 import layers
+    for shape in ((1024, 1024, 512), (256, 784, 512), (8192, 1024, 10), (2048, 4096, 64), (64, 1000000, 8),
+                  (1000000, 8, 8), (512, 65536, 10), (0, 1 << 20, 1 << 20), (1 << 20, 0, 1 << 20), (1 << 20, 1 << 20, 0)):
+        assert layers._small(*shape), shape
+    for shape in ((1025, 1024, 512), (8192, 4096, 10), (16384, 2048, 10), (8192, 4096, 1), (4096, 4096, 30),
+                  (64, 1000000, 9)):
+        assert not layers._small(*shape), shape
