@@ -381,12 +381,10 @@ int ranks_for(int64_t tiles, int64_t K) {
 
 // Parts of a sum of K terms whose `ctas` CTAs have `adders` threads after one
 // another along K: so many that no thread adds more than kMaxTerms of them in a
-// row.  Each addition in FP32 loses up to half a step of the running sum, so the
-// error grows with the row: the weight's gradient of [4000000,8]x[8,8], values of
-// one sign, came out 1.4e-5 off from the 16 CTAs of one cluster (250000 terms a
-// thread) and 8e-8 in parts, and forward and gradients take 3.1 ms instead of
-// 13.6.  FLOAT64 has the digits to spare; there parts only fill idle SMs.
-constexpr int64_t kMaxTerms = 1024;
+// row.  The weight's gradient of [4000000,8]x[8,8], values of one sign, came out
+// 1.4e-5 off from the 16 CTAs of one cluster (250000 terms a thread) and 8e-8 in
+// parts, and forward and gradients take 3.1 ms instead of 13.6.  FLOAT64 has the
+// digits to spare; there parts only fill idle SMs.
 template <typename T>
 int64_t parts_for(int64_t ctas, int64_t adders, int64_t K) {
     int64_t parts = std::min<int64_t>(ceil_div(K, adders * kMaxTerms), 65535);
@@ -607,12 +605,14 @@ __global__ void __launch_bounds__(256, 4) dense_grad_kernel(const GradArgs<T> a)
 
 // Groups of rows: four CTAs an SM (64 registers a thread, one row of a warp in
 // flight: [8192,4096] gelu 68 us, 5.9 TB/s; two rows in flight and two CTAs an SM
-// 75) and no more, at least 32 rows each; where eight are enough for that, or for
-// 512 rows, they are a cluster and need no second launch.
+// 75) and no more unless a warp had more than kMaxTerms rows, at least 32 rows
+// each; where eight are enough for that, or for 512 rows, they are a cluster and
+// need no second launch.
 int64_t grad_groups(int64_t M, int64_t N) {
     const int64_t groups = std::max<int64_t>(
         1, std::min(ceil_div(M, 32), (int64_t)sm_count() * 4 / ceil_div(N, 256)));
-    return M <= 512 ? std::min<int64_t>(groups, 8) : groups;
+    if (M <= 512) return std::min<int64_t>(groups, 8);
+    return std::max(groups, std::min<int64_t>(ceil_div(M, 8 * kMaxTerms), 65535));
 }
 
 template <typename T>

@@ -331,7 +331,11 @@ held_backward_kernel(const Args<T> a, int64_t nb) {
         if (on)
             for (int c = t; c < a.D; c += H::THREADS) {
                 T v = T(0);
-                for (int s = 0; s < a.S; s++) v += buf[s * a.D + c];
+                for (int s0 = 0; s0 < a.S; s0 += 64) {  // up to 8192 positions: 64 at a time
+                    T w = T(0);
+                    for (int s = s0; s < min((int)a.S, s0 + 64); s++) w += buf[s * a.D + c];
+                    v += w;
+                }
                 a.dpart[((int64_t)which * nb + k / a.G) * a.C + g * a.D + c] = v;
             }
         __syncthreads();
@@ -772,12 +776,13 @@ int held_warps(int64_t n) {
     return warps;
 }
 
-// Backward, the sets that share a group's samples: as many as are resident, no
-// more than samples.
+// Backward, the sets that share a group's samples: as many as are resident, more
+// where one would add more than kMaxTerms of them, no more than samples.
 template <typename T, int V>
 int64_t held_sets(int64_t B, int64_t G, int warps) {
     const int cta = std::max(8, warps);
-    return std::min(B, std::max<int64_t>(1, ceil_div((int64_t)sm_count() * (kResident<T, V, true> / 32 / cta) * (cta / warps), G)));
+    const int64_t resident = (int64_t)sm_count() * (kResident<T, V, true> / 32 / cta) * (cta / warps);
+    return std::min(B, std::max(ceil_div(resident, G), ceil_div(B, kMaxTerms)));
 }
 
 template <typename T>

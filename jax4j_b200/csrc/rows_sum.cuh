@@ -6,6 +6,11 @@
 namespace j4c {
 namespace {
 
+// Additions in a row that a thread makes at most, where a sum may be long.  Each
+// in FP32 loses up to half a step of the running sum, so the error grows with the
+// row; cut rows' sums are added after them.
+constexpr int64_t kMaxTerms = 1024;
+
 template <typename T>
 __device__ __forceinline__ T warp_sum(T v) {
 #pragma unroll
