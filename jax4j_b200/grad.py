@@ -548,8 +548,6 @@ def _layer_backward(jaxpr: Jaxpr, values: Dict[int, NDArray], seed: NDArray) -> 
     ids, eq_ids, out = [v.id for v in jaxpr.inVars], [v.id for v in eq.inputs], eq.outputs[0].id
     g_ins = eq.metadata.pull([values[i] for i in eq_ids], values[out], values.get(~out), materialize(seed),
                              [i in ids for i in eq_ids])
-    if ids == eq_ids and len(set(ids)) == len(ids):
-        return g_ins  # every argument once, in order: all of them wanted
     grads: Dict[int, NDArray] = {}
     for v, g in zip(eq.inputs, g_ins):
         if g is not None:
@@ -884,19 +882,44 @@ def vjp(fn: Callable, *args: NDArray):
     if Tracer.current() is not None:
         raise UnsupportedOperationException("JAX.vjp inside a trace")
     jaxpr = make_jaxpr(fn, *args)
+    eqs, tuple_out = jaxpr.equations, jaxpr.__dict__.get("_tuple_out")
+    if (len(eqs) == 1 and eqs[0].primitive is Primitive.FFI_CALL and not tuple_out and not jaxpr.consts
+            and [v.id for v in eqs[0].inputs] == [v.id for v in jaxpr.inVars] and jaxpr.outVars[0] is eqs[0].outputs[0]):
+        return _layer_vjp(jaxpr, list(args))
     values = fill_forward_values(jaxpr, list(args))
     outs = [values[v.id] for v in jaxpr.outVars]
 
     def pullback(*seeds: NDArray) -> List[NDArray]:
-        if len(seeds) != len(outs):
-            raise IllegalArgumentException(f"pullback: {len(outs)} outputs take as many cotangents, got {len(seeds)}")
-        for s, v in zip(seeds, jaxpr.outVars):
-            if s.shape()._d != v.shape._d or s.dtype() is not _float_or_default(v.dtype):
-                raise IllegalArgumentException(f"pullback: cotangent {s.shape()} {s.dtype()} of an output {v.shape} "
-                                               f"{v.dtype}")
+        _check_seeds(jaxpr, seeds)
         return do_backward(jaxpr, values, list(seeds))
 
-    return (tuple(outs) if jaxpr.__dict__.get("_tuple_out") else outs[0]), pullback
+    return (tuple(outs) if tuple_out else outs[0]), pullback
+
+
+def _check_seeds(jaxpr: Jaxpr, seeds) -> None:
+    if len(seeds) != len(jaxpr.outVars):
+        raise IllegalArgumentException(f"pullback: {len(jaxpr.outVars)} outputs take as many cotangents, got {len(seeds)}")
+    for s, v in zip(seeds, jaxpr.outVars):
+        if s.shape()._d != v.shape._d or s.dtype() is not _float_or_default(v.dtype):
+            raise IllegalArgumentException(f"pullback: cotangent {s.shape()} {s.dtype()} of an output {v.shape} {v.dtype}")
+
+
+def _layer_vjp(jaxpr: Jaxpr, args: List[NDArray]):
+    """vjp of a Jaxpr that is one FFI_CALL of its arguments, each once and in
+    order: the layer's own forward and VJP, with no maps of values."""
+    eq = jaxpr.equations[0]
+    out, saved = eq.metadata.forward(args, True)
+    wanted = [True] * len(args)
+
+    def pullback(*seeds: NDArray) -> List[NDArray]:
+        _check_seeds(jaxpr, seeds)
+        if _pmap_context() is not None:  # there the walk notes when each gradient is complete
+            values = dict(zip([v.id for v in eq.inputs], args))
+            values[eq.outputs[0].id], values[~eq.outputs[0].id] = out, saved
+            return do_backward(jaxpr, values, list(seeds))
+        return eq.metadata.pull(args, out, saved, materialize(seeds[0]), wanted)
+
+    return out, pullback
 
 
 def _trace_tree(fn: Callable, tree, leaves: List[NDArray]) -> Jaxpr:

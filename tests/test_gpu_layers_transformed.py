@@ -109,3 +109,54 @@ def test_cond_takes_the_branch_and_its_gradient(J, name):
         np.testing.assert_array_equal(J.JAX.jit(net)(x).numpy(), branch(x).numpy())
         np.testing.assert_array_equal(J.JAX.grad(lambda a: net(a).tanh().sum())(x).numpy(),  # noqa: B023
                                       J.JAX.grad(lambda a: branch(a).tanh().sum())(x).numpy())  # noqa: B023
+
+
+@pytest.mark.parametrize("name", ["dense", "group norm"])
+def test_vjp_of_a_layer(J, name):
+    """JAX.vjp of one layer -- its arguments once and in order, in another order,
+    one of them twice, a closed-over weight, two outputs, an argument left out --
+    against the gradient of the same loss; and inside a pmap."""
+    r = np.random.default_rng(9)
+    x, w = r.standard_normal((8, 32)).astype(np.float32), (r.standard_normal((32, 32)) / 6).astype(np.float32)
+    v, dy = r.standard_normal(32).astype(np.float32), r.standard_normal((8, 32)).astype(np.float32)
+    X, W, V, DY = (arr(J, a) for a in (x, w, v, dy))
+    if name == "dense":
+        f, args = (lambda a, b, c: J.Nn.dense(a, b, c, "silu")), (X, W, V)
+    else:
+        f, args = (lambda a, b, c: J.Nn.groupNorm(a, 4, b, c, activation="silu")), (X, V, V)
+
+    def grads_of(fn, *at):  # through a longer Jaxpr
+        return J.JAX.vjp(lambda *a: fn(*a).mul(DY).sum(), *at)[1](J.ConcreteNDArray.scalar(1.0))
+
+    y, pull = J.JAX.vjp(f, *args)
+    np.testing.assert_array_equal(y.numpy(), f(*args).numpy())
+    want = [g.numpy() for g in grads_of(f, *args)]
+    for _ in range(2):
+        for g, e in zip(pull(DY), want):
+            np.testing.assert_array_equal(g.numpy(), e)
+    swapped = J.JAX.vjp(lambda c, b, a: f(a, b, c), *args[::-1])[1](DY)
+    for g, e in zip(swapped, want[::-1]):
+        np.testing.assert_array_equal(g.numpy(), e)
+    np.testing.assert_array_equal(J.JAX.vjp(lambda a: f(a, *args[1:]), X)[1](DY)[0].numpy(), want[0])
+    extra = J.JAX.vjp(lambda a, q, b, c: f(a, b, c), X, DY, *args[1:])[1](DY)
+    assert not extra[1].numpy().any()
+    np.testing.assert_array_equal(extra[2].numpy(), want[1])
+    two, pull2 = J.JAX.vjp(lambda a, b, c: (f(a, b, c), a), *args)
+    np.testing.assert_array_equal(two[1].numpy(), x)
+    np.testing.assert_array_equal(pull2(DY, DY)[0].numpy(), (want[0] + dy))
+    if name == "dense":
+        twice = J.JAX.vjp(lambda a, b: J.Nn.dense(a, b, None, "silu", a), X, W)[1](DY)
+        res = J.JAX.vjp(lambda a, b, c: J.Nn.dense(a, b, None, "silu", c), X, W, X)[1](DY)
+        np.testing.assert_array_equal(twice[0].numpy(), res[0].numpy() + res[2].numpy())
+        np.testing.assert_array_equal(twice[1].numpy(), res[1].numpy())
+    for bad in ((), (X, X), (V,)):
+        with pytest.raises(J.IllegalArgumentException, match="cotangent"):
+            pull(*bad)
+
+    def body(xs):
+        local = [J.ConcreteNDArray(a.tensor(), a.shape()).to(xs.device()) for a in args[1:]]
+        d = J.ConcreteNDArray(DY.tensor(), DY.shape()).to(xs.device())
+        return J.Lax.psum(J.JAX.vjp(f, xs, *local)[1](d)[1])
+
+    both = J.JAX.pmap(body, [J.Device(None), J.Device(None)])(arr(J, np.stack([x, x]))).numpy()
+    np.testing.assert_array_equal(both, np.stack([want[1] + want[1]] * 2))
