@@ -64,9 +64,10 @@ def group_norm(x: NDArray, groups: int, gamma: Optional[NDArray], beta: Optional
         raise IllegalArgumentException(f"groupNorm takes [batch, ..., channels], got {x.shape()}")
     C = d[-1]
     _floating("groupNorm", x, (gamma, beta))
-    groups = int(groups)
-    if groups < 1 or C < 1 or C % groups:
+    whole = int(groups)
+    if whole != groups or whole < 1 or C < 1 or C % whole:
         raise IllegalArgumentException(f"groupNorm: {C} channels do not divide into {groups} groups")
+    groups = whole
     for name, p in (("gamma", gamma), ("beta", beta)):
         if p is not None and p.shape().dimensions() != (C,):
             raise IllegalArgumentException(f"groupNorm: {name} is {p.shape()}, the channels are [{C}]")

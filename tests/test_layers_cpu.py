@@ -171,3 +171,12 @@ def test_which_products_run_straight_from_their_arrays():
     for shape in ((1025, 1024, 512), (8192, 4096, 10), (16384, 2048, 10), (8192, 4096, 1), (4096, 4096, 30),
                   (64, 1000000, 9)):
         assert not layers._small(*shape), shape
+
+
+def test_group_norm_refuses_half_a_group():
+    x = leaf(2, 3, 8)
+    for groups in (2.5, 0.5, 1.999):
+        with pytest.raises(J.IllegalArgumentException, match="do not divide"):
+            J.Nn.groupNorm(x, groups)
+    jaxpr = J.JAX.make_jaxpr(lambda a: J.Nn.groupNorm(a, 2.0), x)  # a whole number of another type is one
+    assert "group_norm(groups=2," in repr(jaxpr)
