@@ -556,8 +556,10 @@ class Nn:
               residual: Optional[NDArray] = None) -> NDArray:
         """act(x . w + bias) + residual as one operation: x [..., K], w [K, N],
         bias [N], residual like the output [..., N]; FLOAT32 or FLOAT64,
-        reverse-mode differentiable in all four.  Bias, activation and residual
-        are applied in the product's store; activations as for groupNorm."""
+        reverse-mode differentiable in all four (JAX.jvp refuses it; JAX.vmap
+        takes a batched x, and a batched residual with it).  Bias, activation
+        and residual are applied in the product's store; activations as for
+        groupNorm."""
         return _layers.dense(x, w, bias, activation, residual)
 
     @staticmethod
@@ -567,7 +569,8 @@ class Nn:
         over each sample's groups of neighbouring channels; x is [batch, ...,
         channels], channels last, FLOAT32 or FLOAT64 (groups = 1 over
         [batch, channels] is layer norm), gamma and beta [channels].  One
-        operation, reverse-mode differentiable in x, gamma and beta.
+        operation, reverse-mode differentiable in x, gamma and beta (JAX.jvp
+        refuses it; JAX.vmap takes a batched x).
         activation: "none", "relu", "tanh", "sigmoid", "silu" or "gelu" (the
         tanh form)."""
         return _layers.group_norm(x, groups, gamma, beta, eps, activation)

@@ -21,9 +21,9 @@ bool tc_gemm_supported(int64_t M, int64_t K, int64_t N);
 namespace {
 
 // ---- products straight from the arrays --------------------------------------------------------
-// A FLOAT32 product too small for the tcgen05 kernel's splits to pay (each
-// operand is read and written twice before the first MMA, eight launches in
-// all) runs here in one launch of FP32 FMAs, and every FLOAT64 product with the
+// A FLOAT32 product too small for the tcgen05 kernel's splits to pay (before the
+// first MMA the operands are read, once or twice, and written as halves; four
+// launches in all) runs here in one launch of FP32 FMAs, and every FLOAT64 product with the
 // FP64 tensor instruction (tcgen05 has no FP64 kind).  K is cut over a cluster
 // of CTAs so that few output tiles still fill the GPU; their partial sums meet
 // through distributed shared memory and are added in rank order.  A sum too long
@@ -157,8 +157,8 @@ __global__ void __launch_bounds__(kRowsThreads) rows_kernel(const Product<T> p) 
 // FLOAT32: 8 x 4 results a thread.  FLOAT64: a warp has a quarter of the tile as
 // 4 x 4 tiles of m8n8k4 (A element: row lane / 4, k lane % 4; B: k lane % 4,
 // column lane / 4; results: row lane / 4, columns 2 (lane % 4) and the next).
-// FLOAT32 [256,784]x[784,512] takes 16 us, [1024,1024]x[1024,512] 45; FLOAT64 15
-// and, at 2048^3, 572 us (30 TFLOP/s).  Also measured, and no faster in FLOAT32:
+// FLOAT32 [256,784]x[784,512] takes 18 us, [1024,1024]x[1024,512] 47; FLOAT64 18
+// and, at 2048^3, 592 us (29 TFLOP/s).  Also measured, and no faster in FLOAT32:
 // rings of four and six buffers, 8 x 8 results a thread, and two or four shares
 // of K within a CTA; in FLOAT64 FMAs instead of the tensor instruction: 22 and
 // 1021 us.

@@ -1842,7 +1842,7 @@ size_t tail_scratch_bound(int64_t m, int64_t n, int64_t batch) {
 // pair goes through 1000 K in 19.5 and 14.7 (a tile of half the width reads its A
 // as often), and joining the parts of a split tile takes 4.25 a part of 256
 // columns.  Narrow tiles win where wide ones are split for want of tiles
-// ([1024,1024]x[1024,1024] with gelu, residual and pre-activation 37 -> 29 us) or
+// ([1024,1024]x[1024,1024] with gelu, residual and pre-activation 37 -> 28 us) or
 // end in a wave of few (153 of them at [4099,1000]x[1000,2050]: 131 -> 114 us),
 // and lose elsewhere (4096^3: 287 -> 421 us).
 template <int BN, int STAGES>

@@ -185,7 +185,10 @@ class Optim:
         in the leaf's dtype, each product and sum rounded on its own.  lr is a
         number or a FLOAT32 array of one element on the GPU (a schedule that a
         recorded step can follow); weightDecay a number or one per leaf, in
-        PyTrees.flatten order; scale e.g. 1/D for summed gradients."""
+        PyTrees.flatten order; scale e.g. 1/D for summed gradients.
+
+        The new parameters of a dtype are views of one allocation, and so are
+        the new moments: a leaf that is kept alone keeps the memory of all."""
         if Tracer.current() is not None:
             raise UnsupportedOperationException("Optim.adamW is a step between traces, not part of one")
         pl, gl = PyTrees.flatten(params), PyTrees.flatten(grads)
