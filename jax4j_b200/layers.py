@@ -74,7 +74,7 @@ def group_norm(x: NDArray, groups: int, gamma: Optional[NDArray], beta: Optional
     if not eps >= 0.0:
         raise IllegalArgumentException(f"groupNorm: eps is not negative, got {eps}")
     inputs = [x] + [p for p in (gamma, beta) if p is not None]
-    return _GroupNorm(groups, gamma is not None, beta is not None, float(eps), act).run(inputs, False)[0]
+    return _GroupNorm(groups, gamma is not None, beta is not None, float(eps), act).apply(inputs)
 
 
 class _GroupNorm(FfiMeta):
@@ -201,7 +201,7 @@ def dense(x: NDArray, w: NDArray, bias: Optional[NDArray], activation: Optional[
         if residual.shape()._d != xd[:-1] + wd[1:]:
             raise IllegalArgumentException(f"dense: residual is {residual.shape()}, the output {Shape(xd[:-1] + wd[1:])}")
         inputs.append(residual)
-    return _dense_meta(bias is not None, residual is not None, act).run(inputs, False)[0]
+    return _dense_meta(bias is not None, residual is not None, act).apply(inputs)
 
 
 def _split_product(a, a_kind: str, b, b_kind: str, M: int, K: int, N: int, bias, act: int, residual, z, out: torch.Tensor,

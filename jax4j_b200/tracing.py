@@ -79,13 +79,20 @@ class FfiMeta:
     batch(inputs, batched, batch): the function over a leading axis of the
     batched inputs (JAX.vmap).
 
-    A transformation calls run and pull, which under a trace record the call
-    (as any other operation's interpretation there records it) and refuse."""
+    The user's entry calls apply, which records under a trace.  Transformations
+    call run and pull: on traced values the one records (as any other operation
+    interpreted inside a trace) and the other refuses; concrete ones are
+    computed, inside a trace too."""
 
     name = "?"
 
-    def run(self, inputs, keep):
+    def apply(self, inputs):
         if Tracer.current() is not None:
+            return self.record(inputs)
+        return self.forward(inputs, False)[0]
+
+    def run(self, inputs, keep):
+        if Tracer.current() is not None and any(type(x) is TracedNDArray for x in inputs):
             return self.record(inputs), None
         return self.forward(inputs, keep)
 
@@ -97,7 +104,7 @@ class FfiMeta:
         return TracedNDArray(out)
 
     def pull(self, inputs, out, saved, g, wanted):
-        if Tracer.current() is not None:
+        if Tracer.current() is not None and (type(g) is TracedNDArray or any(type(x) is TracedNDArray for x in inputs)):
             raise UnsupportedOperationException(f"the gradient of {self.name} cannot be taken inside a trace")
         return self.vjp(inputs, out, saved, g, wanted)
 

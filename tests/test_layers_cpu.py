@@ -180,3 +180,28 @@ def test_group_norm_refuses_half_a_group():
             J.Nn.groupNorm(x, groups)
     jaxpr = J.JAX.make_jaxpr(lambda a: J.Nn.groupNorm(a, 2.0), x)  # a whole number of another type is one
     assert "group_norm(groups=2," in repr(jaxpr)
+
+
+def test_concrete_values_inside_a_trace_are_computed(monkeypatch):
+    """A Jaxpr interpreted on closed-over arrays inside a trace gives arrays, and
+    its gradient too; the layers' own entries record."""
+    from jax4j_b200 import grad, layers
+    done = []
+    monkeypatch.setattr(layers, "call", lambda name, *a: done.append(name))
+    monkeypatch.setattr(layers, "stream_of", lambda gpu: 0)
+    monkeypatch.setattr(J.ConcreteNDArray, "_stream", lambda self: 0)
+    monkeypatch.setattr(layers, "_grad_workspace", lambda *a: 0)
+    x = leaf(4, 8)
+    w, g = leaf(8, 5).to(x.device()), leaf(4, 5).to(x.device())
+    inner = J.JAX.make_jaxpr(lambda a: J.Nn.dense(a, w, None, "tanh"), x)
+    seen = []
+
+    def outer(a):
+        seen.append(grad.forward_interpret(inner, [x])[0])
+        seen.append(grad.backward_interpret(inner, [x], [g])[0])
+        return J.Nn.dense(x, w)  # recorded, of two constants
+
+    jaxpr = J.JAX.make_jaxpr(outer, leaf(1))
+    assert all(isinstance(s, J.ConcreteNDArray) for s in seen) and [s.shape() for s in seen] == [J.Shape(4, 5), J.Shape(4, 8)]
+    assert done == ["j4c_dot_act", "j4c_dot_act", "j4c_dense_backward"]
+    assert [e.primitive for e in jaxpr.equations] == [J.Primitive.FFI_CALL]
